@@ -11,7 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
-from ctypes import c_float, c_int, c_longlong, c_void_p
+from ctypes import c_double, c_float, c_int, c_longlong, c_void_p
 
 import torch
 
@@ -128,6 +128,22 @@ def stream() -> c_void_p:
     if _raw_stream is not None:
         return c_void_p(_raw_stream(torch.cuda.current_device()))
     return c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+class _Here:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is the current one (free of cost when it already is)."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def status_word(device: torch.device | None = None) -> torch.Tensor:
@@ -250,5 +266,8 @@ def _declare(l: ctypes.CDLL) -> None:
     sig("ob_fp8_delayed_update", [P, I, I, I, F, I, P])
     sig("ob_attn_decode", [P, L, P, P, L, P, P, L, L, L, P, P, L, P, P, I, I, I, I, I, I, F, I, P])
     sig("ob_sample", [P, I, L, I, I, F, I, F, I, ctypes.c_uint64, ctypes.c_uint64, P, P])
+    D = c_double
+    sig("ob_logprobs_fwd", [P, L, I, P, P, P, P, P, P, I, I, I, D, P])
+    sig("ob_logprobs_bwd", [P, L, I, P, P, P, P, P, P, L, I, I, D, P])
     sig("ob_embedding_push", [P, I, P, I, I, I, PP, I, I, P])
     sig("ob_rs_sum", [PP, I, I, I, P, I, I, L, P, L, P, L, I, P, P])

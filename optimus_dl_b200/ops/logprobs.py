@@ -1,0 +1,231 @@
+"""Log probabilities of given tokens, with entropy and the most likely alternatives.
+
+For a row of logits ``z`` over ``V`` tokens, a token ``t`` and a temperature ``T``::
+
+    log p_j = z_j / T - log sum_i exp(z_i / T)
+    logp    = log p_t            entropy = - sum_j p_j log p_j            top = the k largest log p_j
+
+``token_logprobs`` reads the logits once (``csrc/logprobs.cu``) and is differentiable in ``logp`` and ``entropy``;
+``linear_token_logprobs`` does the same for a head projection without holding all logits. Both have PyTorch
+statements with the same semantics for CPU runs and tests. The reference scores with ``log_softmax`` over whole
+``[batch, tokens, vocab]`` logits (optimus_dl/modules/eval/model.py:69-165).
+
+Rules, the same on every path:
+
+* a token id outside ``[0, V)`` (such as the criterion's ignore index) marks a position without a token: its log
+  probability is 0 and it gets no gradient; entropy and alternatives do not depend on the token;
+* a banned token (logit ``-inf``) has probability 0 and adds nothing to the entropy; a row with nothing but banned
+  tokens has log probabilities of ``-inf``, entropy 0 and no gradient;
+* alternatives are ordered by logit, equal ones by lowest id;
+* a row with a NaN or ``+inf`` gives NaN; NaN counts as the largest logit among the alternatives.
+"""
+
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+
+import torch
+import torch.nn.functional as F
+
+from . import _lib, gemm
+
+MAX_TOP_K = 32
+_KERNEL_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+@dataclass
+class TokenLogprobs:
+    logp: torch.Tensor                 # log p(token), fp32, shape of the tokens
+    entropy: torch.Tensor              # entropy of the row's distribution in nats, fp32, same shape
+    top_logp: torch.Tensor | None      # [..., k] log probabilities of the k most likely tokens, most likely first
+    top_ids: torch.Tensor | None       # [..., k] their ids, int64
+
+
+def _check(rows_shape: torch.Size, vocab: int, floating: torch.Tensor, targets: torch.Tensor, top_k: int,
+           temperature: float) -> None:
+    if not floating.is_floating_point():
+        raise TypeError(f"logits must be floating point, got {floating.dtype}")
+    if targets.is_floating_point() or targets.is_complex() or targets.dtype == torch.bool:
+        raise TypeError(f"targets must be token ids of an integer type, got {targets.dtype}")
+    if targets.shape != rows_shape:
+        raise ValueError(f"targets have shape {tuple(targets.shape)}, the rows of logits {tuple(rows_shape)}")
+    if targets.device != floating.device:
+        raise ValueError(f"targets are on {targets.device}, logits on {floating.device}")
+    if vocab < 1:
+        raise ValueError("logits need at least one token")
+    if not 0 <= top_k <= min(MAX_TOP_K, vocab):
+        raise ValueError(f"top_k must be between 0 and {min(MAX_TOP_K, vocab)}, got {top_k}")
+    if not (temperature > 0 and math.isfinite(temperature)):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+
+
+def _ordered(z: torch.Tensor) -> torch.Tensor:
+    """Integers in the order of the values: one zero, NaN above everything."""
+    bits = torch.where(torch.isnan(z), 0x7FFFFFFF, (z + 0.0).float().view(torch.int32))
+    return torch.where(bits < 0, bits ^ 0x7FFFFFFF, bits)
+
+
+class _TokenLogprobsRef(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, top_k, temperature):
+        vocab = logits.shape[-1]
+        z = logits if logits.dtype == torch.float64 else logits.float()
+        top = z.amax(-1, keepdim=True)
+        none = top == -math.inf
+        u = (z - torch.where(none, 0.0, top)) / temperature
+        e = torch.exp(u)
+        total = torch.where(none, 1.0, e.sum(-1, keepdim=True))
+        log_p = u - torch.log(total)
+        entropy = torch.log(total) - torch.where(u == -math.inf, 0.0, u * e).sum(-1, keepdim=True) / total
+        inside = (targets >= 0) & (targets < vocab)
+        at = targets.long().clamp(0, vocab - 1).unsqueeze(-1)
+        logp = torch.where(inside, log_p.gather(-1, at).squeeze(-1), 0.0)
+        top_logp = top_ids = None
+        if top_k:
+            place = torch.arange(vocab, device=z.device)
+            key = _ordered(z).long() * (1 << 32) + (vocab - 1 - place)
+            top_ids = vocab - 1 - torch.topk(key, top_k, dim=-1).values % (1 << 32)
+            top_logp = log_p.gather(-1, top_ids)
+        ctx.save_for_backward(log_p, entropy, inside & ~none.squeeze(-1), at)
+        ctx.dtype, ctx.temperature = logits.dtype, temperature
+        ctx.mark_non_differentiable(*(t for t in (top_logp, top_ids) if t is not None))
+        return logp, entropy.squeeze(-1), top_logp, top_ids
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_logp, d_entropy, *_):
+        log_p, entropy, counts, at = ctx.saved_tensors
+        p = torch.exp(log_p)
+        a = torch.where(counts, d_logp, 0.0).unsqueeze(-1)
+        g = -p * a - d_entropy.unsqueeze(-1) * torch.where(p == 0, 0.0, p * (log_p + entropy))
+        g = g.scatter_add(-1, at, a)
+        return (g / ctx.temperature).to(ctx.dtype), None, None, None
+
+
+def token_logprobs_ref(logits: torch.Tensor, targets: torch.Tensor, *, top_k: int = 0,
+                       temperature: float = 1.0) -> TokenLogprobs:
+    """PyTorch statement of :func:`token_logprobs`: in fp32, or in fp64 for fp64 logits."""
+    return TokenLogprobs(*_TokenLogprobsRef.apply(logits, targets, top_k, temperature))
+
+
+def _forward(z: torch.Tensor, targets: torch.Tensor, top_k: int, temperature: float):
+    """Kernel call on ``z [rows, V]`` (unit column stride) and int64 ``targets [rows]``."""
+    rows, vocab = z.shape
+    num = torch.empty((4, rows), dtype=torch.float32, device=z.device)      # logp, entropy, (max, log2 sum) pairs
+    top_logp = top_ids = None
+    if top_k:
+        top_logp = torch.empty((rows, top_k), dtype=torch.float32, device=z.device)
+        top_ids = torch.empty((rows, top_k), dtype=torch.int64, device=z.device)
+    logp, entropy, stats = num[0], num[1], num[2:]
+    with _lib.on_device(z.device):
+        rc = _lib.lib().ob_logprobs_fwd(_lib.ptr(z), z.stride(0), _KERNEL_DTYPES[z.dtype], _lib.ptr(targets),
+                                        _lib.ptr(logp), _lib.ptr(entropy), _lib.ptr(stats), _lib.ptr(top_logp),
+                                        _lib.ptr(top_ids), rows, vocab, top_k, temperature, _lib.stream())
+    _lib.check(rc, "ob_logprobs_fwd")
+    return logp, entropy, stats, top_logp, top_ids
+
+
+def _backward(z: torch.Tensor, targets: torch.Tensor, stats: torch.Tensor, entropy: torch.Tensor,
+              d_logp: torch.Tensor | None, d_entropy: torch.Tensor | None, temperature: float,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """``d loss / d z``; ``out`` may be ``z`` itself."""
+    rows, vocab = z.shape
+    if out is None:
+        out = torch.empty((rows, vocab), dtype=z.dtype, device=z.device)
+    d_logp = None if d_logp is None else d_logp.to(torch.float32).contiguous()
+    d_entropy = None if d_entropy is None else d_entropy.to(torch.float32).contiguous()
+    with _lib.on_device(z.device):
+        rc = _lib.lib().ob_logprobs_bwd(_lib.ptr(z), z.stride(0), _KERNEL_DTYPES[z.dtype], _lib.ptr(targets),
+                                        _lib.ptr(stats), _lib.ptr(entropy), _lib.ptr(d_logp), _lib.ptr(d_entropy),
+                                        _lib.ptr(out), out.stride(0), rows, vocab, temperature, _lib.stream())
+    _lib.check(rc, "ob_logprobs_bwd")
+    return out
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, targets, top_k, temperature):
+        logp, entropy, stats, top_logp, top_ids = _forward(z, targets, top_k, temperature)
+        ctx.save_for_backward(z, targets, stats, entropy)
+        ctx.temperature = temperature
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(*(t for t in (top_logp, top_ids) if t is not None))
+        return logp, entropy, top_logp, top_ids
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_logp, d_entropy, *_):
+        if d_logp is None and d_entropy is None:
+            return None, None, None, None
+        z, targets, stats, entropy = ctx.saved_tensors
+        return _backward(z, targets, stats, entropy, d_logp, d_entropy, ctx.temperature), None, None, None
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top_k: int = 0,
+                   temperature: float = 1.0) -> TokenLogprobs:
+    """Log probabilities of ``targets [...]`` under ``logits [..., V]`` (see the module docstring).
+
+    bf16, fp16 and fp32 logits of any row stride run in one kernel on CUDA; ``logp`` and ``entropy`` are
+    differentiable, the alternatives (``top_k`` of them, at most 32) are not.
+    """
+    top_k, temperature = int(top_k), float(temperature)
+    if logits.dim() < 1:
+        raise ValueError("logits need a vocabulary dimension")
+    vocab = logits.shape[-1]
+    _check(logits.shape[:-1], vocab, logits, targets, top_k, temperature)
+    if not (logits.is_cuda and logits.dtype in _KERNEL_DTYPES):
+        return token_logprobs_ref(logits, targets, top_k=top_k, temperature=temperature)
+    shape = targets.shape
+    z = logits if logits.dim() == 2 else logits.reshape(-1, vocab)
+    if z.stride(1) != 1 and vocab > 1:
+        z = z.contiguous()
+    tg = targets.reshape(-1).to(torch.int64).contiguous()
+    if z.requires_grad and torch.is_grad_enabled():
+        logp, entropy, top_logp, top_ids = _TokenLogprobs.apply(z, tg, top_k, temperature)
+    else:
+        logp, entropy, _, top_logp, top_ids = _forward(z, tg, top_k, temperature)
+    if len(shape) != 1:
+        logp, entropy = logp.view(shape), entropy.view(shape)
+        if top_k:
+            top_logp, top_ids = top_logp.view(*shape, top_k), top_ids.view(*shape, top_k)
+    return TokenLogprobs(logp, entropy, top_logp, top_ids)
+
+
+@torch.no_grad()
+def linear_token_logprobs(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, top_k: int = 0,
+                          temperature: float = 1.0, chunk_rows: int = 4096) -> TokenLogprobs:
+    """:func:`token_logprobs` of the logits ``x [..., d] @ weight [V, d]^T``, without gradients.
+
+    Rows are taken ``chunk_rows`` at a time, so no more than a chunk of logits is held.
+    """
+    top_k, temperature = int(top_k), float(temperature)
+    vocab = weight.shape[0]
+    _check(x.shape[:-1], vocab, x, targets, top_k, temperature)
+    if chunk_rows < 1:
+        raise ValueError(f"chunk_rows must be positive, got {chunk_rows}")
+    shape, d = targets.shape, x.shape[-1]
+    x2, tg = x.reshape(-1, d), targets.reshape(-1)
+    kernel = x.is_cuda and x.dtype == torch.bfloat16 and weight.dtype == torch.bfloat16 and d % 8 == 0
+    if kernel:
+        x2 = x2.contiguous()
+    rows = x2.shape[0]
+    ld = (vocab + 7) // 8 * 8
+    buf = None
+    parts = []
+    for r0 in range(0, rows, chunk_rows):
+        r1 = min(rows, r0 + chunk_rows)
+        if kernel:
+            if buf is None:
+                buf = torch.empty((min(chunk_rows, rows), ld), dtype=torch.bfloat16, device=x.device)
+            logits = buf[: r1 - r0, :vocab]
+            gemm.gemm(x2[r0:r1], weight, out=logits)
+        else:
+            logits = F.linear(x2[r0:r1], weight)
+        parts.append(token_logprobs(logits, tg[r0:r1], top_k=top_k, temperature=temperature))
+    if not parts:
+        parts.append(token_logprobs(x.new_empty((0, vocab)), tg, top_k=top_k, temperature=temperature))
+    cat = lambda ts: ts[0] if len(ts) == 1 else torch.cat(ts)                                   # noqa: E731
+    return TokenLogprobs(cat([p.logp for p in parts]).view(shape), cat([p.entropy for p in parts]).view(shape),
+                         cat([p.top_logp for p in parts]).view(*shape, top_k) if top_k else None,
+                         cat([p.top_ids for p in parts]).view(*shape, top_k) if top_k else None)
