@@ -71,7 +71,7 @@ class _CountingLib:
 
 
 _NO_LAUNCH = {"ob_norm_bwd_grid", "ob_rope_grid", "ob_bind_thread", "ob_set_flag_wait_iters", "ob_gemm_skinny_splits",
-              "ob_gemm2_ce_tiles"}
+              "ob_gemm2_ce_tiles", "ob_attn_decode_fp8_workspace"}
 _tls = threading.local()
 
 
@@ -269,5 +269,9 @@ def _declare(l: ctypes.CDLL) -> None:
     D = c_double
     sig("ob_logprobs_fwd", [P, L, I, P, P, P, P, P, P, I, I, I, D, P])
     sig("ob_logprobs_bwd", [P, L, I, P, P, P, P, P, P, L, I, I, D, P])
+    sig("ob_kv_fp8_append", [P, P, I, L, L, L, P, P, L, L, L, P, P, L, L, P, P, I, I, I, I, I, I, P, P])
+    sig("ob_attn_decode_fp8", [P, L, I, P, P, L, L, P, P, L, L, L, P, P, L, L, P, P, P, I, I, I, I, I, I, F, I, P, P])
+    sig("ob_attn_decode_fp8_workspace", [I, I, I, I, I])
+    l.ob_attn_decode_fp8_workspace.restype = L
     sig("ob_embedding_push", [P, I, P, I, I, I, PP, I, I, P])
     sig("ob_rs_sum", [PP, I, I, I, P, I, I, L, P, L, P, L, I, P, P])

@@ -1,0 +1,161 @@
+// Writes keys and values into a cache of e4m3 codes with one power-of-two scale for each block of tokens and head.
+//
+//   new      [B, T, Hk, hd]   bf16 / fp16 / fp32, any batch / token / head strides
+//   cache    logical [B, capacity, Hk, hd] codes with any batch / token / head strides
+//   scale    [B, Hk, blocks]  fp32
+//
+// Sequence b holds lens[b] tokens afterwards; the last n_new[b] of them are new[b, :n_new[b]].  One CTA owns one
+// block of one head of one sequence (keys or values), so no two CTAs touch the same codes or scale: it reads the
+// block's new rows once into registers, takes the largest finite magnitude, and writes codes and scale.  A block that
+// already held tokens keeps its scale unless the new rows need a larger one; then the held rows are rounded again at
+// the larger scale in the same CTA.  The kernel is bound by the stream of new rows (2 or 4 bytes read and 1 written
+// per element); the CTA has one thread per 64 elements of a full block, so each thread has all its loads in flight.
+#include "kv_fp8.cuh"
+
+namespace ob {
+namespace kvfp8 {
+
+constexpr int CHUNKS = 8;      // chunks of 8 elements per thread
+
+template <typename T> struct Chunk;
+template <> struct Chunk<__nv_bfloat16> {
+  uint4 u;
+  __device__ void load(const __nv_bfloat16* p) { u = *reinterpret_cast<const uint4*>(p); }
+  __device__ void zero() { u = make_uint4(0, 0, 0, 0); }
+  __device__ float2 pair(int i) const {
+    const uint32_t w = i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w;
+    return unpack_bf16x2(w);
+  }
+};
+template <> struct Chunk<__half> {
+  uint4 u;
+  __device__ void load(const __half* p) { u = *reinterpret_cast<const uint4*>(p); }
+  __device__ void zero() { u = make_uint4(0, 0, 0, 0); }
+  __device__ float2 pair(int i) const {
+    const uint32_t w = i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w;
+    return half2_to_float2(w);
+  }
+};
+template <> struct Chunk<float> {
+  float4 a, b;
+  __device__ void load(const float* p) {
+    a = reinterpret_cast<const float4*>(p)[0];
+    b = reinterpret_cast<const float4*>(p)[1];
+  }
+  __device__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ float2 pair(int i) const {
+    return i == 0 ? make_float2(a.x, a.y) : i == 1 ? make_float2(a.z, a.w) : i == 2 ? make_float2(b.x, b.y) : make_float2(b.z, b.w);
+  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(512) append_kernel(const AppendParams p) {
+  __shared__ float warp_max_[16];
+  const int tid = threadIdx.x;
+  // blockIdx.x = ((b * 2 + kv) * Hk + head) * span + j
+  unsigned i = blockIdx.x;
+  const int j = i % p.span; i /= p.span;
+  const int h = i % p.Hk; i /= p.Hk;
+  const int kv = i & 1, b = i >> 1;
+  const int len = p.lens[b];
+  const int n = p.n_new ? p.n_new[b] : (len == 0 ? 0 : p.T);
+  const int start = len - n;
+  if (n < 0 || n > p.T || start < 0 || len > p.capacity) {       // nothing of this sequence is touched
+    if (tid == 0) atomicCAS(p.status, kStatusOk, kStatusBadArgs);
+    return;
+  }
+  const int blk = start / p.block + j, row0 = blk * p.block;
+  const int lo = max(start, row0), hi = min(len, row0 + p.block);
+  if (lo >= hi) return;
+  const bool holds = lo > row0;
+  const T* src = static_cast<const T*>(kv ? p.v_new : p.k_new) + (long long)b * p.new_batch + (long long)h * p.new_head;
+  uint8_t* dst = static_cast<uint8_t*>(kv ? p.v : p.k) + (long long)b * p.batch + (long long)h * p.head;
+  float* scale = (kv ? p.v_scale : p.k_scale) + (long long)b * p.scale_batch + (long long)h * p.scale_head + blk;
+  const float was = holds ? *scale : 0.f;
+
+  const int per_row = p.hd >> 3, total = p.block * per_row;
+  Chunk<T> c[CHUNKS];
+  float amax = 0.f;
+#pragma unroll
+  for (int r = 0; r < CHUNKS; ++r) {
+    const int at = r * blockDim.x + tid, row = row0 + at / per_row;
+    if (at < total && row >= lo && row < hi)
+      c[r].load(src + (long long)(row - start) * p.new_tok + (at % per_row) * 8);
+    else
+      c[r].zero();
+  }
+#pragma unroll
+  for (int r = 0; r < CHUNKS; ++r)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = c[r].pair(e);
+      const float x = fabsf(f.x), y = fabsf(f.y);
+      if (x < INFINITY) amax = fmaxf(amax, x);
+      if (y < INFINITY) amax = fmaxf(amax, y);
+    }
+  amax = warp_max(amax);
+  if ((tid & 31) == 0) warp_max_[tid >> 5] = amax;
+  __syncthreads();             // also: everyone has read the old scale
+  for (int w = 0; w < (blockDim.x + 31) / 32; ++w) amax = fmaxf(amax, warp_max_[w]);
+  const float now = fmaxf(needed_scale(amax), was), inv = inverse_pow2(now);
+  const float ratio = was * inv;
+  const bool again = holds && now > was;
+#pragma unroll
+  for (int r = 0; r < CHUNKS; ++r) {
+    const int at = r * blockDim.x + tid, row = row0 + at / per_row;
+    if (at >= total) continue;
+    uint8_t* out = dst + (long long)row * p.tok + (at % per_row) * 8;
+    uint32_t w[2] = {0, 0};
+    if (row >= lo && row < hi) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float2 f = c[r].pair(e);
+        f.x = fabsf(f.x) < INFINITY ? f.x * inv : NAN;        // an infinity becomes NaN, not a large number
+        f.y = fabsf(f.y) < INFINITY ? f.y * inv : NAN;
+        w[e >> 1] |= to_codes(f.x, f.y) << (16 * (e & 1));
+      }
+      *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
+    } else if (again && row < lo) {
+      const uint2 old = *reinterpret_cast<const uint2*>(out);
+      const uint32_t o[2] = {old.x, old.y};
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float2 f = half2_to_float2(to_half2(o[e])), g = half2_to_float2(to_half2_hi(o[e]));
+        w[e] = to_codes(f.x * ratio, f.y * ratio) | to_codes(g.x * ratio, g.y * ratio) << 16;
+      }
+      *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
+    }
+  }
+  if (tid == 0) *scale = now;
+}
+
+int launch_append(AppendParams p, int dtype, cudaStream_t stream) {
+  if (p.B <= 0 || p.T <= 0) return 0;
+  p.span = (p.T + 2 * p.block - 2) / p.block;
+  const long long grid = (long long)p.B * 2 * p.Hk * p.span;
+  if (grid > 0x7fffffffLL) return -1;
+  const int threads = max(32, min(512, p.block * p.hd / (8 * CHUNKS)));
+  if (dtype == 0) append_kernel<__nv_bfloat16><<<(unsigned)grid, threads, 0, stream>>>(p);
+  else if (dtype == 1) append_kernel<__half><<<(unsigned)grid, threads, 0, stream>>>(p);
+  else if (dtype == 2) append_kernel<float><<<(unsigned)grid, threads, 0, stream>>>(p);
+  else return -1;
+  return (int)cudaGetLastError();
+}
+
+}  // namespace kvfp8
+}  // namespace ob
+
+// dtype: 0 = bf16, 1 = fp16, 2 = fp32.  Strides of the new rows and scales in elements, of the cache in bytes; rows of
+// both start on 16-byte boundaries.
+extern "C" int ob_kv_fp8_append(const void* k_new, const void* v_new, int dtype, long long new_batch, long long new_tok,
+                                long long new_head, void* k, void* v, long long batch, long long tok, long long head,
+                                void* k_scale, void* v_scale, long long scale_batch, long long scale_head, const void* lens,
+                                const void* n_new, int B, int T, int Hk, int hd, int capacity, int block, void* status,
+                                cudaStream_t stream) {
+  if (Hk <= 0 || hd < 32 || hd > 256 || (hd & (hd - 1)) || block < 16 || block > 128 || (block & (block - 1))) return -1;
+  if ((batch | tok | head) % 16) return -2;
+  return ob::kvfp8::launch_append({k_new, v_new, new_batch, new_tok, new_head, k, v, batch, tok, head, (float*)k_scale,
+                                   (float*)v_scale, scale_batch, scale_head, (const int*)lens, (const int*)n_new,
+                                   (int*)status, B, T, Hk, hd, capacity, block, 0},
+                                  dtype, stream);
+}

@@ -1,0 +1,282 @@
+"""Key / value cache held in 8 bits, and one-token attention over it.
+
+The cache stores e4m3 codes and one fp32 scale for each block of tokens and kv head (keys and values apart): half the
+bytes of the bf16 cache of :mod:`.decode`, which is what a decode step's time and a rollout's memory consist of.
+
+    code = round_to_e4m3(x / s),  s = the smallest power of two with  max |x| over the block <= 448 s
+
+(its exponent between -112 and 119). A block that gains tokens keeps its scale, unless the new ones need a larger one;
+then the codes it holds are rounded again at the larger scale. Powers of two make every division exact, so the result
+does not depend on how a value is computed. NaN stays NaN and infinities become NaN; neither sets a scale.
+
+``append_kv_fp8`` writes new tokens (a padded batch of prompts, or one token each), ``decode_attention_fp8`` appends
+one token per sequence and attends. CUDA runs ``csrc/kv_fp8.cu`` and ``csrc/attention_decode_fp8.cu`` for head
+dimensions 32, 64, 128 and 256, any number of query heads per kv head and bf16 / fp16 queries; the ``*_ref`` functions
+are the PyTorch statements of the same semantics and serve CPU runs, tests and whatever the kernels do not take.
+"""
+
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+
+E4M3_MAX = 448.0
+SCALE_EXP_MIN, SCALE_EXP_MAX = -112, 119
+BLOCKS = (16, 32, 64, 128)
+_HEAD_DIMS = (32, 64, 128, 256)
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _strides(t: torch.Tensor) -> tuple[int, ...]:
+    """Strides, 0 for dimensions of size 1 (whose stride means nothing)."""
+    return tuple([s if n > 1 else 0 for n, s in zip(t.shape, t.stride())])
+
+
+@dataclass
+class Fp8KVCache:
+    """``k``, ``v``: logical ``[B, capacity, Hk, hd]`` float8_e4m3fn with any strides but a unit one in the last
+    dimension (a head-major allocation viewed this way reads fastest); ``k_scale``, ``v_scale``: fp32
+    ``[B, Hk, ceil(capacity / block)]``, powers of two; ``block``: tokens that share a scale (16, 32, 64 or 128)."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+    block: int = 64
+
+    def __post_init__(self) -> None:
+        k, v, ks, vs = self.k, self.v, self.k_scale, self.v_scale
+        if self.block not in BLOCKS:
+            raise ValueError(f"block must be one of {BLOCKS}, got {self.block}")
+        if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn:
+            raise TypeError(f"codes must be float8_e4m3fn, got {k.dtype} and {v.dtype}")
+        if ks.dtype != torch.float32 or vs.dtype != torch.float32:
+            raise TypeError(f"scales must be float32, got {ks.dtype} and {vs.dtype}")
+        if k.dim() != 4 or k.shape != v.shape or _strides(k) != _strides(v) or _strides(k)[3] > 1:
+            raise ValueError("k and v must be [B, capacity, Hk, hd] of the same shape and strides, contiguous in hd")
+        B, cap, Hk, _ = k.shape
+        want = (B, Hk, -(-cap // self.block))
+        if ks.shape != want or vs.shape != want or _strides(ks) != _strides(vs) or _strides(ks)[2] > 1:
+            raise ValueError(f"k_scale and v_scale must be {want} of the same strides, contiguous in the blocks")
+        dev = k.device
+        if v.device != dev or ks.device != dev or vs.device != dev:
+            raise ValueError("codes and scales must be on one device")
+        if dev.type == "cuda":
+            _lib.status_word(dev)        # exists before any capture into a graph
+
+
+def fp8_kv_cache(batch: int, max_len: int, n_kv_head: int, head_dim: int, *, block: int = 64,
+                 device: torch.device | str | None = None) -> Fp8KVCache:
+    """An empty cache, stored head-major."""
+    if min(batch, max_len, n_kv_head, head_dim) < 1:
+        raise ValueError("a cache needs at least one sequence, token, head and dimension")
+    if block not in BLOCKS:
+        raise ValueError(f"block must be one of {BLOCKS}, got {block}")
+    shape = (batch, n_kv_head, max_len, head_dim)
+    codes = [torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2)]
+    scales = [torch.full((batch, n_kv_head, -(-max_len // block)), 2.0 ** SCALE_EXP_MIN, device=device) for _ in range(2)]
+    return Fp8KVCache(codes[0].permute(0, 2, 1, 3), codes[1].permute(0, 2, 1, 3), scales[0], scales[1], block)
+
+
+def _check_new(k_new: torch.Tensor, v_new: torch.Tensor, cache: Fp8KVCache, lead: tuple) -> None:
+    B, _, Hk, hd = cache.k.shape
+    want = (B, *lead, Hk, hd)
+    if k_new.shape != want or v_new.shape != want:
+        raise ValueError(f"new keys and values must be {want}, got {tuple(k_new.shape)} and {tuple(v_new.shape)}")
+    if k_new.dtype != v_new.dtype or k_new.dtype not in _DTYPES:
+        raise TypeError(f"new keys and values must share one of bf16, fp16, fp32: got {k_new.dtype}, {v_new.dtype}")
+    if k_new.device != cache.k.device or v_new.device != cache.k.device:
+        raise ValueError("new keys and values must be on the cache's device")
+
+
+def _check_counts(t: torch.Tensor, cache: Fp8KVCache, what: str) -> None:
+    if t.dtype != torch.int32 or t.shape != (cache.k.shape[0],) or t.device != cache.k.device or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous int32 [{cache.k.shape[0]}] on the cache's device, got "
+                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _kernel_takes(cache: Fp8KVCache) -> bool:
+    k, v = cache.k, cache.v
+    sb, st, sh, _ = _strides(k)
+    return (k.is_cuda and k.shape[3] in _HEAD_DIMS and not (sb | st | sh | k.data_ptr() | v.data_ptr()) & 15)
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` itself if its rows (last dimension) are contiguous and start on 16-byte boundaries, else a copy."""
+    bits, size = t.data_ptr(), t.element_size()
+    *outer, last = _strides(t)
+    for s in outer:
+        bits |= s * size
+    return t if last <= 1 and not bits & 15 else t.clone(memory_format=torch.contiguous_format)
+
+
+def append_kv_fp8(k_new: torch.Tensor, v_new: torch.Tensor, cache: Fp8KVCache, seq_lens: torch.Tensor,
+                  n_new: torch.Tensor | None = None) -> None:
+    """Write ``k_new`` / ``v_new [B, T, Hk, hd]`` (bf16, fp16 or fp32) into the cache.
+
+    ``seq_lens`` (int32 ``[B]``) counts the tokens of each sequence *including* the new ones; the last ``n_new[b]`` of
+    them are ``k_new[b, :n_new[b]]`` (default: all ``T``, and none for a sequence of length 0). Rows behind a
+    sequence's last token stay as they were. Counts that do not fit (``n_new`` outside ``[0, T]``, more new tokens than
+    the sequence has, a length beyond the capacity) raise on the CPU; on CUDA the sequence is left as it was and
+    ``ops._lib.check_status`` raises.
+    """
+    if k_new.dim() != 4:
+        raise ValueError(f"new keys must be [B, T, Hk, hd], got {tuple(k_new.shape)}")
+    _check_new(k_new, v_new, cache, (k_new.shape[1],))
+    _check_counts(seq_lens, cache, "seq_lens")
+    if n_new is not None:
+        _check_counts(n_new, cache, "n_new")
+    if k_new.numel() == 0:
+        return
+    if not _kernel_takes(cache):
+        append_kv_fp8_ref(k_new, v_new, cache, seq_lens, n_new)
+        return
+    k_new, v_new = _rows(k_new), _rows(v_new)
+    if _strides(k_new) != _strides(v_new):
+        k_new, v_new = k_new.contiguous(), v_new.contiguous()
+    k, ks = cache.k, cache.k_scale
+    B, T, Hk, hd = k_new.shape
+    nb, nt, nh, _ = _strides(k_new)
+    sb, st, sh, _ = _strides(k)
+    with _lib.on_device(k.device):
+        rc = _lib.lib().ob_kv_fp8_append(
+            k_new.data_ptr(), v_new.data_ptr(), _DTYPES[k_new.dtype], nb, nt, nh, k.data_ptr(), cache.v.data_ptr(), sb, st,
+            sh, ks.data_ptr(), cache.v_scale.data_ptr(), ks.stride(0), ks.stride(1), seq_lens.data_ptr(),
+            _lib.ptr(n_new), B, T, Hk, hd, k.shape[1], cache.block, _lib.status_word(k.device).data_ptr(), _lib.stream())
+    _lib.check(rc, "ob_kv_fp8_append")
+
+
+def needed_scale(amax: torch.Tensor) -> torch.Tensor:
+    """The smallest power of two ``s`` with ``amax <= 448 s``, its exponent clamped."""
+    mantissa, exponent = torch.frexp(amax.float())               # mantissa in [0.5, 1); 448 = 0.875 * 2^9
+    exponent = torch.where(amax > 0, exponent - 9 + (mantissa > 0.875).int(), SCALE_EXP_MIN)
+    return torch.ldexp(torch.ones_like(mantissa), exponent.clamp(SCALE_EXP_MIN, SCALE_EXP_MAX))
+
+
+def _to_codes(x: torch.Tensor) -> torch.Tensor:
+    """Bytes of the e4m3 values nearest to ``x`` (fp32): finite ones saturate, infinities become NaN."""
+    x = torch.where(torch.isinf(x), math.nan, x).clamp(-E4M3_MAX, E4M3_MAX)
+    return x.to(torch.float8_e4m3fn).view(torch.uint8)
+
+
+def _append_one_ref(new: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, lens: torch.Tensor, n: torch.Tensor,
+                    block: int) -> None:
+    raw = codes.view(torch.uint8)
+    for b in range(new.shape[0]):
+        end = int(lens[b])
+        start = at = end - int(n[b])
+        while at < end:
+            j = at // block
+            row0, stop = j * block, min(end, (j + 1) * block)
+            fresh = new[b, at - start:stop - start].float()                                   # [n, Hk, hd]
+            size = torch.where(torch.isfinite(fresh), fresh.abs(), 0.0).amax(dim=(0, 2))
+            s = needed_scale(size)
+            if at > row0:
+                was = scale[b, :, j].clone()
+                s = torch.maximum(s, was)
+                held = codes[b, row0:at].float() * (was / s)[:, None]
+                raw[b, row0:at] = _to_codes(held)
+            raw[b, at:stop] = _to_codes(fresh / s[:, None])
+            scale[b, :, j] = s
+            at = stop
+
+
+def append_kv_fp8_ref(k_new: torch.Tensor, v_new: torch.Tensor, cache: Fp8KVCache, seq_lens: torch.Tensor,
+                      n_new: torch.Tensor | None = None) -> None:
+    """PyTorch statement of :func:`append_kv_fp8`, block by block."""
+    T, capacity = k_new.shape[1], cache.k.shape[1]
+    n = torch.where(seq_lens == 0, 0, T) if n_new is None else n_new
+    bad = (n < 0) | (n > T) | (n > seq_lens) | (seq_lens > capacity)
+    if bool(bad.any()):
+        raise ValueError(f"sequences {bad.nonzero().flatten().tolist()}: the counts do not fit the cache")
+    _append_one_ref(k_new, cache.k, cache.k_scale, seq_lens, n, cache.block)
+    _append_one_ref(v_new, cache.v, cache.v_scale, seq_lens, n, cache.block)
+
+
+def decode_attention_fp8(q: torch.Tensor, k_new: torch.Tensor | None, v_new: torch.Tensor | None, cache: Fp8KVCache,
+                         seq_lens: torch.Tensor, *, scale: float | None = None,
+                         window: int | None = None) -> torch.Tensor:
+    """Attention of one query token per sequence against its 8-bit cache; the counterpart of
+    :func:`.decode.decode_attention`.
+
+    ``q``: ``[B, Hq, hd]`` (a strided view into a fused qkv row is fine); ``k_new`` / ``v_new [B, Hk, hd]``: the current
+    token's, appended as token ``seq_lens[b] - 1`` first (``None`` if already stored); ``seq_lens``: int32 ``[B]``,
+    counts *including* the current token, taken as the capacity where larger; ``window``: attend to the last so many
+    tokens only. A sequence of length 0 appends nothing and gives zeros. Returns ``[B, Hq, hd]`` of the type of ``q``.
+    """
+    if q.dim() != 3 or q.shape[0] != cache.k.shape[0] or q.shape[2] != cache.k.shape[3] or q.shape[1] % cache.k.shape[2]:
+        raise ValueError(f"q {tuple(q.shape)} does not fit a cache of {tuple(cache.k.shape)}")
+    if not q.is_floating_point():
+        raise TypeError(f"q must be floating point, got {q.dtype}")
+    if q.device != cache.k.device:
+        raise ValueError("q must be on the cache's device")
+    _check_counts(seq_lens, cache, "seq_lens")
+    if (k_new is None) != (v_new is None):
+        raise ValueError("k_new and v_new come together")
+    if k_new is not None:
+        _check_new(k_new, v_new, cache, ())
+        if k_new.dtype != q.dtype:
+            raise TypeError(f"q and the new keys must have one type, got {q.dtype} and {k_new.dtype}")
+    if window is not None and window < 0:
+        raise ValueError(f"window must not be negative, got {window}")
+    B, Hq, hd = q.shape
+    k, ks = cache.k, cache.k_scale
+    capacity, Hk = k.shape[1], k.shape[2]
+    scale = scale if scale is not None else 1.0 / math.sqrt(hd)
+    if not (q.dtype in (torch.bfloat16, torch.float16) and _kernel_takes(cache)):
+        return decode_attention_fp8_ref(q, k_new, v_new, cache, seq_lens, scale=scale, window=window)
+    q = _rows(q)
+    if _strides(q)[1] not in (0, hd):
+        q = q.contiguous()
+    new_batch = new_head = 0
+    if k_new is not None:
+        k_new, v_new = _rows(k_new), _rows(v_new)
+        if _strides(k_new) != _strides(v_new):
+            k_new, v_new = k_new.contiguous(), v_new.contiguous()
+        new_batch, new_head, _ = _strides(k_new)
+    l = _lib.lib()
+    out = torch.empty((B, Hq, hd), dtype=q.dtype, device=q.device)
+    if B == 0:
+        return out
+    ws = torch.empty(l.ob_attn_decode_fp8_workspace(B, Hq, Hk, hd, capacity), dtype=torch.uint8, device=q.device)
+    sb, st, sh, _ = _strides(k)
+    with _lib.on_device(k.device):
+        rc = l.ob_attn_decode_fp8(
+            q.data_ptr(), _strides(q)[0], _DTYPES[q.dtype], _lib.ptr(k_new), _lib.ptr(v_new), new_batch, new_head,
+            k.data_ptr(), cache.v.data_ptr(), sb, st, sh, ks.data_ptr(), cache.v_scale.data_ptr(), ks.stride(0),
+            ks.stride(1), seq_lens.data_ptr(), out.data_ptr(), ws.data_ptr(), B, Hq, Hk, hd, capacity, cache.block,
+            float(scale), int(window or 0), _lib.status_word(k.device).data_ptr(), _lib.stream())
+    _lib.check(rc, "ob_attn_decode_fp8")
+    return out
+
+
+def decode_attention_fp8_ref(q, k_new, v_new, cache: Fp8KVCache, seq_lens, *, scale=None, window=None) -> torch.Tensor:
+    """PyTorch statement of :func:`decode_attention_fp8` in fp32 (fp64 for fp64 queries); also appends."""
+    B, Hq, hd = q.shape
+    capacity, Hk = cache.k.shape[1], cache.k.shape[2]
+    scale = scale if scale is not None else 1.0 / math.sqrt(hd)
+    if k_new is not None:
+        append_kv_fp8_ref(k_new[:, None], v_new[:, None], cache, seq_lens)
+    wide = torch.float64 if q.dtype == torch.float64 else torch.float32
+    lens = seq_lens.long().clamp(0, capacity)
+    pos = torch.arange(capacity, device=q.device)
+    seen = pos < lens[:, None]
+    if window:
+        seen = seen & (pos >= lens[:, None] - int(window))
+    block = pos // cache.block
+
+    def values(codes, scales):                                     # [B, Hk, T, hd]; unseen rows may hold anything
+        x = codes.to(wide).transpose(1, 2) * scales.to(wide)[:, :, block, None]
+        return torch.where(seen[:, None, :, None], x, 0.0)
+
+    s = q.to(wide).view(B, Hk, Hq // Hk, hd) @ values(cache.k, cache.k_scale).transpose(2, 3) * scale
+    s = s.masked_fill(~seen[:, None, None, :], -math.inf)
+    top = s.amax(-1, keepdim=True)
+    p = torch.exp(s - torch.where(top == -math.inf, 0.0, top))
+    total = p.sum(-1, keepdim=True)
+    o = p @ values(cache.v, cache.v_scale) / torch.where(total == 0, 1.0, total)
+    return o.reshape(B, Hq, hd).to(q.dtype)
