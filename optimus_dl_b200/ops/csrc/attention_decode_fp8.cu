@@ -486,7 +486,7 @@ extern "C" int ob_attn_decode_fp8(const void* q, long long q_batch, int q_dtype,
   if (k_new) {
     const int rc = launch_append({k_new, v_new, new_batch, 0, new_head, k, v, batch, tok, head, (float*)k_scale,
                                   (float*)v_scale, scale_batch, scale_head, (const int*)lens, nullptr, (int*)status, B, 1,
-                                  Hk, hd, capacity, block, 0}, q_dtype, stream);
+                                  Hk, hd, capacity, block, 0, 0, 0}, q_dtype, stream);
     if (rc) return rc;
   }
   const int rep = Hq / Hk, nt = groups(rep, hd), nh = 8 * nt;

@@ -49,7 +49,7 @@ template <> struct Chunk<float> {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(512) append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(512) append_kernel(const __grid_constant__ AppendParams p) {
   __shared__ float warp_max_[16];
   const int tid = threadIdx.x;
   // blockIdx.x = ((b * 2 + kv) * Hk + head) * span + j
@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(512) append_kernel(const AppendParams p) {
     if (tid == 0) atomicCAS(p.status, kStatusOk, kStatusBadArgs);
     return;
   }
-  const int blk = start / p.block + j, row0 = blk * p.block;
+  const int blk = (start >> p.block_shift) + j, row0 = blk << p.block_shift;
   const int lo = max(start, row0), hi = min(len, row0 + p.block);
   if (lo >= hi) return;
   const bool holds = lo > row0;
@@ -73,14 +73,14 @@ __global__ void __launch_bounds__(512) append_kernel(const AppendParams p) {
   float* scale = (kv ? p.v_scale : p.k_scale) + (long long)b * p.scale_batch + (long long)h * p.scale_head + blk;
   const float was = holds ? *scale : 0.f;
 
-  const int per_row = p.hd >> 3, total = p.block * per_row;
+  const int row_shift = p.row_shift, total = p.block << row_shift, last = (1 << row_shift) - 1;
   Chunk<T> c[CHUNKS];
   float amax = 0.f;
 #pragma unroll
   for (int r = 0; r < CHUNKS; ++r) {
-    const int at = r * blockDim.x + tid, row = row0 + at / per_row;
+    const int at = r * blockDim.x + tid, row = row0 + (at >> row_shift);
     if (at < total && row >= lo && row < hi)
-      c[r].load(src + (long long)(row - start) * p.new_tok + (at % per_row) * 8);
+      c[r].load(src + (long long)(row - start) * p.new_tok + (at & last) * 8);
     else
       c[r].zero();
   }
@@ -102,9 +102,9 @@ __global__ void __launch_bounds__(512) append_kernel(const AppendParams p) {
   const bool again = holds && now > was;
 #pragma unroll
   for (int r = 0; r < CHUNKS; ++r) {
-    const int at = r * blockDim.x + tid, row = row0 + at / per_row;
+    const int at = r * blockDim.x + tid, row = row0 + (at >> row_shift);
     if (at >= total) continue;
-    uint8_t* out = dst + (long long)row * p.tok + (at % per_row) * 8;
+    uint8_t* out = dst + (long long)row * p.tok + (at & last) * 8;
     uint32_t w[2] = {0, 0};
     if (row >= lo && row < hi) {
 #pragma unroll
@@ -132,6 +132,9 @@ __global__ void __launch_bounds__(512) append_kernel(const AppendParams p) {
 int launch_append(AppendParams p, int dtype, cudaStream_t stream) {
   if (p.B <= 0 || p.T <= 0) return 0;
   p.span = (p.T + 2 * p.block - 2) / p.block;
+  p.block_shift = p.row_shift = 0;
+  while ((1 << p.block_shift) < p.block) ++p.block_shift;
+  while ((8 << p.row_shift) < p.hd) ++p.row_shift;
   const long long grid = (long long)p.B * 2 * p.Hk * p.span;
   if (grid > 0x7fffffffLL) return -1;
   const int threads = max(32, min(512, p.block * p.hd / (8 * CHUNKS)));
@@ -156,6 +159,6 @@ extern "C" int ob_kv_fp8_append(const void* k_new, const void* v_new, int dtype,
   if ((batch | tok | head) % 16) return -2;
   return ob::kvfp8::launch_append({k_new, v_new, new_batch, new_tok, new_head, k, v, batch, tok, head, (float*)k_scale,
                                    (float*)v_scale, scale_batch, scale_head, (const int*)lens, (const int*)n_new,
-                                   (int*)status, B, T, Hk, hd, capacity, block, 0},
+                                   (int*)status, B, T, Hk, hd, capacity, block, 0, 0, 0},
                                   dtype, stream);
 }

@@ -56,7 +56,8 @@ struct AppendParams {
   const int *lens, *n_new;                     // n_new may be null
   int* status;
   int B, T, Hk, hd, capacity, block;
-  int span;                                    // set by the launcher: blocks that a run of T tokens can touch
+  // set by the launcher: blocks that a run of T tokens can touch, log2 of block and of a row's 8-element chunks
+  int span, block_shift, row_shift;
 };
 int launch_append(AppendParams p, int dtype, cudaStream_t stream);
 

@@ -14,12 +14,12 @@
 // without any logit above -inf has log probabilities of -inf, entropy 0 and no gradient.
 //
 // Alternatives: the k largest logits, equal ones by lowest index.  A candidate is one 64-bit number, the logit's
-// order-preserving key above the complement of its index, so "better" is one integer comparison without ties.  After
-// its first batch a CTA takes the k-th best of its threads' best candidates as a threshold: at least k candidates
-// reach it, so nothing below it can be among the k largest.  From then on only candidates at or above the threshold
-// go to a shared list (about k for every doubling of the positions seen; the threshold is raised after 4, 16, 64...
-// batches), and the list is ranked at the end.  A list that overflows (rows sorted upwards) is replaced by k plain
-// arg-max passes over the slice, which the L2 cache serves.
+// order-preserving key above the complement of its index, so "better" is one integer comparison without ties.  The
+// pass over the logits does nothing for them but note in which vector a thread met its maximum.  Afterwards the k-th
+// best of the threads' maxima is a bound that at least k candidates reach; only threads whose maximum reaches it (k of
+// them, unless logits are equal) can hold one of the k best, and the CTA reads their vectors once more, from the L2
+// cache, and lists what reaches the bound: little more than k candidates, which are then ranked by counting.  A list
+// that overflows (thousands of equal logits in one thread's share) is replaced by k plain arg-max passes.
 #include "common.cuh"
 #include <cooperative_groups.h>
 
@@ -32,56 +32,10 @@ constexpr int THREADS = 256;
 constexpr int UNROLL = 4;        // 16-byte loads in flight per thread
 constexpr int MAX_TOPK = 32;
 constexpr int CAP = 1024;        // candidates a CTA can list
-constexpr int MAX_CLUSTER = 16;
+constexpr int MAX_CLUSTER = 8;
 constexpr float FLOOR = -200.0f;
 
 using u64 = unsigned long long;
-
-template <typename T> struct Vec;
-template <> struct Vec<float> {
-  static constexpr int N = 4;
-  __device__ static void unpack(const uint4& u, float (&f)[N]) {
-    f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
-  }
-  __device__ static uint4 pack(const float (&f)[N]) {
-    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-  }
-  __device__ static float load(const float* p) { return *p; }
-  __device__ static float cast(float f) { return f; }
-};
-template <> struct Vec<__nv_bfloat16> {
-  static constexpr int N = 8;
-  __device__ static void unpack(const uint4& u, float (&f)[N]) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-  }
-  __device__ static uint4 pack(const float (&f)[N]) {
-    return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
-  }
-  __device__ static float load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-  __device__ static __nv_bfloat16 cast(float f) { return __float2bfloat16(f); }
-};
-template <> struct Vec<__half> {
-  static constexpr int N = 8;
-  __device__ static void unpack(const uint4& u, float (&f)[N]) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      f[2 * i] = v.x; f[2 * i + 1] = v.y;
-    }
-  }
-  __device__ static uint32_t pack2(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-  __device__ static uint4 pack(const float (&f)[N]) {
-    return make_uint4(pack2(f[0], f[1]), pack2(f[2], f[3]), pack2(f[4], f[5]), pack2(f[6], f[7]));
-  }
-  __device__ static float load(const __half* p) { return __half2float(*p); }
-  __device__ static __half cast(float f) { return __float2half(f); }
-};
 
 __device__ __forceinline__ uint4 load_once(const void* p) {
   uint4 r;
@@ -99,6 +53,79 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+  static constexpr int N = 4;
+  static constexpr uint32_t NONE = 0xff800000u;      // 32 bits of -inf
+  __device__ static void unpack(const uint4& u, float (&f)[N]) {
+    f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+  }
+  __device__ static float max_of(const uint4& u) {
+    float f[N];
+    unpack(u, f);
+    return max_nan(max_nan(f[0], f[1]), max_nan(f[2], f[3]));
+  }
+  __device__ static uint4 pack(const float (&f)[N]) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+  __device__ static float load(const float* p) { return *p; }
+  __device__ static float cast(float f) { return f; }
+};
+template <> struct Vec<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static constexpr uint32_t NONE = 0xff80ff80u;
+  __device__ static void unpack(const uint4& u, float (&f)[N]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+  }
+  __device__ static float max_of(const uint4& u) {       // two elements per instruction
+    const uint32_t w = max2(max2(u.x, u.y), max2(u.z, u.w));
+    return max_nan(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  __device__ static uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  __device__ static uint4 pack(const float (&f)[N]) {
+    return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+  }
+  __device__ static float load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+  __device__ static __nv_bfloat16 cast(float f) { return __float2bfloat16(f); }
+};
+template <> struct Vec<__half> {
+  static constexpr int N = 8;
+  static constexpr uint32_t NONE = 0xfc00fc00u;
+  __device__ static void unpack(const uint4& u, float (&f)[N]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = v.x; f[2 * i + 1] = v.y;
+    }
+  }
+  __device__ static float max_of(const uint4& u) {
+    const uint32_t w = max2(max2(u.x, u.y), max2(u.z, u.w));
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return max_nan(v.x, v.y);
+  }
+  __device__ static uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  __device__ static uint32_t pack2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  __device__ static uint4 pack(const float (&f)[N]) {
+    return make_uint4(pack2(f[0], f[1]), pack2(f[2], f[3]), pack2(f[4], f[5]), pack2(f[6], f[7]));
+  }
+  __device__ static float load(const __half* p) { return __half2float(*p); }
+  __device__ static __half cast(float f) { return __float2half(f); }
+};
 
 // Candidate: order-preserving key (NaN above everything, one zero) over the complement of the index.  Integer
 // arithmetic only, so values below the normal range keep their order.
@@ -138,26 +165,62 @@ __device__ __forceinline__ float log_of(float z, float m, float c, float log2s) 
   return ((z - m) * c - log2s) * 0.6931471805599453f;
 }
 
-// `n` candidates in `list` (0 = none): writes the k best to `top`, best first.  All threads of the CTA.
-__device__ __forceinline__ void rank_into(const u64* list, int n, int k, u64* top) {
+struct Scratch {                 // of a CTA that looks for alternatives
+  u64 list[CAP], few[CAP], top[MAX_TOPK], merged[MAX_TOPK], warp_bound[THREADS / 32], kth;
+  int hot[THREADS];
+  int listed, counted, hots;
+};
+
+// A lower bound of the k-th best of the CTA's candidates, one per thread; the first `active` threads have one (0
+// elsewhere).  The r-th best of the lanes in each of W warps, r = ceil(k / W), and the least of those: r W >= k
+// candidates reach it.  0 when there are too few to tell.  One barrier, before the result is read.
+__device__ __forceinline__ u64 bound(u64 best, int active, int k, u64* warp_bound) {
+  const int warps = max(1, min(active, THREADS) >> 5), warp = threadIdx.x >> 5;
+  if (warp < warps) {
+    u64 w = 0;
+    for (int i = (k + warps - 1) / warps; i > 0; --i) {
+      const uint32_t key = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32));
+      const uint32_t low = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32) == key ? (uint32_t)best : 0u);
+      w = (u64)key << 32 | low;
+      if (best == w) best = 0;
+    }
+    if ((threadIdx.x & 31) == 0) warp_bound[warp] = w;
+  }
+  __syncthreads();
+  u64 b = warp_bound[0];
+  for (int w = 1; w < warps; ++w) b = min(b, warp_bound[w]);
+  return b;
+}
+
+// The k best of `n` candidates in `list` (0 = none), best first.  Barriers inside, none at the end; sc.counted is 0
+// before.
+__device__ __forceinline__ void select_top(const u64* list, int n, int k, u64* top, Scratch& sc) {
+  if (n > 64) {
+    u64 best = 0;
+    for (int i = threadIdx.x; i < n; i += THREADS) best = max(best, list[i]);
+    const u64 b = bound(best, n, k, sc.warp_bound);
+    for (int i = threadIdx.x; i < n; i += THREADS)
+      if (list[i] >= b && list[i] != 0) sc.few[atomicAdd(&sc.counted, 1)] = list[i];
+    __syncthreads();
+    n = sc.counted;
+    list = sc.few;
+  }
   for (int i = threadIdx.x; i < n; i += THREADS) {
     const u64 mine = list[i];
     int r = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) r += list[j] > mine;
     if (r < k && mine != 0) top[r] = mine;
   }
 }
 
 template <typename T, bool TOPK>
-__global__ void __launch_bounds__(THREADS, TOPK ? 3 : 4) forward_kernel(const Params p) {
-  constexpr int N = Vec<T>::N;
+__global__ void __launch_bounds__(THREADS, 4) forward_kernel(const __grid_constant__ Params p) {
+  constexpr int N = Vec<T>::N, STEP = THREADS * UNROLL;
   __shared__ Sums warp_sums[THREADS / 32];
   __shared__ Sums cta_sums;
-  __shared__ u64 list[TOPK ? CAP : 1];
-  __shared__ u64 top[TOPK ? MAX_TOPK : 1];
-  __shared__ u64 merged[TOPK ? MAX_TOPK : 1];
-  __shared__ u64 threshold;
-  __shared__ int listed;
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  Scratch& sc = *reinterpret_cast<Scratch*>(smem_raw);          // TOPK only
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x / p.cluster, rank = blockIdx.x - row * p.cluster;
   const T* z = static_cast<const T*>(p.logits) + (long long)row * p.ld;
@@ -167,120 +230,73 @@ __global__ void __launch_bounds__(THREADS, TOPK ? 3 : 4) forward_kernel(const Pa
   const int nv = (p.V - head) / N;
   const int v0 = (int)((long long)nv * rank / p.cluster), v1 = (int)((long long)nv * (rank + 1) / p.cluster);
   const char* zv = reinterpret_cast<const char*>(z + head);
-  u64 tau = 0;            // the threshold as this thread last saw it, and its value for the quick test
-  float tau_z = -INFINITY;
-  if (TOPK) {
-    if (tid == 0) { threshold = 0; listed = 0; }
-    if (tid < MAX_TOPK) { top[tid] = 0; merged[tid] = 0; }
-    __syncthreads();
-  }
-  auto push = [&](float f, int idx) {
-    const u64 cand = candidate(f, idx);
-    if (cand >= tau) {
-      const int at = atomicAdd(&listed, 1);
-      if (at < CAP) list[at] = cand;
-    }
-  };
-
-  Sums st{-INFINITY, 0.f, 0.f};
-  int batch = 0, next_refresh = 4;
-  for (int base = v0; base < v1; base += THREADS * UNROLL, ++batch) {
-    uint4 raw[UNROLL];
+  auto fetch = [&](int base, uint4 (&raw)[UNROLL]) {             // what lies behind the slice reads as banned
 #pragma unroll
     for (int j = 0; j < UNROLL; ++j) {
       const int i = base + j * THREADS + tid;
+      raw[j] = make_uint4(Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE);
       if (i < v1) raw[j] = load_once(zv + (long long)i * 16);
     }
-    float mx = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < UNROLL; ++j) {
-      if (base + j * THREADS + tid < v1) {
-        float f[N];
-        Vec<T>::unpack(raw[j], f);
-#pragma unroll
-        for (int e = 0; e < N; ++e) mx = max_nan(mx, f[e]);
-      }
-    }
-    Sums fresh{mx, 0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < UNROLL; ++j) {
-      if (base + j * THREADS + tid < v1) {
-        float f[N];
-        Vec<T>::unpack(raw[j], f);
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float u = fmaxf((f[e] - mx) * c, FLOOR);
-          const float x = exp2_fast(u);
-          fresh.s += x;
-          fresh.w = fmaf(u, x, fresh.w);
-        }
-      }
-    }
-    join(st, fresh, c);
-    if (TOPK) {
-      if (batch == 0) {
-        u64 best = 0;
-#pragma unroll
-        for (int j = 0; j < UNROLL; ++j) {
-          const int i = base + j * THREADS + tid;
-          if (i < v1) {
-            float f[N];
-            Vec<T>::unpack(raw[j], f);
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-              const u64 cand = candidate(f[e], head + i * N + e);
-              if (cand > best) best = cand;
-            }
-          }
-        }
-        list[tid] = best;
-        __syncthreads();
-        int r = 0;
-        for (int j = 0; j < THREADS; ++j) r += list[j] > best;
-        if (best != 0 && r == p.k - 1) threshold = best;
-        __syncthreads();
-      } else if (batch == next_refresh) {
-        next_refresh *= 4;
-        __syncthreads();
-        const int n = listed;
-        if (n <= CAP)
-          for (int i = tid; i < n; i += THREADS) {
-            const u64 mine = list[i];
-            int r = 0;
-            for (int j = 0; j < n; ++j) r += list[j] > mine;
-            if (r == p.k - 1) threshold = mine;
-          }
-        __syncthreads();
-      }
-      if (batch == 0 || batch * 4 == next_refresh) {
-        tau = threshold;
-        tau_z = tau == 0 ? -INFINITY : candidate_value(tau);
-      }
-      if (!(mx < tau_z)) {
-#pragma unroll
-        for (int j = 0; j < UNROLL; ++j) {
-          const int i = base + j * THREADS + tid;
-          if (i < v1) {
-            float f[N];
-            Vec<T>::unpack(raw[j], f);
-#pragma unroll
-            for (int e = 0; e < N; ++e)
-              if (!(f[e] < tau_z)) push(f[e], head + i * N + e);
-          }
-        }
-      }
-    }
+  };
+  uint4 raw[UNROLL], next[UNROLL];
+  fetch(v0, raw);
+  // the token's own logit is under way while the row is read
+  float z_t = 0.f;
+  bool inside = false;
+  if (rank == 0 && tid == 0) {
+    const long long t = p.targets[row];
+    inside = t >= 0 && t < p.V;
+    if (inside) z_t = Vec<T>::load(z + t);
   }
+  if (TOPK) {
+    if (tid == 0) { sc.listed = sc.counted = sc.hots = 0; sc.kth = 0; }
+    if (tid < MAX_TOPK) sc.top[tid] = sc.merged[tid] = 0;
+  }
+
+  Sums st{-INFINITY, 0.f, 0.f};
+  int best_vec = v0 + tid;             // TOPK: a vector that holds this thread's maximum (or one behind it)
+  for (int base = v0; base < v1; base += STEP) {
+    fetch(base + STEP, next);
+    float top_of[UNROLL], mx = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < UNROLL; ++j) {
+      top_of[j] = Vec<T>::max_of(raw[j]);
+      mx = max_nan(mx, top_of[j]);
+    }
+    if (TOPK && !(mx <= st.m)) {
+      best_vec = base + (UNROLL - 1) * THREADS + tid;
+#pragma unroll
+      for (int j = UNROLL - 2; j >= 0; --j) if (top_of[j] == mx) best_vec = base + j * THREADS + tid;
+    }
+    float2 s2 = make_float2(0.f, 0.f), w2 = s2;
+    const float2 neg = make_float2(-mx, -mx), cc = make_float2(c, c);
+#pragma unroll
+    for (int j = 0; j < UNROLL; ++j) {
+      float f[N];
+      Vec<T>::unpack(raw[j], f);
+#pragma unroll
+      for (int e = 0; e < N; e += 2) {
+        float2 u = fmul2(fadd2(make_float2(f[e], f[e + 1]), neg), cc);
+        u.x = fmaxf(u.x, FLOOR);
+        u.y = fmaxf(u.y, FLOOR);
+        const float2 x = make_float2(exp2_fast(u.x), exp2_fast(u.y));
+        s2 = fadd2(s2, x);
+        w2 = ffma2(u, x, w2);
+      }
+    }
+    join(st, Sums{mx, s2.x + s2.y, w2.x + w2.y}, c);
+#pragma unroll
+    for (int j = 0; j < UNROLL; ++j) raw[j] = next[j];
+  }
+  const u64 mine = TOPK && v0 + tid < v1 ? candidate(st.m, head + best_vec * N + N - 1) : 0;
   // the ragged ends of the row: fewer than N elements each
   const int tail = p.V - head - nv * N;
   const int extra0 = rank == 0 ? head : 0, extra1 = rank == p.cluster - 1 ? tail : 0;
+  const int extra_at = tid < extra0 ? tid : head + nv * N + (tid - extra0);
+  float extra = -INFINITY;
   if (tid < extra0 + extra1) {
-    const int idx = tid < extra0 ? tid : head + nv * N + (tid - extra0);
-    const float f = Vec<T>::load(z + idx);
-    const float u = f == f ? 0.f : f;      // e^0, or NaN
-    join(st, Sums{f, 1.f + u, 0.f}, c);
-    if (f == -INFINITY && st.m == -INFINITY) st = Sums{-INFINITY, 0.f, 0.f};
-    if (TOPK) push(f, idx);
+    extra = Vec<T>::load(z + extra_at);
+    if (extra != -INFINITY) join(st, Sums{extra, 1.f + (extra == extra ? 0.f : extra), 0.f}, c);
   }
 
   // one triple per CTA
@@ -294,24 +310,81 @@ __global__ void __launch_bounds__(THREADS, TOPK ? 3 : 4) forward_kernel(const Pa
   }
   if (lane == 0) warp_sums[warp] = st;
   __syncthreads();
-  if (tid == 0) {
-    Sums t = warp_sums[0];
-    for (int i = 1; i < THREADS / 32; ++i) join(t, warp_sums[i], c);
-    cta_sums = t;
+  if (warp == 0) {
+    Sums t = lane < THREADS / 32 ? warp_sums[lane] : Sums{-INFINITY, 0.f, 0.f};
+#pragma unroll
+    for (int o = THREADS / 64; o > 0; o >>= 1) {
+      Sums b;
+      b.m = __shfl_xor_sync(0xffffffffu, t.m, o);
+      b.s = __shfl_xor_sync(0xffffffffu, t.s, o);
+      b.w = __shfl_xor_sync(0xffffffffu, t.w, o);
+      join(t, b, c);
+    }
+    if (lane == 0) cta_sums = t;
   }
   if (TOPK) {
-    const int n = listed;
+    // the k-th best of the threads' maxima
+    const u64 rough = bound(mine, v1 - v0, p.k, sc.warp_bound);
+    if (mine != 0 && mine >= rough) sc.list[atomicAdd(&sc.counted, 1)] = mine;
+    __syncthreads();
+    const int near = sc.counted;
+    for (int i = tid; i < near; i += THREADS) {
+      const u64 m = sc.list[i];
+      int r = 0;
+#pragma unroll 8
+      for (int j = 0; j < near; ++j) r += sc.list[j] > m;
+      if (r == p.k - 1) sc.kth = m;
+    }
+    __syncthreads();
+    // threads that can hold a candidate at or above it; equal maxima count, their indices are not exact
+    const u64 kth = sc.kth;
+    if (mine != 0 && mine >> 32 >= kth >> 32) sc.hot[atomicAdd(&sc.hots, 1)] = tid;
+    if (tid == 0) sc.counted = 0;
+    __syncthreads();
+    const float kth_z = kth == 0 ? -INFINITY : candidate_value(kth);
+    const int kth_at = kth == 0 ? 0x7fffffff : candidate_index(kth);
+    auto push = [&](float f, int idx) {
+      const u64 cand = candidate(f, idx);
+      if (cand >= kth) {
+        const int at = atomicAdd(&sc.listed, 1);
+        if (at < CAP) sc.list[at] = cand;
+      }
+    };
+    const int hots = sc.hots, each = (v1 - v0 + THREADS - 1) / THREADS, looks = hots * each;
+    for (int w = tid; w < looks; w += STEP) {
+      int at[UNROLL];
+#pragma unroll
+      for (int j = 0; j < UNROLL; ++j) {
+        const int q = (w + j * THREADS) / hots, h = (w + j * THREADS) - q * hots;
+        at[j] = w + j * THREADS < looks ? v0 + q * THREADS + sc.hot[h] : v1;
+        raw[j] = make_uint4(Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE);
+        if (at[j] < v1) raw[j] = load_once(zv + (long long)at[j] * 16);
+      }
+#pragma unroll
+      for (int j = 0; j < UNROLL; ++j) {
+        const float mx = Vec<T>::max_of(raw[j]);
+        if (at[j] < v1 && !(mx < kth_z) && !(mx == kth_z && head + at[j] * N > kth_at)) {
+          float f[N];
+          Vec<T>::unpack(raw[j], f);
+#pragma unroll
+          for (int e = 0; e < N; ++e)
+            if (!(f[e] < kth_z)) push(f[e], head + at[j] * N + e);
+        }
+      }
+    }
+    if (tid < extra0 + extra1) push(extra, extra_at);
+    __syncthreads();
+    const int n = sc.listed;
     if (n <= CAP) {
-      rank_into(list, n, p.k, top);
+      select_top(sc.list, n, p.k, sc.top, sc);
     } else {
       // more candidates than the list holds: k arg-max passes, each below the one before
       u64 limit = ~0ull;
       for (int r = 0; r < p.k; ++r) {
         u64 best = 0;
         for (int i = v0 + tid; i < v1; i += THREADS) {
-          const uint4 raw = *reinterpret_cast<const uint4*>(zv + (long long)i * 16);
           float f[N];
-          Vec<T>::unpack(raw, f);
+          Vec<T>::unpack(load_once(zv + (long long)i * 16), f);
 #pragma unroll
           for (int e = 0; e < N; ++e) {
             const u64 cand = candidate(f[e], head + i * N + e);
@@ -319,130 +392,138 @@ __global__ void __launch_bounds__(THREADS, TOPK ? 3 : 4) forward_kernel(const Pa
           }
         }
         if (tid < extra0 + extra1) {
-          const int idx = tid < extra0 ? tid : head + nv * N + (tid - extra0);
-          const u64 cand = candidate(Vec<T>::load(z + idx), idx);
+          const u64 cand = candidate(extra, extra_at);
           if (cand < limit && cand > best) best = cand;
         }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          const u64 b = __shfl_xor_sync(0xffffffffu, best, o);
-          if (b > best) best = b;
-        }
+        for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
         __syncthreads();
-        if (lane == 0) list[warp] = best;
+        if (lane == 0) sc.list[warp] = best;
         __syncthreads();
-        best = list[0];
-        for (int i = 1; i < THREADS / 32; ++i) if (list[i] > best) best = list[i];
-        if (tid == 0) top[r] = best;
+        best = sc.list[0];
+        for (int i = 1; i < THREADS / 32; ++i) best = max(best, sc.list[i]);
+        if (tid == 0) sc.top[r] = best;
         if (best == 0) break;
         limit = best;
       }
     }
   }
   __syncthreads();
-  u64* chosen = top;
   if (p.cluster > 1) {
     cg::cluster_group cl = cg::this_cluster();
     cl.sync();
     if (rank == 0) {
-      if (tid == 0) {
-        Sums t = cta_sums;
-        for (int r = 1; r < p.cluster; ++r) join(t, *cl.map_shared_rank(&cta_sums, r), c);
-        warp_sums[0] = t;
+      if (warp == 0) {
+        Sums t = lane < p.cluster ? *cl.map_shared_rank(&cta_sums, lane) : Sums{-INFINITY, 0.f, 0.f};
+#pragma unroll
+        for (int o = MAX_CLUSTER / 2; o > 0; o >>= 1) {
+          Sums b;
+          b.m = __shfl_xor_sync(0xffffffffu, t.m, o);
+          b.s = __shfl_xor_sync(0xffffffffu, t.s, o);
+          b.w = __shfl_xor_sync(0xffffffffu, t.w, o);
+          join(t, b, c);
+        }
+        if (lane == 0) warp_sums[0] = t;
       }
       if (TOPK) {
         const int n = p.cluster * p.k;
-        for (int i = tid; i < n; i += THREADS) list[i] = cl.map_shared_rank(top, i / p.k)[i % p.k];
+        for (int i = tid; i < n; i += THREADS) sc.list[i] = cl.map_shared_rank(sc.top, i / p.k)[i % p.k];
+        if (tid == 0) sc.counted = 0;
         __syncthreads();
-        rank_into(list, n, p.k, merged);
-        chosen = merged;
+        select_top(sc.list, n, p.k, sc.merged, sc);
       }
     }
     cl.sync();            // no CTA leaves while its shared memory is read
     if (rank != 0) return;
-    if (tid == 0) cta_sums = warp_sums[0];
-    __syncthreads();
   }
-  const Sums total = cta_sums;
+  const Sums total = p.cluster > 1 ? warp_sums[0] : cta_sums;
   const bool none = total.m == -INFINITY, broken = !(total.m < INFINITY);     // +inf and NaN
   const float log2s = broken ? NAN : none ? 0.f : log2f(total.s);
   const float m = none ? 0.f : total.m;
   if (tid == 0) {
-    const long long t = p.targets[row];
-    float lp = 0.f;
-    if (t >= 0 && t < p.V) lp = log_of(Vec<T>::load(z + t), m, c, log2s);
-    p.logp[row] = lp;
+    p.logp[row] = inside ? log_of(z_t, m, c, log2s) : 0.f;
     p.entropy[row] = none ? 0.f : (log2s - total.w / total.s) * 0.6931471805599453f;
     p.stats[row] = make_float2(total.m, log2s);
   }
   if (TOPK && tid < p.k) {
-    const u64 cand = chosen[tid];
+    const u64 cand = p.cluster > 1 ? sc.merged[tid] : sc.top[tid];
     p.top_logp[(long long)row * p.k + tid] = log_of(candidate_value(cand), m, c, log2s);
     p.top_ids[(long long)row * p.k + tid] = candidate_index(cand);
   }
 }
 
-// One thread handles UNROLL vectors of a row; the row's five numbers are the same for the whole CTA.  `dz` may be
-// the logits themselves.
+// dz of one row's share: two batches of loads are in flight per thread, and the row's numbers are fetched behind the
+// first.  Rows are taken from the last to the first: a forward pass that ran just before left its last rows in the L2
+// cache.  `dz` may be the logits themselves (every element is read and written by the same thread).
 template <typename T>
-__global__ void __launch_bounds__(THREADS)
-backward_kernel(const T* logits, long long ld, const long long* __restrict__ targets,
-                const float2* __restrict__ stats, const float* __restrict__ entropy, const float* __restrict__ d_logp,
-                const float* __restrict__ d_entropy, T* dz, long long dz_ld, int V, int pieces, float c,
-                float inv_t) {
-  constexpr int N = Vec<T>::N;
-  const int row = blockIdx.x / pieces, piece = blockIdx.x - row * pieces, tid = threadIdx.x;
+__global__ void __launch_bounds__(THREADS, 4)
+backward_kernel(const T* logits, long long ld, const long long* __restrict__ targets, const float2* __restrict__ stats,
+                const float* __restrict__ entropy, const float* __restrict__ d_logp, const float* __restrict__ d_entropy,
+                T* dz, long long dz_ld, int rows, int V, int pieces, float c, float inv_t) {
+  constexpr int N = Vec<T>::N, STEP = THREADS * UNROLL;
+  const int up = blockIdx.x / pieces, piece = blockIdx.x - up * pieces, row = rows - 1 - up, tid = threadIdx.x;
   const T* z = logits + (long long)row * ld;
   T* g = dz + (long long)row * dz_ld;
+  const int head = min(V, (int)(((16 - (reinterpret_cast<uintptr_t>(g) & 15)) & 15) / sizeof(T)));
+  const int nv = (V - head) / N;
+  const int v0 = (int)((long long)nv * piece / pieces), v1 = (int)((long long)nv * (piece + 1) / pieces);
+  const bool aligned = (reinterpret_cast<uintptr_t>(z + head) & 15) == 0;
+  auto fetch = [&](int base, uint4 (&raw)[UNROLL]) {
+#pragma unroll
+    for (int j = 0; j < UNROLL; ++j) {
+      const int i = base + j * THREADS + tid;
+      if (i < v1) {
+        if (aligned) {
+          raw[j] = load_once(z + head + (long long)i * N);
+        } else {
+          T tmp[N];
+#pragma unroll
+          for (int e = 0; e < N; ++e) tmp[e] = z[head + (long long)i * N + e];
+          memcpy(&raw[j], tmp, 16);
+        }
+      }
+    }
+  };
+  uint4 raw[UNROLL], next[UNROLL];
+  fetch(v0, raw);
   const float2 st = stats[row];
   const bool none = st.x == -INFINITY;
   const float m = none ? 0.f : st.x;
   const long long t64 = targets[row];
-  const int t = t64 >= 0 && t64 < V && !none ? (int)t64 : -1;
-  const float gl = (t64 >= 0 && t64 < V && d_logp) ? d_logp[row] : 0.f, gh = d_entropy ? d_entropy[row] : 0.f;
+  const bool inside = t64 >= 0 && t64 < V;
+  const int t = inside && !none ? (int)t64 : -1;
+  const float gl = inside && d_logp ? d_logp[row] : 0.f, gh = d_entropy ? d_entropy[row] : 0.f;
   // p (log p + H) = p (v ln 2 + H) with v = log2 p: dz = -(p / T) (a + b v), a = g_l + g_H H, b = g_H ln 2
-  const float a = none ? 0.f : gl + gh * entropy[row], b = none ? 0.f : gh * 0.6931471805599453f;
-  auto grad = [&](float f, int idx) {
+  const float a = none ? 0.f : -inv_t * (gl + gh * entropy[row]), b = none ? 0.f : -inv_t * gh * 0.6931471805599453f;
+  const float at_token = gl * inv_t;
+  auto grad = [&](float f) {
     const float v = max_nan((f - m) * c - st.y, FLOOR);
-    const float pr = exp2_fast(v);
-    float r = -pr * fmaf(b, v, a);
-    if (idx == t) r += gl;
-    return r * inv_t;
+    return exp2_fast(v) * fmaf(b, v, a);
   };
-  const int head = min(V, (int)(((16 - (reinterpret_cast<uintptr_t>(g) & 15)) & 15) / sizeof(T)));
-  const int nv = (V - head) / N;
-  const bool aligned = (reinterpret_cast<uintptr_t>(z + head) & 15) == 0;
-  const int base = piece * THREADS * UNROLL + tid;
-  uint4 raw[UNROLL];
+  for (int base = v0; base < v1; base += STEP) {
+    fetch(base + STEP, next);
 #pragma unroll
-  for (int j = 0; j < UNROLL; ++j) {
-    const int i = base + j * THREADS;
-    if (i < nv) {
-      if (aligned) {
-        raw[j] = load_once(z + head + (long long)i * N);
-      } else {
-        T tmp[N];
+    for (int j = 0; j < UNROLL; ++j) {
+      const int i = base + j * THREADS + tid;
+      if (i < v1) {
+        float f[N];
+        Vec<T>::unpack(raw[j], f);
 #pragma unroll
-        for (int e = 0; e < N; ++e) tmp[e] = z[head + (long long)i * N + e];
-        memcpy(&raw[j], tmp, 16);
+        for (int e = 0; e < N; ++e) f[e] = grad(f[e]);
+        const unsigned off = (unsigned)(t - (head + i * N));       // t = -1 is never below N
+        if (off < N)
+#pragma unroll
+          for (int e = 0; e < N; ++e) if (e == off) f[e] += at_token;
+        *reinterpret_cast<uint4*>(g + head + (long long)i * N) = Vec<T>::pack(f);
       }
     }
-  }
 #pragma unroll
-  for (int j = 0; j < UNROLL; ++j) {
-    const int i = base + j * THREADS;
-    if (i < nv) {
-      float f[N];
-      Vec<T>::unpack(raw[j], f);
-#pragma unroll
-      for (int e = 0; e < N; ++e) f[e] = grad(f[e], head + i * N + e);
-      *reinterpret_cast<uint4*>(g + head + (long long)i * N) = Vec<T>::pack(f);
-    }
+    for (int j = 0; j < UNROLL; ++j) raw[j] = next[j];
   }
   const int tail = V - head - nv * N;
   if (piece == 0 && tid < head + tail) {
     const int idx = tid < head ? tid : nv * N + tid;
-    g[idx] = Vec<T>::cast(grad(Vec<T>::load(z + idx), idx));
+    g[idx] = Vec<T>::cast(grad(Vec<T>::load(z + idx)) + (idx == t ? at_token : 0.f));
   }
 }
 
@@ -453,20 +534,22 @@ static int run_forward(const Params& p, cudaStream_t stream) {
   cfg.gridDim = dim3((unsigned)((long long)p.rows * p.cluster));
   cfg.blockDim = dim3(THREADS);
   cfg.stream = stream;
+  cfg.dynamicSmemBytes = p.k > 0 ? sizeof(Scratch) : 0;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = p.cluster;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = p.cluster > 1 ? 1 : 0;
-  if (p.cluster > 8) OB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   return (int)cudaLaunchKernelEx(&cfg, kern, p);
 }
 
-// CTAs that share a row: enough for a few waves of the 148 SMs, but not less than one full batch of loads each.
+// CTAs that share a row: as many as make two per SM with the rows there are, each with at least one full batch of
+// loads.  Measured, V = 151936, k = 20, 64 rows: 20.6 us with 1, 15.8 with 2, 15.4 with 4, 16.9 with 8; 257 rows of
+// 50257: 14.4 us with 1, 16.5 with 2; one row of 128256, k = 5: 14.4 us with 1, 8.9 with 8, 10.3 with 16.
 static int pick_cluster(int rows, int V, int vec) {
   int cl = 1;
-  while (cl < MAX_CLUSTER && (long long)rows * cl < 148 * 6 && V / (cl * 2) >= THREADS * vec) cl *= 2;
+  while (cl < MAX_CLUSTER && (long long)rows * cl * 2 <= 148 * 2 && V / (cl * 2) >= THREADS * vec) cl *= 2;
   return cl;
 }
 
@@ -497,14 +580,20 @@ extern "C" int ob_logprobs_bwd(const void* logits, long long ld, int dtype, cons
   if (rows <= 0) return 0;
   if (V <= 0 || !(temperature > 0.0)) return -1;
   const int vec = dtype == 2 ? 4 : 8;
-  const int pieces = (V / vec + THREADS * UNROLL - 1) / (THREADS * UNROLL) + (V / vec == 0);
+  // CTAs per row: four per SM, of half a batch of loads at least, and no more than 8 batches each.  Measured: one row of
+  // 128256 bf16 18.5 us with 1, 6.2 with 8, 4.2 with 16; 1000 rows of 50257 42.5 us with 1, 45.2 with 4; 4096 rows of
+  // 128256 340 us with 1 (16 batches), 336 with 2, 350 with 4; 2048 such rows in fp32 339 us with 1, 327 with 4.
+  int pieces = 1;
+  while (V / vec / (pieces * 2) >= THREADS * UNROLL / 2 &&
+         ((long long)rows * pieces < 148 * 4 || V / vec / pieces > THREADS * UNROLL * 8))
+    pieces *= 2;
   if ((long long)rows * pieces > 0x7fffffffLL) return -1;
   const float c = (float)(1.4426950408889634 / temperature), inv_t = (float)(1.0 / temperature);
   const unsigned grid = (unsigned)((long long)rows * pieces);
 #define OB_LAUNCH(T)                                                                                                  \
   backward_kernel<T><<<grid, THREADS, 0, stream>>>((const T*)logits, ld, (const long long*)targets, (const float2*)stats, \
                                                    (const float*)entropy, (const float*)d_logp, (const float*)d_entropy, \
-                                                   (T*)dz, dz_ld, V, pieces, c, inv_t)
+                                                   (T*)dz, dz_ld, rows, V, pieces, c, inv_t)
   if (dtype == 0) OB_LAUNCH(__nv_bfloat16);
   else if (dtype == 1) OB_LAUNCH(__half);
   else if (dtype == 2) OB_LAUNCH(float);
