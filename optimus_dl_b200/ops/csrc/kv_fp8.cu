@@ -17,40 +17,51 @@ namespace kvfp8 {
 
 constexpr int CHUNKS = 8;      // chunks of 8 elements per thread
 
-template <typename T> struct Chunk;
-template <> struct Chunk<__nv_bfloat16> {
+// Eight elements.  abs_max: the largest magnitude as fp32 bits, which order infinities and NaN above every number.
+struct Chunk16 {
   uint4 u;
-  __device__ void load(const __nv_bfloat16* p) { u = *reinterpret_cast<const uint4*>(p); }
+  __device__ void load(const void* p) { u = *static_cast<const uint4*>(p); }
   __device__ void zero() { u = make_uint4(0, 0, 0, 0); }
-  __device__ float2 pair(int i) const {
-    const uint32_t w = i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w;
-    return unpack_bf16x2(w);
+  __device__ uint32_t word(int i) const { return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w; }
+  __device__ uint32_t abs_max16() const {          // both types order their magnitudes as integers
+    const uint32_t m = 0x7fff7fffu;
+    const uint32_t w = __vmaxu2(__vmaxu2(u.x & m, u.y & m), __vmaxu2(u.z & m, u.w & m));
+    return max(w & 0xffffu, w >> 16);
   }
 };
-template <> struct Chunk<__half> {
-  uint4 u;
-  __device__ void load(const __half* p) { u = *reinterpret_cast<const uint4*>(p); }
-  __device__ void zero() { u = make_uint4(0, 0, 0, 0); }
-  __device__ float2 pair(int i) const {
-    const uint32_t w = i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w;
-    return half2_to_float2(w);
-  }
+template <typename T> struct Chunk;
+template <> struct Chunk<__nv_bfloat16> : Chunk16 {
+  __device__ uint32_t abs_max() const { return abs_max16() << 16; }
+  __device__ float2 pair(int i) const { return make_float2(__uint_as_float(word(i) << 16), __uint_as_float(word(i) & 0xffff0000u)); }
+};
+template <> struct Chunk<__half> : Chunk16 {
+  __device__ uint32_t abs_max() const { return __float_as_uint(half2_to_float2(abs_max16()).x); }
+  __device__ float2 pair(int i) const { return half2_to_float2(word(i)); }
 };
 template <> struct Chunk<float> {
   float4 a, b;
-  __device__ void load(const float* p) {
-    a = reinterpret_cast<const float4*>(p)[0];
-    b = reinterpret_cast<const float4*>(p)[1];
+  __device__ void load(const void* p) {
+    a = static_cast<const float4*>(p)[0];
+    b = static_cast<const float4*>(p)[1];
   }
   __device__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ uint32_t abs_max() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = pair(i);
+      m = max(m, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+    }
+    return m;
+  }
   __device__ float2 pair(int i) const {
     return i == 0 ? make_float2(a.x, a.y) : i == 1 ? make_float2(a.z, a.w) : i == 2 ? make_float2(b.x, b.y) : make_float2(b.z, b.w);
   }
 };
 
 template <typename T>
-__global__ void __launch_bounds__(512) append_kernel(const __grid_constant__ AppendParams p) {
-  __shared__ float warp_max_[16];
+__global__ void __launch_bounds__(512, sizeof(T) == 4 ? 1 : 2) append_kernel(const __grid_constant__ AppendParams p) {
+  __shared__ uint32_t warp_max_[2][16];
   const int tid = threadIdx.x;
   // blockIdx.x = ((b * 2 + kv) * Hk + head) * span + j
   unsigned i = blockIdx.x;
@@ -75,7 +86,6 @@ __global__ void __launch_bounds__(512) append_kernel(const __grid_constant__ App
 
   const int row_shift = p.row_shift, total = p.block << row_shift, last = (1 << row_shift) - 1;
   Chunk<T> c[CHUNKS];
-  float amax = 0.f;
 #pragma unroll
   for (int r = 0; r < CHUNKS; ++r) {
     const int at = r * blockDim.x + tid, row = row0 + (at >> row_shift);
@@ -84,20 +94,31 @@ __global__ void __launch_bounds__(512) append_kernel(const __grid_constant__ App
     else
       c[r].zero();
   }
+  auto block_max = [&](uint32_t m, int buf) {
+    m = __reduce_max_sync(0xffffffffu, m);
+    if ((tid & 31) == 0) warp_max_[buf][tid >> 5] = m;
+    __syncthreads();           // the first one also: everyone has read the old scale
+    for (int w = 0; w < blockDim.x / 32; ++w) m = max(m, warp_max_[buf][w]);
+    return m;
+  };
+  uint32_t bits = 0;
 #pragma unroll
-  for (int r = 0; r < CHUNKS; ++r)
+  for (int r = 0; r < CHUNKS; ++r) bits = max(bits, c[r].abs_max());
+  bits = block_max(bits, 0);
+  const bool special = bits >= 0x7f800000u;                       // an infinity or NaN among them
+  if (special) {
+    bits = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 f = c[r].pair(e);
-      const float x = fabsf(f.x), y = fabsf(f.y);
-      if (x < INFINITY) amax = fmaxf(amax, x);
-      if (y < INFINITY) amax = fmaxf(amax, y);
-    }
-  amax = warp_max(amax);
-  if ((tid & 31) == 0) warp_max_[tid >> 5] = amax;
-  __syncthreads();             // also: everyone has read the old scale
-  for (int w = 0; w < (blockDim.x + 31) / 32; ++w) amax = fmaxf(amax, warp_max_[w]);
-  const float now = fmaxf(needed_scale(amax), was), inv = inverse_pow2(now);
+    for (int r = 0; r < CHUNKS; ++r)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = c[r].pair(e);
+        if (fabsf(f.x) < INFINITY) bits = max(bits, __float_as_uint(f.x) & 0x7fffffffu);
+        if (fabsf(f.y) < INFINITY) bits = max(bits, __float_as_uint(f.y) & 0x7fffffffu);
+      }
+    bits = block_max(bits, 1);
+  }
+  const float now = fmaxf(needed_scale(__uint_as_float(bits)), was), inv = inverse_pow2(now);
   const float ratio = was * inv;
   const bool again = holds && now > was;
 #pragma unroll
@@ -109,9 +130,12 @@ __global__ void __launch_bounds__(512) append_kernel(const __grid_constant__ App
     if (row >= lo && row < hi) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float2 f = c[r].pair(e);
-        f.x = fabsf(f.x) < INFINITY ? f.x * inv : NAN;        // an infinity becomes NaN, not a large number
-        f.y = fabsf(f.y) < INFINITY ? f.y * inv : NAN;
+        const float2 x = c[r].pair(e);
+        float2 f = fmul2(x, make_float2(inv, inv));
+        if (special) {                                            // an infinity becomes NaN, not a large number
+          if (!(fabsf(x.x) < INFINITY)) f.x = NAN;
+          if (!(fabsf(x.y) < INFINITY)) f.y = NAN;
+        }
         w[e >> 1] |= to_codes(f.x, f.y) << (16 * (e & 1));
       }
       *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
