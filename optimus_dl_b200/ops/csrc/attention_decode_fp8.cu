@@ -8,23 +8,28 @@
 //
 // The kernel is bound by the stream of codes (2 HD bytes per token and kv head).  What follows from that:
 //
-// * Codes go straight from global memory to registers with 16-byte loads, no shared memory in between.  The products
-//   run transposed, S^T = K Q^T and O^T = V^T P^T, on 16 x 8 x 16 tensor-core tiles (mma.sync: a tile is far too small
-//   for tcgen05): tokens are the M side of the first product and head dimensions that of the second, the up to 8 query
-//   heads that share a kv head are the N side of both, so no row of a tile is padding.  The K side of either product
-//   may be permuted freely, so each thread takes its 16 contiguous bytes as they come: for K as consecutive k pairs of
-//   one token, for V as the same 16 dimensions of four tokens, whose bytes are interleaved with byte permutes.  e4m3
-//   to f16 is one exact conversion for two codes; P gets from the accumulator layout of the first product to the
+// * The products run transposed, S^T = K Q^T and O^T = V^T P^T, on 16 x 8 x 16 tensor-core tiles (mma.sync: a tile is
+//   far too small for tcgen05): tokens are the M side of the first product and head dimensions that of the second, the
+//   up to 8 query heads that share a kv head are the N side of both, so no row of a tile is padding.  The K side of
+//   either product may be permuted freely, so each thread takes 16 contiguous bytes as they come: for K as consecutive k
+//   pairs of one token, for V as the same 16 dimensions of four tokens, whose bytes are interleaved with byte permutes.
+//   e4m3 to f16 is one exact conversion for two codes; P gets from the accumulator layout of the first product to the
 //   operand layout of the second with one 8 x 8 transpose (movmatrix) for 8 tokens.
+// * So every thread consumes exactly the bytes it asked for.  It copies them into a two-stage ring of its own in shared
+//   memory (cp.async, conflict-free, no barrier): the registers hold no codes in flight, 16 warps fit on an SM and each
+//   has one to two units of 16 tokens (4 to 8 KB at HD 128) under way at all times, also across sequences.
 // * q is scaled by a power of two per head so that its largest element lies in [2^14, 2^15): f16 then holds a bf16 or
-//   fp16 q exactly down to 2^-28 of that.  Probabilities are held as p 2^15 s_v / r in f16, r being the largest
-//   value scale met so far, so the smallest normal one is 2^-29 of the row's maximum and nothing overflows.  Scores,
-//   maxima, sums and both accumulators are fp32.
+//   fp16 q exactly down to 2^-28 of that.  The softmax runs against a reference that follows the maximum only when a
+//   score exceeds it by more than 2^8, so most units need no reduction across lanes and no rescaling.  Probabilities
+//   are held as p 2^7 s_v / r in f16, r being the largest value scale met so far: at most 2^15, normal down to 2^-21 of
+//   the reference.  Scores, references, sums and both accumulators are fp32.
 // * Work is cut evenly, not by sequence: units of 16 tokens of one (sequence, kv head, group of query heads) are
 //   numbered through the batch, every CTA takes an equal run of them and every warp an equal part of that.  A warp
 //   that sees all units of a segment writes its output; parts are joined first inside the CTA through shared memory
 //   (at most two per warp) and then, at most two per CTA, by a second kernel.  A ragged batch or a single long
 //   sequence therefore keeps every SM busy to the end, and the workspace does not depend on the batch.
+// * The three launches of a step (append, attention, join) overlap: each starts while the one before it drains and
+//   waits for its results only where it reads them (programmatic dependent launch).
 #include "kv_fp8.cuh"
 
 namespace ob {
@@ -32,10 +37,17 @@ namespace decode_fp8 {
 
 using namespace kvfp8;
 
-constexpr int WARPS = 8;
+#ifndef W_
+#define W_ 8
+#define C_ 2
+#endif
+constexpr int WARPS = W_;
+template <int HD, int NT> constexpr int CTAS = NT == 1 && HD <= 128 ? C_ : 1;
 constexpr int THREADS = WARPS * 32;
 constexpr int UNIT = 16;                 // tokens
-constexpr int MAX_BATCH = 4096;          // sequences per launch (their unit counts are held in shared memory)
+constexpr int MAX_BATCH = 2048;          // sequences per launch (their lengths are held in shared memory)
+constexpr float LAZY = 8.f;              // log2 of how far a score may exceed the reference
+constexpr float P_SCALE = 128.f;         // 2^7: probabilities up to 2^8 stay below 2^15 in f16
 constexpr int COMBINE_GROUPS = 8;
 
 struct Params {
@@ -47,7 +59,7 @@ struct Params {
   const int* lens;
   void* out;
   float* part_o; float2* part_ml; int2* part_info;
-  int B, Hq, Hk, rep, chunks, capacity, block_shift, window, min_units;
+  int B, Hq, Hk, rep, chunks, capacity, block_shift, window, min_units, appended;
   float scale_log2;
 };
 
@@ -78,12 +90,9 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// WORDS 32-bit words of codes from `p`, chunks of at most 16 bytes that lie `step` bytes apart; zeros when !ok.
+// WORDS 32-bit words of codes from `p`, in chunks of at most 16 bytes that lie `step` bytes apart.
 template <int WORDS>
-__device__ __forceinline__ void load_codes(uint32_t (&w)[WORDS], const uint8_t* p, int step, bool ok) {
-#pragma unroll
-  for (int i = 0; i < WORDS; ++i) w[i] = 0;
-  if (!ok) return;
+__device__ __forceinline__ void load_codes(uint32_t (&w)[WORDS], const uint8_t* p, int step) {
   if constexpr (WORDS == 1) {
     asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(w[0]) : "l"(p));
   } else if constexpr (WORDS == 2) {
@@ -95,29 +104,80 @@ __device__ __forceinline__ void load_codes(uint32_t (&w)[WORDS], const uint8_t* 
                    : "=r"(w[4 * i]), "=r"(w[4 * i + 1]), "=r"(w[4 * i + 2]), "=r"(w[4 * i + 3]) : "l"(p + i * step));
   }
 }
+template <int WORDS>
+__device__ __forceinline__ void load_codes_if(uint32_t (&w)[WORDS], const uint8_t* p, int step, bool ok) {
+  if (ok) {
+    load_codes(w, p, step);
+  } else {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) w[i] = 0;
+  }
+}
+__device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_launch_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-__device__ __forceinline__ float load_q(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ float load_q(const __half* p) { return __half2float(*p); }
+__device__ __forceinline__ float2 unpack_q(uint32_t u, const __nv_bfloat16*) { return unpack_bf16x2(u); }
+__device__ __forceinline__ float2 unpack_q(uint32_t u, const __half*) { return half2_to_float2(u); }
 __device__ __forceinline__ uint32_t pack_out(float a, float b, const __nv_bfloat16*) { return pack_bf16x2(a, b); }
 __device__ __forceinline__ uint32_t pack_out(float a, float b, const __half*) { return pack_half2(a, b); }
 __device__ __forceinline__ void store_out(__nv_bfloat16* p, float f) { *p = __float2bfloat16(f); }
 __device__ __forceinline__ void store_out(__half* p, float f) { *p = __float2half(f); }
 
+// PER consecutive numbers of one lane
+template <int PER>
+__device__ __forceinline__ void read_floats(float (&x)[PER], const float* p) {
+  if constexpr (PER == 1) {
+    x[0] = *p;
+  } else if constexpr (PER == 2) {
+    const float2 v = *reinterpret_cast<const float2*>(p);
+    x[0] = v.x; x[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; i += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(p + i);
+      x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+    }
+  }
+}
+template <int PER>
+__device__ __forceinline__ void write_floats(float* p, const float (&x)[PER]) {
+  if constexpr (PER == 1) {
+    *p = x[0];
+  } else if constexpr (PER == 2) {
+    *reinterpret_cast<float2*>(p) = make_float2(x[0], x[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+  }
+}
+template <int PER, typename T>
+__device__ __forceinline__ void write_out(T* p, const float (&x)[PER]) {
+  if constexpr (PER == 1) {
+    store_out(p, x[0]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; i += 2) reinterpret_cast<uint32_t*>(p)[i / 2] = pack_out(x[i], x[i + 1], p);
+  }
+}
+
 __device__ __forceinline__ int clamp_len(int len, int capacity) { return min(max(len, 0), capacity); }
 __device__ __forceinline__ int first_token(int len, int window) { return window > 0 && len > window ? len - window : 0; }
 
 template <int HD, int NT, typename T>
-__global__ void __launch_bounds__(THREADS, NT == 1 && HD <= 128 ? 2 : 1) decode_kernel(const Params p) {
+__global__ void __launch_bounds__(THREADS, CTAS<HD, NT>) decode_kernel(const __grid_constant__ Params p) {
   constexpr int KS = HD / 16;            // k-steps of the first product = words of one token's codes per thread
   constexpr int VW = HD / 32;            // words of one token's values per thread
   constexpr int NH = 8 * NT;
+  constexpr int KCB = HD >= 64 ? 16 : 8, VCB = HD >= 128 ? 16 : HD / 8;      // bytes of a thread's key / value chunks
   extern __shared__ __align__(16) uint8_t smem_raw[];
-  auto* slots = reinterpret_cast<Slot<HD, NT>*>(smem_raw);                       // [2 * WARPS]
-  int* cum = reinterpret_cast<int*>(smem_raw + sizeof(Slot<HD, NT>) * 2 * WARPS);  // [B + 1] units per head
-  __shared__ long long tag[2 * WARPS];
+  auto* slots = reinterpret_cast<Slot<HD, NT>*>(smem_raw);               // [2 * WARPS]: entered in the middle, left unfinished
+  int* cum = reinterpret_cast<int*>(slots + 2 * WARPS);                  // [B + 1] units per head, summed up
+  int* lens = cum + p.B + 1;                                             // [B]
+  __shared__ int tag[2 * WARPS];
   __shared__ int scan[WARPS + 1];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int HC = p.Hk * p.chunks;
+  let_next_launch_start();
 
   // units of every sequence, and their running sum
   const int per_thread = (p.B + THREADS - 1) / THREADS;
@@ -127,6 +187,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 && HD <= 128 ? 2 : 1) decode_
     if (b < p.B) {
       const int len = clamp_len(p.lens[b], p.capacity);
       const int n = len > 0 ? (len + UNIT - 1) / UNIT - first_token(len, p.window) / UNIT : 0;
+      lens[b] = len;
       cum[b + 1] = n;
       mine += n;
     }
@@ -161,21 +222,70 @@ __global__ void __launch_bounds__(THREADS, NT == 1 && HD <= 128 ? 2 : 1) decode_
   if (per < p.min_units) per = p.min_units;
   const long long A = min(total, per * blockIdx.x), E = min(total, A + per);
   const long long per_warp = (E - A + WARPS - 1) / WARPS;
-  const long long ua = min(E, A + per_warp * warp), ue = min(E, ua + per_warp);
+  const long long ua = min(E, A + per_warp * warp);
+  const int count = (int)(min(E, ua + per_warp) - ua);      // units of this warp
 
-  for (long long u = ua; u < ue;) {
-    int lo = 0, hi = p.B;                // the sequence of unit u: cum[b] * HC <= u < cum[b + 1] * HC
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if ((long long)cum[mid] * HC <= u) lo = mid; else hi = mid;
+  // the segment and position of the first unit: cum[b] * HC <= ua < cum[b + 1] * HC
+  int b = 0, hc = 0, un = 0;
+  if (count > 0) {
+    int hi = p.B;
+    while (hi - b > 1) {
+      const int mid = (b + hi) >> 1;
+      if ((long long)cum[mid] * HC <= ua) b = mid; else hi = mid;
     }
-    const int b = lo, n = cum[b + 1] - cum[b];
-    const long long rel = u - (long long)cum[b] * HC;
-    const int hc = (int)(rel / n), u0 = (int)(rel - (long long)hc * n);
-    const int u1 = (int)min((long long)n, u0 + (ue - u));
+    const unsigned rel = (unsigned)(ua - (long long)cum[b] * HC), n = cum[b + 1] - cum[b];
+    hc = rel / n;
+    un = rel - hc * n;
+  }
+
+  if (p.appended) wait_for_launch_before();      // codes and scales of the new token
+  for (int done = 0; done < count;) {
+    const int n = cum[b + 1] - cum[b], u0 = un, u1 = min(n, un + count - done);
     const int hk = hc / p.chunks, chunk = hc - hk * p.chunks;
-    const int len = clamp_len(p.lens[b], p.capacity), first = first_token(len, p.window);
+    const int len = lens[b], first = first_token(len, p.window), unit0 = first / UNIT;
     const int heads = min(NH, p.rep - chunk * NH), h0 = hk * p.rep + chunk * NH;
+
+    const long long tok = p.tok;
+    const uint8_t *kp, *vp;
+    {
+      const long long base = (long long)b * p.batch + (long long)hk * p.head, tk = (long long)(unit0 + un) * UNIT;
+      kp = p.k + base + (tk + g) * tok + t * KCB;
+      vp = p.v + base + (tk + 2 * t) * tok + g * VCB;
+    }
+    const long long srow = (long long)b * p.scale_batch + (long long)hk * p.scale_head;
+    const float *ks_p = p.k_scale + srow, *vs_p = p.v_scale + srow;
+    uint32_t ka[KS], kc[KS], va[4][VW];
+    float ks, vs;
+    auto fetch_k = [&](int unit) {
+      const int tk = (unit0 + unit) * UNIT;
+      if (tk >= first && tk + UNIT <= len) {
+        load_codes(ka, kp, 64);
+        load_codes(kc, kp + 8 * tok, 64);
+      } else {
+        load_codes_if(ka, kp, 64, tk + g >= first && tk + g < len);
+        load_codes_if(kc, kp + 8 * tok, 64, tk + g + 8 >= first && tk + g + 8 < len);
+      }
+      ks = ks_p[tk >> p.block_shift];
+      kp += UNIT * tok;
+    };
+    auto fetch_v = [&](int unit) {
+      const int tk = (unit0 + unit) * UNIT, row = tk + 2 * t;
+      if (tk >= first && tk + UNIT <= len) {
+        load_codes(va[0], vp, 128);
+        load_codes(va[1], vp + tok, 128);
+        load_codes(va[2], vp + 8 * tok, 128);
+        load_codes(va[3], vp + 9 * tok, 128);
+      } else {
+        load_codes_if(va[0], vp, 128, row >= first && row < len);
+        load_codes_if(va[1], vp + tok, 128, row + 1 >= first && row + 1 < len);
+        load_codes_if(va[2], vp + 8 * tok, 128, row + 8 >= first && row + 8 < len);
+        load_codes_if(va[3], vp + 9 * tok, 128, row + 9 >= first && row + 9 < len);
+      }
+      vs = vs_p[tk >> p.block_shift];
+      vp += UNIT * tok;
+    };
+    fetch_k(un);
+    fetch_v(un);
 
     // query heads as the B operand of the first product: k pairs of head g, dimensions as the codes are loaded
     uint32_t qf[NT][KS][2];
@@ -184,16 +294,17 @@ __global__ void __launch_bounds__(THREADS, NT == 1 && HD <= 128 ? 2 : 1) decode_
     for (int nt = 0; nt < NT; ++nt) {
       const bool live = nt * 8 + g < heads;
       const T* qp = static_cast<const T*>(p.q) + (long long)b * p.q_batch + (long long)(h0 + nt * 8 + (live ? g : 0)) * HD;
-      float qv[KS][4];
-      float amax = 0.f;
+      uint2 raw[KS];
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const int d = HD == 32 ? t * 8 + s * 4 : (s >> 2) * 64 + t * 16 + (s & 3) * 4;
+        raw[s] = live ? *reinterpret_cast<const uint2*>(qp + d) : make_uint2(0, 0);
+      }
+      float amax = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          qv[s][e] = live ? load_q(qp + d + e) : 0.f;
-          amax = fmaxf(amax, fabsf(qv[s][e]));
-        }
+      for (int s = 0; s < KS; ++s) {
+        const float2 x = unpack_q(raw[s].x, qp), y = unpack_q(raw[s].y, qp);
+        amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(y.x), fabsf(y.y)));
       }
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
@@ -201,8 +312,9 @@ __global__ void __launch_bounds__(THREADS, NT == 1 && HD <= 128 ? 2 : 1) decode_
       const float up = pow2(14 - ex), down = pow2(ex - 14) * p.scale_log2;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        qf[nt][s][0] = pack_half2(qv[s][0] * up, qv[s][1] * up);
-        qf[nt][s][1] = pack_half2(qv[s][2] * up, qv[s][3] * up);
+        const float2 x = unpack_q(raw[s].x, qp), y = unpack_q(raw[s].y, qp);
+        qf[nt][s][0] = pack_half2(x.x * up, x.y * up);
+        qf[nt][s][1] = pack_half2(y.x * up, y.y * up);
       }
       f_scale[nt][0] = __shfl_sync(0xffffffffu, down, 2 * t * 4);
       f_scale[nt][1] = __shfl_sync(0xffffffffu, down, (2 * t + 1) * 4);
@@ -217,25 +329,10 @@ __global__ void __launch_bounds__(THREADS, NT == 1 && HD <= 128 ? 2 : 1) decode_
 #pragma unroll
       for (int j = 0; j < KS; ++j) acc[nt][j][0] = acc[nt][j][1] = acc[nt][j][2] = acc[nt][j][3] = 0.f;
     }
-    const uint8_t* kb = p.k + (long long)b * p.batch + (long long)hk * p.head + t * (HD >= 64 ? 16 : 8);
-    const uint8_t* vb = p.v + (long long)b * p.batch + (long long)hk * p.head + g * (VW >= 4 ? 16 : VW * 4);
-    const float* ks_p = p.k_scale + (long long)b * p.scale_batch + (long long)hk * p.scale_head;
-    const float* vs_p = p.v_scale + (long long)b * p.scale_batch + (long long)hk * p.scale_head;
-    const int unit0 = first / UNIT;
 
-    for (int un = u0; un < u1; ++un) {
+    for (; un < u1; ++un) {
       const int tk = (unit0 + un) * UNIT;
       const bool whole = tk >= first && tk + UNIT <= len;
-      auto seen = [&](int row) { return whole || (tk + row >= first && tk + row < len); };
-      uint32_t ka[KS], kc[KS], va[4][VW];
-      load_codes(ka, kb + (long long)(tk + g) * p.tok, 64, seen(g));
-      load_codes(kc, kb + (long long)(tk + g + 8) * p.tok, 64, seen(g + 8));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 2 * t + (i & 1) + (i >> 1) * 8;
-        load_codes(va[i], vb + (long long)(tk + row) * p.tok, 128, seen(row));
-      }
-      const float ks = ks_p[tk >> p.block_shift], vs = vs_p[tk >> p.block_shift];
 
       float s[NT][4];
 #pragma unroll
@@ -246,45 +343,61 @@ __global__ void __launch_bounds__(THREADS, NT == 1 && HD <= 128 ? 2 : 1) decode_
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) mma(s[nt], a0, a1, a2, a3, qf[nt][i][0], qf[nt][i][1]);
       }
-      // raise the value reference if this block's scale is larger
-      float drop = 1.f;
-      if (vs > r) {
-        drop = r * inverse_pow2(vs);
-        r = vs;
-        inv_r = inverse_pow2(vs);
+      const float ks_now = ks, vs_now = vs;
+      if (un + 1 < u1) fetch_k(un + 1);
+      // scores in log2 units; the reference moves only if one exceeds it by more than LAZY
+      bool high = vs_now > r;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float f0 = f_scale[nt][0] * ks_now, f1 = f_scale[nt][1] * ks_now;
+        s[nt][0] *= f0; s[nt][1] *= f1; s[nt][2] *= f0; s[nt][3] *= f1;
+        if (!whole) {
+          if (tk + g < first || tk + g >= len) s[nt][0] = s[nt][1] = -INFINITY;
+          if (tk + g + 8 < first || tk + g + 8 >= len) s[nt][2] = s[nt][3] = -INFINITY;
+        }
+        high |= fmaxf(s[nt][0], s[nt][2]) > m[nt][0] + LAZY || fmaxf(s[nt][1], s[nt][3]) > m[nt][1] + LAZY;
       }
-      const float w = vs * inv_r * 32768.f;
+      if (__any_sync(0xffffffffu, high)) {
+        float drop = 1.f;                // of the value reference, if this block's scale is larger
+        if (vs_now > r) {
+          drop = r * inverse_pow2(vs_now);
+          r = vs_now;
+          inv_r = inverse_pow2(vs_now);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float m0 = fmaxf(s[nt][0], s[nt][2]), m1 = fmaxf(s[nt][1], s[nt][3]);
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) {
+            m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
+            m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+          }
+          m0 = fmaxf(m0, m[nt][0]);
+          m1 = fmaxf(m1, m[nt][1]);
+          // -inf only while every score was -inf: nothing to scale then
+          const float a0 = m0 == m[nt][0] ? 1.f : exp2_fast(m[nt][0] - m0), a1 = m1 == m[nt][1] ? 1.f : exp2_fast(m[nt][1] - m1);
+          m[nt][0] = m0;
+          m[nt][1] = m1;
+          l[nt][0] *= a0;
+          l[nt][1] *= a1;
+          const float d0 = a0 * drop, d1 = a1 * drop;
+#pragma unroll
+          for (int j = 0; j < KS; ++j) {
+            acc[nt][j][0] *= d0; acc[nt][j][1] *= d1; acc[nt][j][2] *= d0; acc[nt][j][3] *= d1;
+          }
+        }
+      }
+      const float w = vs_now * inv_r * P_SCALE;
       uint32_t pf[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float f0 = f_scale[nt][0] * ks, f1 = f_scale[nt][1] * ks;
-        float x[4] = {s[nt][0] * f0, s[nt][1] * f1, s[nt][2] * f0, s[nt][3] * f1};
-        if (!whole) {
-          if (!seen(g)) x[0] = x[1] = -INFINITY;
-          if (!seen(g + 8)) x[2] = x[3] = -INFINITY;
-        }
-        float m0 = fmaxf(x[0], x[2]), m1 = fmaxf(x[1], x[3]);
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-          m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
-          m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
-        }
-        m0 = fmaxf(m0, m[nt][0]);
-        m1 = fmaxf(m1, m[nt][1]);
-        const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
-        const float a0 = exp2_fast(m[nt][0] - b0), a1 = exp2_fast(m[nt][1] - b1);
-        m[nt][0] = m0;
-        m[nt][1] = m1;
-        const float p0 = exp2_fast(x[0] - b0), p1 = exp2_fast(x[1] - b1), p2 = exp2_fast(x[2] - b0), p3 = exp2_fast(x[3] - b1);
-        l[nt][0] = l[nt][0] * a0 + p0 + p2;
-        l[nt][1] = l[nt][1] * a1 + p1 + p3;
+        const float b0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], b1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+        const float p0 = exp2_fast(s[nt][0] - b0), p1 = exp2_fast(s[nt][1] - b1);
+        const float p2 = exp2_fast(s[nt][2] - b0), p3 = exp2_fast(s[nt][3] - b1);
+        l[nt][0] += p0 + p2;
+        l[nt][1] += p1 + p3;
         pf[nt][0] = transpose8(pack_half2(p0 * w, p1 * w));
         pf[nt][1] = transpose8(pack_half2(p2 * w, p3 * w));
-        const float d0 = a0 * drop, d1 = a1 * drop;
-#pragma unroll
-        for (int j = 0; j < KS; ++j) {
-          acc[nt][j][0] *= d0; acc[nt][j][1] *= d1; acc[nt][j][2] *= d0; acc[nt][j][3] *= d1;
-        }
       }
 #pragma unroll
       for (int i = 0; i < VW; ++i) {
@@ -298,11 +411,13 @@ __global__ void __launch_bounds__(THREADS, NT == 1 && HD <= 128 ? 2 : 1) decode_
           mma(acc[nt][2 * i + 1], e0, e1, e2, e3, pf[nt][0], pf[nt][1]);
         }
       }
+      if (un + 1 < u1) fetch_v(un + 1);
     }
 
     // this warp's part of the segment: the whole of it is written out, a piece goes to shared memory
     const bool complete = u0 == 0 && u1 == n;
-    const int slot = warp * 2 + (u0 == 0);
+    const int which = u0 == 0;
+    Slot<HD, NT>& part = slots[2 * warp + which];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -311,72 +426,76 @@ __global__ void __launch_bounds__(THREADS, NT == 1 && HD <= 128 ? 2 : 1) decode_
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         const int h = nt * 8 + 2 * t + c;
-        const float inv = sum == 0.f ? 0.f : 1.f / sum * (1.f / 32768.f);
-        if (complete) {
-          if (h < heads) {
-            T* o = static_cast<T*>(p.out) + ((long long)b * p.Hq + h0 + h) * HD;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum * (1.f / P_SCALE);
 #pragma unroll
-            for (int i = 0; i < VW; ++i) {
-              // words 4 and up of a 256-wide head lie 128 dimensions on
-              const int d = (i >> 2) * 128 + g * (VW >= 4 ? 16 : VW * 4) + (i & 3) * 4;
-              uint2 pk;
-              pk.x = pack_out(acc[nt][2 * i][c] * inv * r, acc[nt][2 * i][c + 2] * inv * r, o);
-              pk.y = pack_out(acc[nt][2 * i + 1][c] * inv * r, acc[nt][2 * i + 1][c + 2] * inv * r, o);
-              *reinterpret_cast<uint2*>(o + d) = pk;
-            }
+        for (int i = 0; i < VW; ++i) {
+          // words 4 and up of a 256-wide head lie 128 dimensions on
+          const int d = (i >> 2) * 128 + g * VCB + (i & 3) * 4;
+          const float x0 = acc[nt][2 * i][c] * inv * r, x1 = acc[nt][2 * i][c + 2] * inv * r;
+          const float x2 = acc[nt][2 * i + 1][c] * inv * r, x3 = acc[nt][2 * i + 1][c + 2] * inv * r;
+          if (!complete) {
+            *reinterpret_cast<float4*>(&part.o[h][d]) = make_float4(x0, x1, x2, x3);
+          } else if (h < heads) {
+            T* o = static_cast<T*>(p.out) + ((long long)b * p.Hq + h0 + h) * HD + d;
+            *reinterpret_cast<uint2*>(o) = make_uint2(pack_out(x0, x1, o), pack_out(x2, x3, o));
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < VW; ++i) {
-            const int d = (i >> 2) * 128 + g * (VW >= 4 ? 16 : VW * 4) + (i & 3) * 4;
-            *reinterpret_cast<float4*>(&slots[slot].o[h][d]) =
-                make_float4(acc[nt][2 * i][c] * inv * r, acc[nt][2 * i][c + 2] * inv * r, acc[nt][2 * i + 1][c] * inv * r,
-                            acc[nt][2 * i + 1][c + 2] * inv * r);
-          }
-          if (g == 0) { slots[slot].m[h] = m[nt][c]; slots[slot].l[h] = sum; }
         }
+        if (!complete && g == 0) { part.m[h] = m[nt][c]; part.l[h] = sum; }
       }
-    if (!complete && lane == 0) tag[slot] = (long long)b * HC + hc;
-    u += u1 - u0;
+    if (!complete && lane == 0) tag[2 * warp + which] = b * HC + hc;
+    done += u1 - u0;
+    if (done < count) {
+      un = 0;
+      if (++hc == HC) {
+        hc = 0;
+        do ++b; while (cum[b + 1] == cum[b]);
+      }
+    }
   }
   __syncthreads();
 
-  // join the parts of each segment inside the CTA; parts of one segment lie in neighbouring slots
+  // Join the parts of each segment inside the CTA, a warp for each head: lane j holds the reference and sum of slot j,
+  // every lane HD / 32 dimensions.
+  constexpr int PER = HD / 32;
+  static_assert(2 * WARPS <= 32, "one lane per slot");
+  const int my_tag = lane < 2 * WARPS ? tag[lane] : -1;
   int2 info[2] = {make_int2(-1, 0), make_int2(-1, 0)};
-  for (int i = 0; i < 2 * WARPS;) {
-    const long long seg = tag[i];
-    if (seg < 0) { ++i; continue; }
-    int end = i + 1;
-    while (end < 2 * WARPS && (tag[end] == seg || tag[end] < 0)) ++end;
-    const int b = (int)(seg / HC), hc = (int)(seg - (long long)b * HC);
-    const int hk = hc / p.chunks, chunk = hc - hk * p.chunks;
+  for (unsigned left = __ballot_sync(0xffffffffu, my_tag >= 0); left;) {
+    const int seg = __shfl_sync(0xffffffffu, my_tag, __ffs(left) - 1);
+    const unsigned members = __ballot_sync(0xffffffffu, my_tag == seg);
+    left &= ~members;
+    const int b = seg / HC, hc = seg - b * HC, hk = hc / p.chunks, chunk = hc - hk * p.chunks;
     const int n = cum[b + 1] - cum[b];
     const long long s0 = (long long)cum[b] * HC + (long long)hc * n, s1 = s0 + n;
     const bool complete = s0 >= A && s1 <= E;
     const int heads = min(NH, p.rep - chunk * NH), h0 = hk * p.rep + chunk * NH;
     const int which = s0 >= A;           // 1: the segment starts in this CTA
     const long long part = (long long)blockIdx.x * 2 + which;
-    for (int e = tid; e < NH * HD; e += THREADS) {
-      const int h = e / HD, d = e - h * HD;
-      float top = -INFINITY;
-      for (int j = i; j < end; ++j) if (tag[j] == seg) top = fmaxf(top, slots[j].m[h]);
-      float num = 0.f, den = 0.f;
-      for (int j = i; j < end; ++j)
-        if (tag[j] == seg && slots[j].l[h] != 0.f) {
-          const float wgt = exp2_fast(slots[j].m[h] - top) * slots[j].l[h];
-          num += wgt * slots[j].o[h][d];
-          den += wgt;
-        }
-      const float o = den == 0.f ? 0.f : num / den;
+    if (!complete) info[which] = make_int2(seg, which ? (int)((s1 - 1) / per) - (int)blockIdx.x : 0);
+    for (int h = warp; h < heads; h += WARPS) {
+      const float m = my_tag == seg ? slots[lane].m[h] : -INFINITY, l = my_tag == seg ? slots[lane].l[h] : 0.f;
+      const float top = warp_max(m);
+      const float wgt = l == 0.f ? 0.f : exp2_fast(m - top) * l;
+      const float den = warp_sum(wgt), inv = den == 0.f ? 0.f : 1.f / den;
+      float o[PER] = {};
+      for (unsigned todo = members; todo; todo &= todo - 1) {
+        const int j = __ffs(todo) - 1;
+        const float w = __shfl_sync(0xffffffffu, wgt, j);
+        float x[PER];
+        read_floats(x, &slots[j].o[h][lane * PER]);
+        if (w != 0.f)
+#pragma unroll
+          for (int e = 0; e < PER; ++e) o[e] += w * x[e];
+      }
+#pragma unroll
+      for (int e = 0; e < PER; ++e) o[e] *= inv;
       if (complete) {
-        if (h < heads) store_out(static_cast<T*>(p.out) + ((long long)b * p.Hq + h0 + h) * HD + d, o);
+        write_out(static_cast<T*>(p.out) + ((long long)b * p.Hq + h0 + h) * HD + lane * PER, o);
       } else {
-        p.part_o[part * NH * HD + e] = o;
-        if (d == 0) p.part_ml[part * NH + h] = make_float2(top, den);
+        write_floats(p.part_o + (part * NH + h) * HD + lane * PER, o);
+        if (lane == 0) p.part_ml[part * NH + h] = make_float2(top, den);
       }
     }
-    if (!complete) info[which] = make_int2((int)seg, which ? (int)((s1 - 1) / per) - (int)blockIdx.x : 0);
-    i = end;
   }
   if (tid == 0) {
     p.part_info[2 * blockIdx.x] = info[0];
@@ -386,10 +505,11 @@ __global__ void __launch_bounds__(THREADS, NT == 1 && HD <= 128 ? 2 : 1) decode_
 
 // Joins the parts of a segment that starts in CTA blockIdx.x and goes on in the CTAs behind it; one head per CTA here.
 template <int HD, int NH, typename T>
-__global__ void __launch_bounds__(COMBINE_GROUPS * 32) combine_kernel(const Params p) {
+__global__ void __launch_bounds__(COMBINE_GROUPS * 32) combine_kernel(const __grid_constant__ Params p) {
   constexpr int PER = HD / 32;
   __shared__ float so[COMBINE_GROUPS][HD];
   __shared__ float sm[COMBINE_GROUPS], sl[COMBINE_GROUPS];
+  wait_for_launch_before();
   const int2 info = p.part_info[2 * blockIdx.x + 1];
   if (info.x < 0) return;
   const int HC = p.Hk * p.chunks;
@@ -427,15 +547,31 @@ __global__ void __launch_bounds__(COMBINE_GROUPS * 32) combine_kernel(const Para
   }
 }
 
+template <typename... Args>
+static cudaError_t launch_behind(bool overlap, void (*kern)(Args...), dim3 grid, int threads, size_t smem, cudaStream_t stream,
+                                 const Params& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = overlap ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, p);
+}
+
 template <int HD, int NT, typename T>
 static int launch(const Params& p, int grid, cudaStream_t stream) {
-  const size_t smem = sizeof(Slot<HD, NT>) * 2 * WARPS + sizeof(int) * (p.B + 1);
+  const size_t smem = sizeof(Slot<HD, NT>) * 2 * WARPS + sizeof(int) * (2 * p.B + 1);
   auto kern = decode_kernel<HD, NT, T>;
   OB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  kern<<<grid, THREADS, smem, stream>>>(p);
-  OB_CUDA_CHECK(cudaGetLastError());
-  combine_kernel<HD, 8 * NT, T><<<dim3(grid, min(8 * NT, p.rep)), COMBINE_GROUPS * 32, 0, stream>>>(p);
-  return (int)cudaGetLastError();
+  OB_CUDA_CHECK(launch_behind(p.appended, kern, dim3(grid), THREADS, smem, stream, p));
+  OB_CUDA_CHECK(launch_behind(true, combine_kernel<HD, 8 * NT, T>, dim3(grid, min(8 * NT, p.rep)), COMBINE_GROUPS * 32, 0,
+                              stream, p));
+  return 0;
 }
 
 // Two groups of 8 query heads per pass over the codes where the accumulators of both fit beside them.
@@ -455,7 +591,7 @@ constexpr int MIN_UNITS = 8;
 static int grid_size(int B, int Hk, int rep, int hd, int capacity) {
   const int nt = groups(rep, hd), chunks = (rep + 8 * nt - 1) / (8 * nt);
   const long long most = (long long)B * Hk * chunks * ((capacity + UNIT - 1) / UNIT + 1);
-  const long long want = (most + MIN_UNITS - 1) / MIN_UNITS, fit = nt == 1 && hd <= 128 ? 296 : 148;
+  const long long want = (most + MIN_UNITS - 1) / MIN_UNITS, fit = nt == 1 && hd <= 128 ? 148 * C_ : 148;
   return (int)(want < fit ? want : fit);
 }
 
@@ -510,6 +646,7 @@ extern "C" int ob_attn_decode_fp8(const void* q, long long q_batch, int q_dtype,
     p.B = nb; p.Hq = Hq; p.Hk = Hk; p.rep = rep; p.chunks = (rep + nh - 1) / nh; p.capacity = capacity;
     p.block_shift = shift; p.window = window; p.min_units = MIN_UNITS;
     p.scale_log2 = scale * 1.4426950408889634f;
+    p.appended = k_new != nullptr && b0 == 0;      // the launch before is the append
     const int rc = q_dtype == 0 ? dispatch<__nv_bfloat16>(p, hd, nt, grid, stream) : dispatch<__half>(p, hd, nt, grid, stream);
     if (rc) return rc;
   }

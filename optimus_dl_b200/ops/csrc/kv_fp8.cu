@@ -16,6 +16,61 @@ namespace ob {
 namespace kvfp8 {
 
 constexpr int CHUNKS = 8;      // chunks of 8 elements per thread
+constexpr int ONE_WARPS = 4;   // rows per CTA when every sequence gets one token
+
+// PER elements of a row per lane
+template <int PER>
+__device__ __forceinline__ void load_row(float (&x)[PER], const float* p) {
+  if constexpr (PER == 1) x[0] = *p;
+  else
+#pragma unroll
+    for (int i = 0; i < PER; i += 2) {
+      const float2 v = *reinterpret_cast<const float2*>(p + i);
+      x[i] = v.x; x[i + 1] = v.y;
+    }
+}
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float2 to_float2(uint32_t w, const __nv_bfloat16*) { return unpack_bf16x2(w); }
+__device__ __forceinline__ float2 to_float2(uint32_t w, const __half*) { return half2_to_float2(w); }
+template <int PER, typename T>
+__device__ __forceinline__ void load_row(float (&x)[PER], const T* p) {
+  if constexpr (PER == 1) x[0] = to_float(*p);
+  else {
+    uint32_t w[PER / 2];
+    if constexpr (PER == 8) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(p);
+    else if constexpr (PER == 4) *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(p);
+    else w[0] = *reinterpret_cast<const uint32_t*>(p);
+#pragma unroll
+    for (int i = 0; i < PER / 2; ++i) {
+      const float2 v = to_float2(w[i], p);
+      x[2 * i] = v.x; x[2 * i + 1] = v.y;
+    }
+  }
+}
+template <int PER>
+__device__ __forceinline__ void store_codes(uint8_t* p, const float (&x)[PER]) {
+  if constexpr (PER == 1) *p = (uint8_t)to_codes(x[0], 0.f);
+  else if constexpr (PER == 2) *reinterpret_cast<uint16_t*>(p) = (uint16_t)to_codes(x[0], x[1]);
+  else
+#pragma unroll
+    for (int i = 0; i < PER; i += 4)
+      *reinterpret_cast<uint32_t*>(p + i) = to_codes(x[i], x[i + 1]) | to_codes(x[i + 2], x[i + 3]) << 16;
+}
+template <int PER>
+__device__ __forceinline__ void load_codes(float (&x)[PER], const uint8_t* p) {
+  if constexpr (PER <= 2) {
+    const float2 v = half2_to_float2(to_half2(PER == 1 ? *p : *reinterpret_cast<const uint16_t*>(p)));
+    x[0] = v.x;
+    if constexpr (PER == 2) x[1] = v.y;
+  } else
+#pragma unroll
+    for (int i = 0; i < PER; i += 4) {
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(p + i);
+      const float2 a = half2_to_float2(to_half2(w)), b = half2_to_float2(to_half2_hi(w));
+      x[i] = a.x; x[i + 1] = a.y; x[i + 2] = b.x; x[i + 3] = b.y;
+    }
+}
 
 // Eight elements.  abs_max: the largest magnitude as fp32 bits, which order infinities and NaN above every number.
 struct Chunk16 {
@@ -63,6 +118,7 @@ template <typename T>
 __global__ void __launch_bounds__(512, sizeof(T) == 4 ? 1 : 2) append_kernel(const __grid_constant__ AppendParams p) {
   __shared__ uint32_t warp_max_[2][16];
   const int tid = threadIdx.x;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the attention launch may start its own set-up
   // blockIdx.x = ((b * 2 + kv) * Hk + head) * span + j
   unsigned i = blockIdx.x;
   const int j = i % p.span; i /= p.span;
@@ -153,6 +209,66 @@ __global__ void __launch_bounds__(512, sizeof(T) == 4 ? 1 : 2) append_kernel(con
   if (tid == 0) *scale = now;
 }
 
+// One token per sequence (T = 1), a warp for each row: the same rules, without a block-wide step.
+template <typename T, int HD>
+__global__ void __launch_bounds__(ONE_WARPS * 32) append_one_kernel(const __grid_constant__ AppendParams p) {
+  constexpr int PER = HD / 32;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  // item = (b * 2 + kv) * Hk + head
+  const long long item = (long long)blockIdx.x * ONE_WARPS + (threadIdx.x >> 5);
+  if (item >= 2LL * p.B * p.Hk) return;
+  unsigned i = (unsigned)item;
+  const int h = i % p.Hk; i /= p.Hk;
+  const int kv = i & 1, b = i >> 1;
+  const T* src = static_cast<const T*>(kv ? p.v_new : p.k_new) + (long long)b * p.new_batch + (long long)h * p.new_head;
+  float x[PER];
+  load_row(x, src + lane * PER);
+  const int len = p.lens[b], n = p.n_new ? p.n_new[b] : len != 0;
+  if (n < 0 || n > 1 || len < n || len > p.capacity) {
+    if (lane == 0) atomicCAS(p.status, kStatusOk, kStatusBadArgs);
+    return;
+  }
+  if (n == 0) return;
+  const int pos = len - 1, blk = pos >> p.block_shift, row0 = blk << p.block_shift;
+  uint8_t* dst = static_cast<uint8_t*>(kv ? p.v : p.k) + (long long)b * p.batch + (long long)h * p.head + lane * PER;
+  float* scale = (kv ? p.v_scale : p.k_scale) + (long long)b * p.scale_batch + (long long)h * p.scale_head + blk;
+  const float was = pos > row0 ? *scale : 0.f;
+  uint32_t bits = 0;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const uint32_t m = __float_as_uint(x[e]) & 0x7fffffffu;
+    if (m < 0x7f800000u) bits = max(bits, m);
+    else x[e] = NAN;                                              // an infinity becomes NaN, not a large number
+  }
+  bits = __reduce_max_sync(0xffffffffu, bits);
+  const float now = fmaxf(needed_scale(__uint_as_float(bits)), was), inv = inverse_pow2(now);
+#pragma unroll
+  for (int e = 0; e < PER; ++e) x[e] *= inv;
+  store_codes(dst + (long long)pos * p.tok, x);
+  if (now > was) {
+    if (lane == 0) *scale = now;
+    const float ratio = was * inv;
+    for (int row = row0; row < pos; ++row) {                      // rows that are held, at the larger scale
+      uint8_t* at = dst + (long long)row * p.tok;
+      load_codes(x, at);
+#pragma unroll
+      for (int e = 0; e < PER; ++e) x[e] *= ratio;
+      store_codes(at, x);
+    }
+  }
+}
+
+template <typename T>
+static int launch_one(const AppendParams& p, cudaStream_t stream) {
+  const unsigned grid = (unsigned)((2LL * p.B * p.Hk + ONE_WARPS - 1) / ONE_WARPS);
+  if (p.hd == 32) append_one_kernel<T, 32><<<grid, ONE_WARPS * 32, 0, stream>>>(p);
+  else if (p.hd == 64) append_one_kernel<T, 64><<<grid, ONE_WARPS * 32, 0, stream>>>(p);
+  else if (p.hd == 128) append_one_kernel<T, 128><<<grid, ONE_WARPS * 32, 0, stream>>>(p);
+  else append_one_kernel<T, 256><<<grid, ONE_WARPS * 32, 0, stream>>>(p);
+  return (int)cudaGetLastError();
+}
+
 int launch_append(AppendParams p, int dtype, cudaStream_t stream) {
   if (p.B <= 0 || p.T <= 0) return 0;
   p.span = (p.T + 2 * p.block - 2) / p.block;
@@ -160,7 +276,10 @@ int launch_append(AppendParams p, int dtype, cudaStream_t stream) {
   while ((1 << p.block_shift) < p.block) ++p.block_shift;
   while ((8 << p.row_shift) < p.hd) ++p.row_shift;
   const long long grid = (long long)p.B * 2 * p.Hk * p.span;
-  if (grid > 0x7fffffffLL) return -1;
+  if (grid > 0x7fffffffLL || 2LL * p.B * p.Hk > 0x7fffffffLL) return -1;
+  if (p.T == 1)
+    return dtype == 0 ? launch_one<__nv_bfloat16>(p, stream) : dtype == 1 ? launch_one<__half>(p, stream)
+         : dtype == 2 ? launch_one<float>(p, stream) : -1;
   const int threads = max(32, min(512, p.block * p.hd / (8 * CHUNKS)));
   if (dtype == 0) append_kernel<__nv_bfloat16><<<(unsigned)grid, threads, 0, stream>>>(p);
   else if (dtype == 1) append_kernel<__half><<<(unsigned)grid, threads, 0, stream>>>(p);
