@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(THREADS, 4) forward_kernel(const __grid_consta
   if (tid == 0) {
     p.logp[row] = inside ? log_of(z_t, m, c, log2s) : 0.f;
     p.entropy[row] = none ? 0.f : (log2s - total.w / total.s) * 0.6931471805599453f;
-    p.stats[row] = make_float2(total.m, log2s);
+    if (p.stats) p.stats[row] = make_float2(total.m, log2s);
   }
   if (TOPK && tid < p.k) {
     const u64 cand = p.cluster > 1 ? sc.merged[tid] : sc.top[tid];

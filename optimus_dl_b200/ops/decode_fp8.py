@@ -17,6 +17,7 @@ are the PyTorch statements of the same semantics and serve CPU runs, tests and w
 
 from __future__ import annotations
 
+import functools
 import math
 from dataclasses import dataclass
 
@@ -33,10 +34,11 @@ _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 def _strides(t: torch.Tensor) -> tuple[int, ...]:
     """Strides, 0 for dimensions of size 1 (whose stride means nothing)."""
-    return tuple([s if n > 1 else 0 for n, s in zip(t.shape, t.stride())])
+    strides = t.stride()
+    return tuple([s if n > 1 else 0 for n, s in zip(t.shape, strides)]) if 1 in t.shape else strides
 
 
-@dataclass
+@dataclass(frozen=True)
 class Fp8KVCache:
     """``k``, ``v``: logical ``[B, capacity, Hk, hd]`` float8_e4m3fn with any strides but a unit one in the last
     dimension (a head-major allocation viewed this way reads fastest); ``k_scale``, ``v_scale``: fp32
@@ -56,17 +58,30 @@ class Fp8KVCache:
             raise TypeError(f"codes must be float8_e4m3fn, got {k.dtype} and {v.dtype}")
         if ks.dtype != torch.float32 or vs.dtype != torch.float32:
             raise TypeError(f"scales must be float32, got {ks.dtype} and {vs.dtype}")
-        if k.dim() != 4 or k.shape != v.shape or _strides(k) != _strides(v) or _strides(k)[3] > 1:
+        strides = _strides(k)
+        if k.dim() != 4 or k.shape != v.shape or strides != _strides(v) or strides[3] > 1:
             raise ValueError("k and v must be [B, capacity, Hk, hd] of the same shape and strides, contiguous in hd")
-        B, cap, Hk, _ = k.shape
-        want = (B, Hk, -(-cap // self.block))
-        if ks.shape != want or vs.shape != want or _strides(ks) != _strides(vs) or _strides(ks)[2] > 1:
+        B, capacity, Hk, hd = k.shape
+        want = (B, Hk, -(-capacity // self.block))
+        scale_strides = _strides(ks)
+        if ks.shape != want or vs.shape != want or scale_strides != _strides(vs) or scale_strides[2] > 1:
             raise ValueError(f"k_scale and v_scale must be {want} of the same strides, contiguous in the blocks")
         dev = k.device
         if v.device != dev or ks.device != dev or vs.device != dev:
             raise ValueError("codes and scales must be on one device")
-        if dev.type == "cuda":
-            _lib.status_word(dev)        # exists before any capture into a graph
+        keep = object.__setattr__
+        keep(self, "_device", dev)
+        keep(self, "_kernels", False)
+        if k.is_cuda:
+            sb, st, sh, _ = strides
+            keep(self, "_kernels", hd in _HEAD_DIMS and not (sb | st | sh | k.data_ptr() | v.data_ptr()) & 15)
+            keep(self, "_status", _lib.status_word(dev))        # exists before any capture into a graph
+            keep(self, "_geometry", (sb, st, sh, scale_strides[0], scale_strides[1]))
+
+    def _args(self) -> tuple:
+        """What describes the cache to the kernels: codes and their strides, scales and theirs."""
+        sb, st, sh, cb, ch = self._geometry
+        return (self.k.data_ptr(), self.v.data_ptr(), sb, st, sh, self.k_scale.data_ptr(), self.v_scale.data_ptr(), cb, ch)
 
 
 def fp8_kv_cache(batch: int, max_len: int, n_kv_head: int, head_dim: int, *, block: int = 64,
@@ -82,36 +97,41 @@ def fp8_kv_cache(batch: int, max_len: int, n_kv_head: int, head_dim: int, *, blo
     return Fp8KVCache(codes[0].permute(0, 2, 1, 3), codes[1].permute(0, 2, 1, 3), scales[0], scales[1], block)
 
 
-def _check_new(k_new: torch.Tensor, v_new: torch.Tensor, cache: Fp8KVCache, lead: tuple) -> None:
-    B, _, Hk, hd = cache.k.shape
-    want = (B, *lead, Hk, hd)
+def _check_new(k_new: torch.Tensor, v_new: torch.Tensor, cache: Fp8KVCache, want: tuple) -> None:
     if k_new.shape != want or v_new.shape != want:
         raise ValueError(f"new keys and values must be {want}, got {tuple(k_new.shape)} and {tuple(v_new.shape)}")
     if k_new.dtype != v_new.dtype or k_new.dtype not in _DTYPES:
         raise TypeError(f"new keys and values must share one of bf16, fp16, fp32: got {k_new.dtype}, {v_new.dtype}")
-    if k_new.device != cache.k.device or v_new.device != cache.k.device:
+    if k_new.device != cache._device or v_new.device != cache._device:
         raise ValueError("new keys and values must be on the cache's device")
 
 
-def _check_counts(t: torch.Tensor, cache: Fp8KVCache, what: str) -> None:
-    if t.dtype != torch.int32 or t.shape != (cache.k.shape[0],) or t.device != cache.k.device or not t.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous int32 [{cache.k.shape[0]}] on the cache's device, got "
-                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
+def _check_counts(t: torch.Tensor, cache: Fp8KVCache, batch: int, what: str) -> None:
+    if t.dtype != torch.int32 or t.shape != (batch,) or t.device != cache._device or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous int32 [{batch}] on the cache's device, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
 
 
-def _kernel_takes(cache: Fp8KVCache) -> bool:
-    k, v = cache.k, cache.v
-    sb, st, sh, _ = _strides(k)
-    return (k.is_cuda and k.shape[3] in _HEAD_DIMS and not (sb | st | sh | k.data_ptr() | v.data_ptr()) & 15)
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` itself if its rows (last dimension) are contiguous and start on 16-byte boundaries, else a copy."""
+def _row_strides(t: torch.Tensor) -> tuple[torch.Tensor, tuple[int, ...]]:
+    """``t`` and its strides, or those of a copy if its rows (last dimension) are not contiguous or do not start on
+    16-byte boundaries."""
+    strides = _strides(t)
     bits, size = t.data_ptr(), t.element_size()
-    *outer, last = _strides(t)
-    for s in outer:
+    for s in strides[:-1]:
         bits |= s * size
-    return t if last <= 1 and not bits & 15 else t.clone(memory_format=torch.contiguous_format)
+    if strides[-1] > 1 or bits & 15:
+        t = t.clone(memory_format=torch.contiguous_format)
+        strides = _strides(t)
+    return t, strides
+
+
+def _new_rows(k_new: torch.Tensor, v_new: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, tuple[int, ...]]:
+    k_new, k_strides = _row_strides(k_new)
+    v_new, v_strides = _row_strides(v_new)
+    if k_strides != v_strides:
+        k_new, v_new = k_new.contiguous(), v_new.contiguous()
+        k_strides = _strides(k_new)
+    return k_new, v_new, k_strides
 
 
 def append_kv_fp8(k_new: torch.Tensor, v_new: torch.Tensor, cache: Fp8KVCache, seq_lens: torch.Tensor,
@@ -124,29 +144,25 @@ def append_kv_fp8(k_new: torch.Tensor, v_new: torch.Tensor, cache: Fp8KVCache, s
     the sequence has, a length beyond the capacity) raise on the CPU; on CUDA the sequence is left as it was and
     ``ops._lib.check_status`` raises.
     """
+    B, capacity, Hk, hd = cache.k.shape
     if k_new.dim() != 4:
         raise ValueError(f"new keys must be [B, T, Hk, hd], got {tuple(k_new.shape)}")
-    _check_new(k_new, v_new, cache, (k_new.shape[1],))
-    _check_counts(seq_lens, cache, "seq_lens")
+    T = k_new.shape[1]
+    _check_new(k_new, v_new, cache, (B, T, Hk, hd))
+    _check_counts(seq_lens, cache, B, "seq_lens")
     if n_new is not None:
-        _check_counts(n_new, cache, "n_new")
-    if k_new.numel() == 0:
+        _check_counts(n_new, cache, B, "n_new")
+    if T == 0:
         return
-    if not _kernel_takes(cache):
+    if not cache._kernels:
         append_kv_fp8_ref(k_new, v_new, cache, seq_lens, n_new)
         return
-    k_new, v_new = _rows(k_new), _rows(v_new)
-    if _strides(k_new) != _strides(v_new):
-        k_new, v_new = k_new.contiguous(), v_new.contiguous()
-    k, ks = cache.k, cache.k_scale
-    B, T, Hk, hd = k_new.shape
-    nb, nt, nh, _ = _strides(k_new)
-    sb, st, sh, _ = _strides(k)
-    with _lib.on_device(k.device):
+    k_new, v_new, (nb, nt, nh, _) = _new_rows(k_new, v_new)
+    with _lib.on_device(cache._device):
         rc = _lib.lib().ob_kv_fp8_append(
-            k_new.data_ptr(), v_new.data_ptr(), _DTYPES[k_new.dtype], nb, nt, nh, k.data_ptr(), cache.v.data_ptr(), sb, st,
-            sh, ks.data_ptr(), cache.v_scale.data_ptr(), ks.stride(0), ks.stride(1), seq_lens.data_ptr(),
-            _lib.ptr(n_new), B, T, Hk, hd, k.shape[1], cache.block, _lib.status_word(k.device).data_ptr(), _lib.stream())
+            k_new.data_ptr(), v_new.data_ptr(), _DTYPES[k_new.dtype], nb, nt, nh, *cache._args(),
+            seq_lens.data_ptr(), None if n_new is None else n_new.data_ptr(), B, T, Hk, hd, capacity, cache.block,
+            cache._status.data_ptr(), _lib.stream())
     _lib.check(rc, "ob_kv_fp8_append")
 
 
@@ -208,50 +224,53 @@ def decode_attention_fp8(q: torch.Tensor, k_new: torch.Tensor | None, v_new: tor
     counts *including* the current token, taken as the capacity where larger; ``window``: attend to the last so many
     tokens only. A sequence of length 0 appends nothing and gives zeros. Returns ``[B, Hq, hd]`` of the type of ``q``.
     """
-    if q.dim() != 3 or q.shape[0] != cache.k.shape[0] or q.shape[2] != cache.k.shape[3] or q.shape[1] % cache.k.shape[2]:
-        raise ValueError(f"q {tuple(q.shape)} does not fit a cache of {tuple(cache.k.shape)}")
-    if not q.is_floating_point():
-        raise TypeError(f"q must be floating point, got {q.dtype}")
-    if q.device != cache.k.device:
+    B, capacity, Hk, hd = cache.k.shape
+    shape = q.shape
+    if len(shape) != 3 or shape[0] != B or shape[2] != hd or shape[1] % Hk:
+        raise ValueError(f"q {tuple(shape)} does not fit a cache of {tuple(cache.k.shape)}")
+    dtype, Hq = q.dtype, shape[1]
+    if not dtype.is_floating_point:
+        raise TypeError(f"q must be floating point, got {dtype}")
+    if q.device != cache._device:
         raise ValueError("q must be on the cache's device")
-    _check_counts(seq_lens, cache, "seq_lens")
+    _check_counts(seq_lens, cache, B, "seq_lens")
     if (k_new is None) != (v_new is None):
         raise ValueError("k_new and v_new come together")
     if k_new is not None:
-        _check_new(k_new, v_new, cache, ())
-        if k_new.dtype != q.dtype:
-            raise TypeError(f"q and the new keys must have one type, got {q.dtype} and {k_new.dtype}")
+        _check_new(k_new, v_new, cache, (B, Hk, hd))
+        if k_new.dtype != dtype:
+            raise TypeError(f"q and the new keys must have one type, got {dtype} and {k_new.dtype}")
     if window is not None and window < 0:
         raise ValueError(f"window must not be negative, got {window}")
-    B, Hq, hd = q.shape
-    k, ks = cache.k, cache.k_scale
-    capacity, Hk = k.shape[1], k.shape[2]
     scale = scale if scale is not None else 1.0 / math.sqrt(hd)
-    if not (q.dtype in (torch.bfloat16, torch.float16) and _kernel_takes(cache)):
+    if not (cache._kernels and dtype in (torch.bfloat16, torch.float16)):
         return decode_attention_fp8_ref(q, k_new, v_new, cache, seq_lens, scale=scale, window=window)
-    q = _rows(q)
-    if _strides(q)[1] not in (0, hd):
+    out = torch.empty(shape, dtype=dtype, device=cache._device)
+    if B == 0 or Hq == 0:
+        return out
+    q, (q_batch, q_head, _) = _row_strides(q)
+    if q_head not in (0, hd):
         q = q.contiguous()
+        q_batch = Hq * hd
+    new_k = new_v = None
     new_batch = new_head = 0
     if k_new is not None:
-        k_new, v_new = _rows(k_new), _rows(v_new)
-        if _strides(k_new) != _strides(v_new):
-            k_new, v_new = k_new.contiguous(), v_new.contiguous()
-        new_batch, new_head, _ = _strides(k_new)
+        k_new, v_new, (new_batch, new_head, _) = _new_rows(k_new, v_new)
+        new_k, new_v = k_new.data_ptr(), v_new.data_ptr()
     l = _lib.lib()
-    out = torch.empty((B, Hq, hd), dtype=q.dtype, device=q.device)
-    if B == 0:
-        return out
-    ws = torch.empty(l.ob_attn_decode_fp8_workspace(B, Hq, Hk, hd, capacity), dtype=torch.uint8, device=q.device)
-    sb, st, sh, _ = _strides(k)
-    with _lib.on_device(k.device):
+    ws = torch.empty(_workspace(B, Hq, Hk, hd, capacity), dtype=torch.uint8, device=cache._device)
+    with _lib.on_device(cache._device):
         rc = l.ob_attn_decode_fp8(
-            q.data_ptr(), _strides(q)[0], _DTYPES[q.dtype], _lib.ptr(k_new), _lib.ptr(v_new), new_batch, new_head,
-            k.data_ptr(), cache.v.data_ptr(), sb, st, sh, ks.data_ptr(), cache.v_scale.data_ptr(), ks.stride(0),
-            ks.stride(1), seq_lens.data_ptr(), out.data_ptr(), ws.data_ptr(), B, Hq, Hk, hd, capacity, cache.block,
-            float(scale), int(window or 0), _lib.status_word(k.device).data_ptr(), _lib.stream())
+            q.data_ptr(), q_batch, _DTYPES[dtype], new_k, new_v, new_batch, new_head, *cache._args(),
+            seq_lens.data_ptr(), out.data_ptr(), ws.data_ptr(), B, Hq, Hk, hd, capacity, cache.block,
+            scale, window or 0, cache._status.data_ptr(), _lib.stream())
     _lib.check(rc, "ob_attn_decode_fp8")
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace(B: int, Hq: int, Hk: int, hd: int, capacity: int) -> int:
+    return _lib.lib().ob_attn_decode_fp8_workspace(B, Hq, Hk, hd, capacity)
 
 
 def decode_attention_fp8_ref(q, k_new, v_new, cache: Fp8KVCache, seq_lens, *, scale=None, window=None) -> torch.Tensor:

@@ -109,36 +109,46 @@ def token_logprobs_ref(logits: torch.Tensor, targets: torch.Tensor, *, top_k: in
     return TokenLogprobs(*_TokenLogprobsRef.apply(logits, targets, top_k, temperature))
 
 
-def _forward(z: torch.Tensor, targets: torch.Tensor, top_k: int, temperature: float):
-    """Kernel call on ``z [rows, V]`` (unit column stride) and int64 ``targets [rows]``."""
+def _forward(z: torch.Tensor, targets: torch.Tensor, top_k: int, temperature: float, keep: bool):
+    """Kernel call on ``z [rows, V]`` (unit column stride) and contiguous int64 ``targets [rows]``. Returns ``logp,
+    entropy, top_logp, top_ids, num``; with ``keep``, ``num[1:]`` is what the gradient needs: the entropy, and the
+    maximum and log2 sum of every row as pairs."""
     rows, vocab = z.shape
-    num = torch.empty((4, rows), dtype=torch.float32, device=z.device)      # logp, entropy, (max, log2 sum) pairs
+    dev = z.device
+    num = torch.empty((4 if keep else 2, rows), dtype=torch.float32, device=dev)
     top_logp = top_ids = None
     if top_k:
-        top_logp = torch.empty((rows, top_k), dtype=torch.float32, device=z.device)
-        top_ids = torch.empty((rows, top_k), dtype=torch.int64, device=z.device)
-    logp, entropy, stats = num[0], num[1], num[2:]
-    with _lib.on_device(z.device):
-        rc = _lib.lib().ob_logprobs_fwd(_lib.ptr(z), z.stride(0), _KERNEL_DTYPES[z.dtype], _lib.ptr(targets),
-                                        _lib.ptr(logp), _lib.ptr(entropy), _lib.ptr(stats), _lib.ptr(top_logp),
-                                        _lib.ptr(top_ids), rows, vocab, top_k, temperature, _lib.stream())
+        top_logp = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
+        top_ids = torch.empty((rows, top_k), dtype=torch.int64, device=dev)
+    at = num.data_ptr()
+    with _lib.on_device(dev):
+        rc = _lib.lib().ob_logprobs_fwd(
+            z.data_ptr(), z.stride(0), _KERNEL_DTYPES[z.dtype], targets.data_ptr(), at, at + 4 * rows,
+            at + 8 * rows if keep else None, top_logp.data_ptr() if top_k else None, top_ids.data_ptr() if top_k else None,
+            rows, vocab, top_k, temperature, _lib.stream())
     _lib.check(rc, "ob_logprobs_fwd")
-    return logp, entropy, stats, top_logp, top_ids
+    return num[0], num[1], top_logp, top_ids, num
 
 
-def _backward(z: torch.Tensor, targets: torch.Tensor, stats: torch.Tensor, entropy: torch.Tensor,
-              d_logp: torch.Tensor | None, d_entropy: torch.Tensor | None, temperature: float,
-              out: torch.Tensor | None = None) -> torch.Tensor:
-    """``d loss / d z``; ``out`` may be ``z`` itself."""
+def _rows_fp32(g: torch.Tensor) -> torch.Tensor:
+    return g if g.dtype == torch.float32 and g.is_contiguous() else g.to(torch.float32).contiguous()
+
+
+def _backward(z: torch.Tensor, targets: torch.Tensor, num: torch.Tensor, d_logp: torch.Tensor | None,
+              d_entropy: torch.Tensor | None, temperature: float, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``d loss / d z`` from what ``_forward`` kept; ``out`` may be ``z`` itself."""
     rows, vocab = z.shape
     if out is None:
         out = torch.empty((rows, vocab), dtype=z.dtype, device=z.device)
-    d_logp = None if d_logp is None else d_logp.to(torch.float32).contiguous()
-    d_entropy = None if d_entropy is None else d_entropy.to(torch.float32).contiguous()
+    # the converted gradients live until the launch has been queued
+    d_logp = None if d_logp is None else _rows_fp32(d_logp)
+    d_entropy = None if d_entropy is None else _rows_fp32(d_entropy)
+    at = num.data_ptr()
     with _lib.on_device(z.device):
-        rc = _lib.lib().ob_logprobs_bwd(_lib.ptr(z), z.stride(0), _KERNEL_DTYPES[z.dtype], _lib.ptr(targets),
-                                        _lib.ptr(stats), _lib.ptr(entropy), _lib.ptr(d_logp), _lib.ptr(d_entropy),
-                                        _lib.ptr(out), out.stride(0), rows, vocab, temperature, _lib.stream())
+        rc = _lib.lib().ob_logprobs_bwd(
+            z.data_ptr(), z.stride(0), _KERNEL_DTYPES[z.dtype], targets.data_ptr(), at + 8 * rows, at + 4 * rows,
+            None if d_logp is None else d_logp.data_ptr(), None if d_entropy is None else d_entropy.data_ptr(),
+            out.data_ptr(), out.stride(0), rows, vocab, temperature, _lib.stream())
     _lib.check(rc, "ob_logprobs_bwd")
     return out
 
@@ -146,11 +156,13 @@ def _backward(z: torch.Tensor, targets: torch.Tensor, stats: torch.Tensor, entro
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, targets, top_k, temperature):
-        logp, entropy, stats, top_logp, top_ids = _forward(z, targets, top_k, temperature)
-        ctx.save_for_backward(z, targets, stats, entropy)
+        logp, entropy, top_logp, top_ids, num = _forward(z, targets, top_k, temperature, True)
+        ctx.save_for_backward(z, targets, num)
         ctx.temperature = temperature
         ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(*(t for t in (top_logp, top_ids) if t is not None))
+        if not top_k:
+            return logp, entropy
+        ctx.mark_non_differentiable(top_logp, top_ids)
         return logp, entropy, top_logp, top_ids
 
     @staticmethod
@@ -158,8 +170,8 @@ class _TokenLogprobs(torch.autograd.Function):
     def backward(ctx, d_logp, d_entropy, *_):
         if d_logp is None and d_entropy is None:
             return None, None, None, None
-        z, targets, stats, entropy = ctx.saved_tensors
-        return _backward(z, targets, stats, entropy, d_logp, d_entropy, ctx.temperature), None, None, None
+        z, targets, num = ctx.saved_tensors
+        return _backward(z, targets, num, d_logp, d_entropy, ctx.temperature), None, None, None
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top_k: int = 0,
@@ -172,20 +184,27 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top_k: int = 
     top_k, temperature = int(top_k), float(temperature)
     if logits.dim() < 1:
         raise ValueError("logits need a vocabulary dimension")
-    vocab = logits.shape[-1]
+    vocab, shape = logits.shape[-1], targets.shape
     _check(logits.shape[:-1], vocab, logits, targets, top_k, temperature)
     if not (logits.is_cuda and logits.dtype in _KERNEL_DTYPES):
         return token_logprobs_ref(logits, targets, top_k=top_k, temperature=temperature)
-    shape = targets.shape
-    z = logits if logits.dim() == 2 else logits.reshape(-1, vocab)
+    flat = len(shape) == 1
+    z, tg = logits, targets
+    if not flat:
+        z, tg = z.reshape(-1, vocab), tg.reshape(-1)
     if z.stride(1) != 1 and vocab > 1:
         z = z.contiguous()
-    tg = targets.reshape(-1).to(torch.int64).contiguous()
+    if tg.dtype != torch.int64 or not tg.is_contiguous():
+        tg = tg.to(torch.int64).contiguous()
+    top_logp = top_ids = None
     if z.requires_grad and torch.is_grad_enabled():
-        logp, entropy, top_logp, top_ids = _TokenLogprobs.apply(z, tg, top_k, temperature)
+        if top_k:
+            logp, entropy, top_logp, top_ids = _TokenLogprobs.apply(z, tg, top_k, temperature)
+        else:
+            logp, entropy = _TokenLogprobs.apply(z, tg, 0, temperature)
     else:
-        logp, entropy, _, top_logp, top_ids = _forward(z, tg, top_k, temperature)
-    if len(shape) != 1:
+        logp, entropy, top_logp, top_ids, _ = _forward(z, tg, top_k, temperature, False)
+    if not flat:
         logp, entropy = logp.view(shape), entropy.view(shape)
         if top_k:
             top_logp, top_ids = top_logp.view(*shape, top_k), top_ids.view(*shape, top_k)
