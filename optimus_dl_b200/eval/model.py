@@ -15,6 +15,7 @@ from typing import Any
 
 import torch
 
+from ..ops.logprobs import token_logprobs
 from ..recipe.generation import generate_stream, unwrap
 
 logger = logging.getLogger(__name__)
@@ -101,19 +102,24 @@ class LLMBaselinesModel(_LMBase):
                 spans.append((len(full) - 1 - n_cont, len(full) - 1, full[len(full) - n_cont:]))
             T = max(len(r) for r in rows)
             x = torch.zeros((len(rows), T), dtype=torch.long)
+            wanted = torch.full((len(rows), T), -100, dtype=torch.long)      # the continuation's tokens, where they are scored
             for j, r in enumerate(rows):
                 x[j, : len(r)] = torch.tensor(r, dtype=torch.long)
-            seq_lens = torch.tensor([len(r) for r in rows], dtype=torch.long)
-            logits = self.model(x.to(self._device), seq_lens=seq_lens.to(self._device))["logits"].float()
-            logp = torch.log_softmax(logits, dim=-1).cpu()
-            for j, i in enumerate(idx):
                 a, b, targets = spans[j]
+                if b > a:
+                    wanted[j, a:b] = torch.tensor(targets, dtype=torch.long)
+            seq_lens = torch.tensor([len(r) for r in rows], dtype=torch.long)
+            logits = self.model(x.to(self._device), seq_lens=seq_lens.to(self._device))["logits"]
+            if int(wanted.max()) >= logits.shape[-1]:
+                raise IndexError(f"token {int(wanted.max())} is outside the model's vocabulary of {logits.shape[-1]}")
+            scored = token_logprobs(logits, wanted.to(logits.device), top_k=1)
+            logp, best = scored.logp.cpu(), scored.top_ids[..., 0].cpu()
+            for j, i in enumerate(idx):
+                a, b, _ = spans[j]
                 if b <= a:
                     out[i] = (0.0, True)
                     continue
-                tgt = torch.tensor(targets, dtype=torch.long)
-                lp = logp[j, a:b]
-                out[i] = (float(lp.gather(-1, tgt[:, None]).sum()), bool((lp.argmax(-1) == tgt).all()))
+                out[i] = (float(logp[j, a:b].sum()), bool((best[j, a:b] == wanted[j, a:b]).all()))
         return out
 
     def loglikelihood(self, requests: list) -> list[tuple[float, bool]]:

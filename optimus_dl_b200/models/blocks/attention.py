@@ -118,6 +118,7 @@ class BaseSelfAttention(nn.Module):
         """Inference with a key/value cache: a multi-token call is a prefill that fills the cache, a
         one-token call attends over the cache with the decode kernel (which also appends)."""
         from ...ops import decode as dec_ops
+        from ...ops import decode_fp8 as fp8_ops
 
         kv = self.kv
         B, T, _ = x.shape
@@ -142,8 +143,12 @@ class BaseSelfAttention(nn.Module):
         v_new = work[..., (Hq + Hk) * hd:].reshape(B, T, Hk, hd)
         if T > 1 or not kv.filled:
             assert not kv.filled, "multi-token calls are only supported as the prefill of an empty cache"
-            kv.k[:, :T].copy_(k_new)
-            kv.v[:, :T].copy_(v_new)
+            if kv.fp8 is not None:
+                lens = torch.full((B,), T, dtype=torch.int32, device=x.device)
+                fp8_ops.append_kv_fp8(k_new, v_new, kv.fp8, lens)
+            else:
+                kv.k[:, :T].copy_(k_new)
+                kv.v[:, :T].copy_(v_new)
             doc_start = attn_ops.build_doc_start(B, T, x.device, None, None)
             y = attn_ops.attention_rotated(work, n_head=Hq, n_kv_head=Hk, head_dim=hd, doc_start=doc_start,
                                            window=self.sliding_window)
@@ -152,8 +157,12 @@ class BaseSelfAttention(nn.Module):
             q = w2[:, : Hq * hd].unflatten(1, (Hq, hd))
             kn = w2[:, Hq * hd:(Hq + Hk) * hd].unflatten(1, (Hk, hd))
             vn = w2[:, (Hq + Hk) * hd:].unflatten(1, (Hk, hd))
-            y = dec_ops.decode_attention(q, kn, vn, kv.k, kv.v, kv.seq_lens, window=self.sliding_window,
-                                         n_splits=kv.n_splits, workspace=kv.workspace).view(B, 1, Hq * hd)
+            if kv.fp8 is not None:
+                y = fp8_ops.decode_attention_fp8(q, kn, vn, kv.fp8, kv.seq_lens, window=self.sliding_window)
+            else:
+                y = dec_ops.decode_attention(q, kn, vn, kv.k, kv.v, kv.seq_lens, window=self.sliding_window,
+                                             n_splits=kv.n_splits, workspace=kv.workspace)
+            y = y.view(B, 1, Hq * hd)
         return lin_ops.linear(y, self.wo.weight, self.wo.bias)
 
 

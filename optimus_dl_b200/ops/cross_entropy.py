@@ -23,6 +23,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib, gemm
+from . import logprobs as lp_ops
 
 SOFTCAP = {None: 0, "none": 0, "tanh": 1, "sigmoid": 2}
 
@@ -177,11 +178,12 @@ class _LinearTokenLoss(torch.autograd.Function):
     ``loss_fn(nll_chunk, r0, r1) -> (loss_chunk, dloss_dnll_chunk)`` is evaluated per row chunk
     between the statistics kernel and the gradient kernel, so losses whose per-token weight depends
     on the log-probability itself (clipped policy ratios, KL penalties) need one pass over the
-    ``[tokens, vocab]`` logits, which are never held beyond a chunk.
+    ``[tokens, vocab]`` logits, which are never held beyond a chunk. With ``entropy_weight [tokens]`` the
+    weighted entropies join the sum; both kernels of a chunk are those of ``ops.logprobs`` then.
     """
 
     @staticmethod
-    def forward(ctx, x, weight, targets, loss_fn, chunk_rows):
+    def forward(ctx, x, weight, targets, loss_fn, chunk_rows, entropy_weight):
         l = _lib.lib()
         dev = x.device
         x2 = x.reshape(-1, x.shape[-1])
@@ -203,68 +205,94 @@ class _LinearTokenLoss(torch.autograd.Function):
         st = torch.empty((5, chunk_rows), dtype=torch.float32, device=dev)
         best = torch.empty(chunk_rows, dtype=torch.int32, device=dev)
         nll_all = torch.empty(T, dtype=torch.float32, device=dev)
+        entropy_all = None if entropy_weight is None else torch.empty(T, dtype=torch.float32, device=dev)
         total = torch.zeros((), dtype=torch.float32, device=dev)
         first = True
         for r0 in range(0, T, chunk_rows):
             r1 = min(T, r0 + chunk_rows)
             rows = r1 - r0
-            fused = not (need_dx or need_dw) and gemm.ce_stats_gemm(x2[r0:r1], weight, tg[r0:r1], st[:, :rows],
-                                                                     best[:rows], 0, 0, 1.0)
+            fused = entropy_weight is None and not (need_dx or need_dw) and gemm.ce_stats_gemm(
+                x2[r0:r1], weight, tg[r0:r1], st[:, :rows], best[:rows], 0, 0, 1.0)
             if not fused:
                 if logits_buf is None:
                     logits_buf = torch.empty((chunk_rows, ld), dtype=torch.bfloat16, device=dev)
                 out_view = logits_buf[:rows].as_strided((rows, V), (ld, 1))
                 gemm.gemm(x2[r0:r1], weight, out=out_view)
+            if entropy_weight is not None:
+                logp, entropy_all[r0:r1], _, _, num = lp_ops._forward(out_view, tg[r0:r1], 0, 1.0, True)
+                nll = -logp
+            elif not fused:
                 rc = l.ob_ce_stats(_lib.ptr(out_view), ld, _lib.ptr(tg[r0:r1]), _lib.ptr(st[0]), _lib.ptr(st[1]),
                                    _lib.ptr(st[2]), _lib.ptr(st[3]), _lib.ptr(st[4]), _lib.ptr(best), rows, V, 0, 0, 1.0,
                                    _lib.stream())
                 _lib.check(rc, "ob_ce_stats")
-            lse = st[0, :rows] + torch.log(st[1, :rows])
-            nll = lse - st[3, :rows]
+            if entropy_weight is None:
+                lse = st[0, :rows] + torch.log(st[1, :rows])
+                nll = lse - st[3, :rows]
             nll_all[r0:r1] = nll
             loss_chunk, dl_dnll = loss_fn(nll, r0, r1)
             total += loss_chunk.sum()
+            if entropy_weight is not None:
+                total += (entropy_weight[r0:r1] * entropy_all[r0:r1]).sum()
             if need_dx or need_dw:
                 w_rows = dl_dnll.to(torch.float32).contiguous()
+            if (need_dx or need_dw) and entropy_weight is not None:
+                lp_ops._backward(out_view, tg[r0:r1], num, -w_rows, entropy_weight[r0:r1], 1.0, out=out_view)
+            elif need_dx or need_dw:
                 rc = l.ob_ce_grad(_lib.ptr(out_view), ld, _lib.ptr(tg[r0:r1]), _lib.ptr(lse.contiguous()), rows, V, 0, V,
                                   -(1 << 62), 0.0, None, 1.0, 0, 1.0, _lib.ptr(w_rows), _lib.stream())
                 _lib.check(rc, "ob_ce_grad")
-                if need_dx:
-                    gemm.gemm(out_view, weight, b_mn=True, out=dx[r0:r1])
-                if need_dw:
-                    gemm.gemm(out_view, x2[r0:r1], a_mn=True, b_mn=True, out=dw, accumulate=(not first) or first_acc)
+            if need_dx:
+                gemm.gemm(out_view, weight, b_mn=True, out=dx[r0:r1])
+            if need_dw:
+                gemm.gemm(out_view, x2[r0:r1], a_mn=True, b_mn=True, out=dw, accumulate=(not first) or first_acc)
             first = False
         ctx.save_for_backward(dx if need_dx else torch.empty(0), dw if (need_dw and mg is None) else torch.empty(0))
         ctx.x_shape = x.shape
         ctx.flags = (need_dx, need_dw and mg is None)
-        ctx.mark_non_differentiable(nll_all)
-        return total, nll_all
+        if entropy_weight is None:
+            ctx.mark_non_differentiable(nll_all)
+            return total, nll_all
+        ctx.mark_non_differentiable(nll_all, entropy_all)
+        return total, nll_all, entropy_all
 
     @staticmethod
-    def backward(ctx, dloss, _dnll):
+    def backward(ctx, dloss, *_):
         dx, dw = ctx.saved_tensors
         need_dx, need_dw = ctx.flags
         gx = (dx * dloss.to(dx.dtype)).view(ctx.x_shape) if need_dx else None
         gw = dw * dloss.to(dw.dtype) if need_dw else None
-        return gx, gw, None, None, None
+        return gx, gw, None, None, None, None
 
 
-def linear_token_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, loss_fn, chunk_rows: int = 4096):
+def linear_token_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, loss_fn, chunk_rows: int = 4096,
+                      entropy_weight: torch.Tensor | None = None):
     """``(sum_i loss_i, nll)`` where ``nll_i = -log softmax(x_i W^T)[target_i]`` and
     ``loss_fn(nll_chunk, r0, r1) -> (loss_chunk, dloss/dnll chunk)`` defines the per-token loss.
 
     The returned sum is differentiable with respect to ``x`` and ``weight`` (the gradient uses the
     derivative ``loss_fn`` reports, treated as exact); ``nll`` is detached. Every target must be a
     valid class: mask tokens through ``loss_fn`` (zero loss and zero derivative), not the target.
+
+    With ``entropy_weight`` (one fp32 number per token, treated as constant) the sum also holds
+    ``sum_i entropy_weight_i H_i``, ``H_i`` being the entropy of the token's distribution, and its gradient;
+    returns ``(sum, nll, entropy)`` then.
     """
+    if entropy_weight is not None:
+        entropy_weight = entropy_weight.detach().reshape(-1).to(torch.float32).contiguous()
+        if entropy_weight.shape[0] != targets.numel():
+            raise ValueError(f"entropy_weight has {entropy_weight.shape[0]} numbers for {targets.numel()} tokens")
     if x.is_cuda and x.dtype == torch.bfloat16 and weight.dtype == torch.bfloat16 and x.shape[-1] % 8 == 0:
-        return _LinearTokenLoss.apply(x, weight, targets, loss_fn, chunk_rows)
+        return _LinearTokenLoss.apply(x, weight, targets, loss_fn, chunk_rows, entropy_weight)
     logits = F.linear(x.reshape(-1, x.shape[-1]), weight).float()
     nll = F.cross_entropy(logits, targets.reshape(-1), reduction="none")
     loss_vals, dl = loss_fn(nll.detach(), 0, nll.numel())
     # same contract as the kernel path: the value comes from loss_fn, the gradient from its reported derivative
     total = loss_vals.sum().detach() + ((nll - nll.detach()) * dl.detach()).sum()
-    return total, nll.detach()
+    if entropy_weight is None:
+        return total, nll.detach()
+    entropy = lp_ops.token_logprobs(logits, targets.reshape(-1)).entropy
+    return total + (entropy_weight * entropy).sum(), nll.detach(), entropy.detach()
 
 
 class _SumGradOverGroup(torch.autograd.Function):

@@ -32,6 +32,11 @@ _HEAD_DIMS = (32, 64, 128, 256)
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
+def has_kernel(head_dim: int, dtype: torch.dtype) -> bool:
+    """Whether decode steps of this head dimension and model type run in the CUDA kernels."""
+    return head_dim in _HEAD_DIMS and dtype in (torch.bfloat16, torch.float16)
+
+
 def _strides(t: torch.Tensor) -> tuple[int, ...]:
     """Strides, 0 for dimensions of size 1 (whose stride means nothing)."""
     strides = t.stride()
@@ -243,7 +248,7 @@ def decode_attention_fp8(q: torch.Tensor, k_new: torch.Tensor | None, v_new: tor
     if window is not None and window < 0:
         raise ValueError(f"window must not be negative, got {window}")
     scale = scale if scale is not None else 1.0 / math.sqrt(hd)
-    if not (cache._kernels and dtype in (torch.bfloat16, torch.float16)):
+    if not (cache._kernels and has_kernel(hd, dtype)):
         return decode_attention_fp8_ref(q, k_new, v_new, cache, seq_lens, scale=scale, window=window)
     out = torch.empty(shape, dtype=dtype, device=cache._device)
     if B == 0 or Hq == 0:

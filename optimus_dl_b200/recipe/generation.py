@@ -5,7 +5,11 @@ The reference re-runs the full prefix for every new token, both in its ``generat
 (optimus_dl/recipe/serve/base.py). ``generate`` keeps that call contract (prompt ids in, new ids
 out, per-sequence EOS stop with padding, greedy / temperature / top-k / top-p) but runs one prefill
 and then single-token steps over per-layer caches: cached keys and values are read once per step
-by ``ops.decode.decode_attention`` and the next token comes from the fused sampler.
+by ``ops.decode.decode_attention`` and the next token comes from the fused sampler. With
+``kv_cache_dtype="fp8"`` the caches hold e4m3 codes with a scale for each 64 tokens and head
+(``ops.decode_fp8``): half the memory and half the bytes a step reads, at the codes' precision; the
+prompt itself is attended to unrounded. ``logprobs=k`` also gives every new token's log probability,
+the entropy of its distribution and the ``k`` most likely alternatives (``ops.logprobs``).
 
 On CUDA the decode step's launch sequence is identical from step to step (lengths and positions
 live in device tensors), so it is captured once into a CUDA graph and replayed.
@@ -21,16 +25,21 @@ import torch
 import torch.nn as nn
 
 from ..ops import decode as dec_ops
+from ..ops import decode_fp8 as fp8_ops
+from ..ops.logprobs import MAX_TOP_K, TokenLogprobs, token_logprobs
 
 logger = logging.getLogger(__name__)
 
 
 class LayerKV:
-    """One attention layer's cache ``[B, Tmax, Hk, hd]`` plus the session state shared by all layers."""
+    """One attention layer's cache ``[B, Tmax, Hk, hd]`` plus the session state shared by all layers; ``fp8`` is the
+    cache when it is held in 8 bits (``k`` and ``v`` are its codes then)."""
 
-    def __init__(self, session: "DecodeSession", k: torch.Tensor, v: torch.Tensor):
+    def __init__(self, session: "DecodeSession", k: torch.Tensor, v: torch.Tensor,
+                 fp8: fp8_ops.Fp8KVCache | None = None):
         self._s = session
         self.k, self.v = k, v
+        self.fp8 = fp8
         self.workspace: dict = {}
 
     @property
@@ -76,10 +85,18 @@ def supports_kv_cache(model: nn.Module) -> bool:
     return bool(_attention_modules(m)) and getattr(m, "_tp", None) is None
 
 
-class DecodeSession:
-    """Caches for ``batch`` sequences of up to ``max_len`` tokens, attached to the model's attention layers."""
+def check_kv_cache_dtype(name: str | None) -> None:
+    if name not in (None, "fp8"):
+        raise ValueError(f"kv_cache_dtype must be null or 'fp8', got {name!r}")
 
-    def __init__(self, model: nn.Module, batch: int, max_len: int, dtype: torch.dtype | None = None):
+
+class DecodeSession:
+    """Caches for ``batch`` sequences of up to ``max_len`` tokens, attached to the model's attention layers.
+    ``kv_cache_dtype``: None (``dtype``, the model's by default) or ``"fp8"``."""
+
+    def __init__(self, model: nn.Module, batch: int, max_len: int, dtype: torch.dtype | None = None,
+                 kv_cache_dtype: str | None = None):
+        check_kv_cache_dtype(kv_cache_dtype)
         self.model = unwrap(model)
         self.attn = _attention_modules(self.model)
         assert self.attn, "model has no cache-capable attention layers"
@@ -94,7 +111,15 @@ class DecodeSession:
         # enough CTAs for about four full waves (three resident per SM), but at least two 64-token tiles per split
         self.n_splits = max(1, min(32, (12 * sms + ctas - 1) // ctas, (max_len + 127) // 128))
         self.layers = []
+        if kv_cache_dtype == "fp8" and self.device.type == "cuda":
+            for a in self.attn:
+                if not fp8_ops.has_kernel(a.head_dim, self.dtype):
+                    raise ValueError(f"the 8-bit cache has no kernel for head dimension {a.head_dim} and {self.dtype}")
         for a in self.attn:
+            if kv_cache_dtype == "fp8":
+                c = fp8_ops.fp8_kv_cache(batch, self.max_len, a.n_kv_head, a.head_dim, device=self.device)
+                self.layers.append(LayerKV(self, c.k, c.v, c))
+                continue
             # stored head-major ([B, Hk, T, hd]: one contiguous stream per (sequence, head)), used as [B, T, Hk, hd]
             shape = (batch, a.n_kv_head, max_len, a.head_dim)
             self.layers.append(LayerKV(self, torch.zeros(shape, dtype=self.dtype, device=self.device).permute(0, 2, 1, 3),
@@ -173,8 +198,15 @@ class DecodeSession:
 def generate_stream(model: nn.Module, input_ids: torch.Tensor, max_new_tokens: int, temperature: float = 1.0,
                     top_k: int | None = None, top_p: float | None = None, greedy: bool = False,
                     eos_token_id: int | None = None, use_kv_cache: bool = True, seed: int = 0,
-                    generator: torch.Generator | None = None, use_graph: bool = True) -> Iterator[torch.Tensor]:
-    """Yield the new tokens ``[B]`` step by step (finished sequences yield the padding id)."""
+                    generator: torch.Generator | None = None, use_graph: bool = True,
+                    kv_cache_dtype: str | None = None, logprobs: int | None = None
+                    ) -> Iterator[torch.Tensor] | Iterator[tuple[torch.Tensor, TokenLogprobs]]:
+    """Yield the new tokens ``[B]`` step by step (finished sequences yield the padding id). With ``logprobs`` (0 or
+    more alternatives) every step yields ``(tokens, TokenLogprobs)``, the log probabilities being the model's own:
+    before temperature, top-k and top-p. ``kv_cache_dtype`` applies wherever a cache is used."""
+    check_kv_cache_dtype(kv_cache_dtype)
+    if logprobs is not None and not 0 <= logprobs <= MAX_TOP_K:
+        raise ValueError(f"logprobs must be between 0 and {MAX_TOP_K}, got {logprobs}")
     root = unwrap(model)
     is_module = isinstance(root, nn.Module)      # any callable returning {"logits": ...} can be sampled from, uncached
     was_training = root.training if is_module else False
@@ -188,17 +220,18 @@ def generate_stream(model: nn.Module, input_ids: torch.Tensor, max_new_tokens: i
     finished = torch.zeros(B, dtype=torch.bool, device=input_ids.device)
     pick = lambda lg, i: dec_ops.sample(lg, temperature, top_k, top_p, greedy, seed=seed, offset=i,  # noqa: E731
                                         generator=generator)
+    step = lambda nxt, lg: nxt if logprobs is None else (nxt, token_logprobs(lg, nxt, top_k=logprobs))  # noqa: E731
     try:
         cached = use_kv_cache and is_module and supports_kv_cache(root) and T0 + max_new_tokens <= limit
         if cached:
-            with DecodeSession(root, B, T0 + max_new_tokens) as sess:
+            with DecodeSession(root, B, T0 + max_new_tokens, kv_cache_dtype=kv_cache_dtype) as sess:
                 logits = sess.prefill(input_ids)
                 for i in range(max_new_tokens):
                     nxt = pick(logits, i)
                     if eos_token_id is not None:
                         nxt = torch.where(finished, torch.full_like(nxt, pad), nxt)
                         finished |= nxt == eos_token_id
-                    yield nxt
+                    yield step(nxt, logits)
                     if i + 1 == max_new_tokens or (eos_token_id is not None and bool(finished.all())):
                         break
                     logits = sess.step(nxt, use_graph=use_graph)
@@ -211,7 +244,7 @@ def generate_stream(model: nn.Module, input_ids: torch.Tensor, max_new_tokens: i
                 if eos_token_id is not None:
                     nxt = torch.where(finished, torch.full_like(nxt, pad), nxt)
                     finished |= nxt == eos_token_id
-                yield nxt
+                yield step(nxt, logits)
                 if eos_token_id is not None and bool(finished.all()):
                     break
                 cur = torch.cat([cur, nxt[:, None]], dim=1)
@@ -221,15 +254,28 @@ def generate_stream(model: nn.Module, input_ids: torch.Tensor, max_new_tokens: i
 
 
 @torch.no_grad()
-def generate(model: nn.Module, input_ids: torch.Tensor, max_new_tokens: int, **kwargs: Any) -> torch.Tensor:
-    """New tokens ``[B, n]`` (``n <= max_new_tokens``; stops early once every sequence hit EOS)."""
-    toks = [t[:, None] for t in generate_stream(model, input_ids, max_new_tokens, **kwargs)]
-    if not toks:
-        return torch.empty((input_ids.shape[0], 0), dtype=torch.long, device=input_ids.device)
-    return torch.cat(toks, dim=1)
+def generate(model: nn.Module, input_ids: torch.Tensor, max_new_tokens: int,
+             **kwargs: Any) -> torch.Tensor | tuple[torch.Tensor, TokenLogprobs]:
+    """New tokens ``[B, n]`` (``n <= max_new_tokens``; stops early once every sequence hit EOS); with ``logprobs`` a
+    tuple of them and their ``TokenLogprobs`` (``[B, n]``, alternatives ``[B, n, k]``)."""
+    steps = list(generate_stream(model, input_ids, max_new_tokens, **kwargs))
+    k = kwargs.get("logprobs")
+    toks = steps if k is None else [t for t, _ in steps]
+    B, dev = input_ids.shape[0], input_ids.device
+    out = torch.stack(toks, dim=1) if toks else torch.empty((B, 0), dtype=torch.long, device=dev)
+    if k is None:
+        return out
+    rows = [r for _, r in steps]
+    if not rows:
+        none = torch.empty((B, 0), device=dev)
+        return out, TokenLogprobs(none, none, none[..., None].expand(B, 0, k) if k else None,
+                                  out[..., None].expand(B, 0, k) if k else None)
+    join = lambda name: torch.stack([getattr(r, name) for r in rows], dim=1)                   # noqa: E731
+    return out, TokenLogprobs(join("logp"), join("entropy"), join("top_logp") if k else None,
+                              join("top_ids") if k else None)
 
 
 @contextlib.contextmanager
-def decode_session(model: nn.Module, batch: int, max_len: int):
-    with DecodeSession(model, batch, max_len) as s:
+def decode_session(model: nn.Module, batch: int, max_len: int, kv_cache_dtype: str | None = None):
+    with DecodeSession(model, batch, max_len, kv_cache_dtype=kv_cache_dtype) as s:
         yield s

@@ -92,18 +92,29 @@ class GRPORecipe(TrainingIterationMixin):
     @torch.no_grad()
     def rollout(self, model: torch.nn.Module, prompts: torch.Tensor, step: int) -> tuple[torch.Tensor, torch.Tensor]:
         """``prompts [P, L]`` -> sequences ``[P * G, L + n]`` and the mask ``[P * G, n]`` of tokens that count."""
+        return self.rollout_scored(model, prompts, step, False)[:2]
+
+    @torch.no_grad()
+    def rollout_scored(self, model: torch.nn.Module, prompts: torch.Tensor, step: int,
+                       with_logprobs: bool = True) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+        """:meth:`rollout`, with the log probabilities ``[P * G, n]`` the completions were sampled under (at
+        temperature 1, from the decode steps' logits) as a third part."""
         g = self.cfg.grpo
         eng = getattr(unwrap(model), "_sharding_engine", None)
         if eng is not None:
             eng.gather_all()
         rep = prompts.repeat_interleave(int(g.group_size), dim=0)
-        outs = []
+        outs, scores = [], []
         bs = max(int(g.rollout_batch_size), 1)
         for s in range(0, rep.shape[0], bs):
             chunk = rep[s:s + bs]
             new = generate(model, chunk, int(g.max_new_tokens), temperature=float(g.temperature), top_k=g.get("top_k"),
                            top_p=g.get("top_p"), eos_token_id=g.get("eos_token_id"), use_kv_cache=bool(g.use_kv_cache),
-                           seed=int(self.cfg.common.seed) * 7919 + step * 131 + s, use_graph=bool(g.use_cuda_graph))
+                           seed=int(self.cfg.common.seed) * 7919 + step * 131 + s, use_graph=bool(g.use_cuda_graph),
+                           kv_cache_dtype=g.get("kv_cache_dtype"), logprobs=0 if with_logprobs else None)
+            if with_logprobs:
+                new, scored = new
+                scores.append(torch.nn.functional.pad(scored.logp, (0, int(g.max_new_tokens) - new.shape[1])))
             if new.shape[1] < int(g.max_new_tokens):  # every sequence of the chunk ended early
                 pad = torch.full((new.shape[0], int(g.max_new_tokens) - new.shape[1]), int(g.eos_token_id or 0),
                                  dtype=new.dtype, device=new.device)
@@ -115,7 +126,7 @@ class GRPORecipe(TrainingIterationMixin):
         if eos is not None:
             ended = (completions == int(eos)).int().cumsum(-1)
             mask = (ended - (completions == int(eos)).int()) == 0   # keep tokens up to and including the first EOS
-        return torch.cat([rep, completions], dim=1), mask
+        return torch.cat([rep, completions], dim=1), mask, torch.cat(scores, dim=0) if with_logprobs else None
 
     @torch.no_grad()
     def token_logprobs(self, model: torch.nn.Module, seqs: torch.Tensor, prompt_len: int) -> torch.Tensor:
@@ -142,7 +153,8 @@ class GRPORecipe(TrainingIterationMixin):
         root = unwrap(model)
         mb = max(int(g.micro_batch_size), 1)
         n_tok = float(mask.sum().clamp(min=1))
-        sums = {"loss": 0.0, "kl_sum": 0.0, "clipped_sum": 0.0, "ratio_sum": 0.0}
+        sums = {"loss": 0.0, "kl_sum": 0.0, "clipped_sum": 0.0, "ratio_sum": 0.0, "entropy_sum": 0.0}
+        entropy_coef = float(g.get("entropy_coef") or 0.0)
         optimizer.zero_grad()
         model.train()
         starts = list(range(0, seqs.shape[0], mb))
@@ -163,16 +175,21 @@ class GRPORecipe(TrainingIterationMixin):
 
             with accumulation_context(model, i == len(starts) - 1):
                 hidden = model(x[:, :-1], skip_lm_head=True)["hidden"][:, prompt_len - 1:]
-                loss, _ = ce_ops.linear_token_loss(hidden.reshape(-1, hidden.shape[-1]), root.lm_head.weight, tg, loss_fn)
+                # the objective gains entropy_coef * entropy, averaged over the tokens that count
+                weight = m.float() * (-entropy_coef / n_tok) if entropy_coef else None
+                loss, _, *entropy = ce_ops.linear_token_loss(hidden.reshape(-1, hidden.shape[-1]), root.lm_head.weight, tg,
+                                                             loss_fn, entropy_weight=weight)
                 loss.backward()
             sums["loss"] += float(loss.detach())
+            if entropy:
+                sums["entropy_sum"] += float((entropy[0] * m).sum())
             for st in stats_box:
                 for k in ("kl_sum", "clipped_sum", "ratio_sum"):
                     sums[k] += float(st[k])
         self._optimizer_step(model, optimizer, None, self.cfg.optimization.get("clip_grad_norm"))
         optimizer.zero_grad()
         return {"loss": sums["loss"], "kl": sums["kl_sum"] / n_tok, "clip_frac": sums["clipped_sum"] / n_tok,
-                "ratio": sums["ratio_sum"] / n_tok}
+                "ratio": sums["ratio_sum"] / n_tok, **({"entropy": sums["entropy_sum"] / n_tok} if entropy_coef else {})}
 
     # ------------------------------------------------------------------ run
     def run(self) -> None:
@@ -204,13 +221,14 @@ class GRPORecipe(TrainingIterationMixin):
                 with meters_group("train", log_freq=int(c.log_freq)) as should_log:
                     t0 = time.perf_counter()
                     prompts = prompt_src(it, n_local, L, device)
-                    seqs, mask = self.rollout(model, prompts, it)
+                    seqs, mask, old_logp = self.rollout_scored(model, prompts, it, bool(g.get("rollout_logprobs", False)))
                     if device.type == "cuda":
                         torch.cuda.synchronize(device)
                     t_roll = time.perf_counter() - t0
                     rewards = reward_fn(seqs[:, :L], seqs[:, L:], mask)
                     adv = group_advantages(rewards, int(g.group_size), float(g.advantage_eps))
-                    old_logp = self.token_logprobs(model, seqs, L)
+                    if old_logp is None:
+                        old_logp = self.token_logprobs(model, seqs, L)
                     ref_logp = self.token_logprobs(ref, seqs, L) if ref is not None else None
                     stats = {}
                     for _ in range(max(int(g.updates_per_rollout), 1)):
@@ -227,6 +245,8 @@ class GRPORecipe(TrainingIterationMixin):
                     log_averaged("kl", stats["kl"], round=6)
                     log_averaged("clip_frac", stats["clip_frac"], round=5)
                     log_averaged("ratio", stats["ratio"], round=5)
+                    if "entropy" in stats:
+                        log_averaged("entropy", stats["entropy"], round=5)
                     log_summed("generated_tokens", n_gen)
                     log_averaged("perf/rollout_s", t_roll, round=3)
                     log_averaged("perf/step_s", t_all, round=3)

@@ -22,6 +22,9 @@ def main() -> None:
     ap.add_argument("--micro-batch", type=int, default=8)
     ap.add_argument("--steps", type=int, default=2)
     ap.add_argument("--warmup", type=int, default=1)
+    ap.add_argument("--kv-cache-dtype", default=None, choices=["fp8"], help="hold the rollout's cache in 8 bits")
+    ap.add_argument("--rollout-logprobs", action="store_true",
+                    help="take sampling-time log probabilities from the decode steps")
     args = ap.parse_args()
 
     from ...core import conf
@@ -40,7 +43,8 @@ def main() -> None:
         "model_transforms": [{"_name": "fully_shard"}],
         "grpo": {"num_prompts": args.prompts * world, "prompt_length": args.prompt_length, "group_size": args.group_size,
                  "max_new_tokens": args.new_tokens, "micro_batch_size": args.micro_batch,
-                 "rollout_batch_size": args.prompts * args.group_size},
+                 "rollout_batch_size": args.prompts * args.group_size, "kv_cache_dtype": args.kv_cache_dtype,
+                 "rollout_logprobs": args.rollout_logprobs},
         "optimization": {"iterations": 1, "optimizer": {"_name": "adamw", "lr": 1e-6, "weight_decay": 0.0}},
     })
     recipe = build("grpo_recipe", non_resolving_instantiate(cfg))
@@ -64,11 +68,12 @@ def main() -> None:
     for it in range(total_steps):
         prompts = src(it, args.prompts, L, device)
         e0 = ev()
-        seqs, mask = recipe.rollout(model, prompts, it)
+        seqs, mask, old = recipe.rollout_scored(model, prompts, it, args.rollout_logprobs)
         e1 = ev()
         rewards = reward_fn(seqs[:, :L], seqs[:, L:], mask)
         adv = group_advantages(rewards, int(g.group_size))
-        old = recipe.token_logprobs(model, seqs, L)
+        if old is None:
+            old = recipe.token_logprobs(model, seqs, L)
         refp = recipe.token_logprobs(ref, seqs, L) if ref is not None else None
         e2 = ev()
         recipe.train_on_rollout(model, optimizer, seqs, mask, adv, old, refp, L)
@@ -87,7 +92,7 @@ def main() -> None:
         step_ms = float(t.sum())
         print(json.dumps({
             "metric": "GRPO step (rollout + log-probs + update), device-timed, max over ranks", "model": args.model,
-            "n_gpus": world, "sequences_per_step": n_seq, "prompt_length": L, "new_tokens": args.new_tokens,
+            "kv_cache_dtype": args.kv_cache_dtype, "rollout_logprobs": args.rollout_logprobs, "n_gpus": world, "sequences_per_step": n_seq, "prompt_length": L, "new_tokens": args.new_tokens,
             "rollout_ms": round(float(t[0]), 1), "logprobs_ms": round(float(t[1]), 1), "update_ms": round(float(t[2]), 1),
             "step_ms": round(step_ms, 1), "generated_tokens_per_s_rollout": round(gen / float(t[0]) * 1e3, 1),
             "decode_ms_per_token_step": round(float(t[0]) / args.new_tokens, 3),

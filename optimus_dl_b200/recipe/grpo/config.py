@@ -39,12 +39,16 @@ class GRPOSection:
     eos_token_id: int | None = None
     clip_eps: float = 0.2
     kl_coef: float = 0.04
+    entropy_coef: float = 0.0      # weight of the policy's entropy, added to the objective (0 = not computed)
     updates_per_rollout: int = 1
     micro_batch_size: int = 8      # sequences per forward/backward
     rollout_batch_size: int = 64   # sequences decoded together
     advantage_eps: float = 1e-6
     use_kv_cache: bool = True
     use_cuda_graph: bool = True
+    kv_cache_dtype: str | None = None   # "fp8": rollouts read an 8-bit cache (half its memory and traffic)
+    rollout_logprobs: bool = False      # sampling-time log probabilities from the decode steps' own logits (with an
+                                        # 8-bit cache: of the distribution that was sampled) instead of a forward pass
     reward: Any = field(default_factory=lambda: {"_name": "even_fraction"})
     prompts: Any = field(default_factory=lambda: {"_name": "uniform_random"})
 

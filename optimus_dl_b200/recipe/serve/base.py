@@ -6,7 +6,8 @@ streaming; temperature 0 means greedy; prompts longer than the model's context a
 the left). Differences by design: tokens come from ``recipe.generation`` (one prefill, then
 single-token steps on the cached keys / values instead of a full forward per token), ``top_p`` is
 accepted, ``usage`` reports real token counts, ``/v1/completions`` can stream too, and
-``GET /health`` answers liveness probes. The server handles one request at a time
+``GET /health`` answers liveness probes, and answers that are not streamed can carry log probabilities (``logprobs``
+of a completion; ``logprobs`` and ``top_logprobs`` of a chat). The server handles one request at a time
 (``http.server.HTTPServer``), as the reference does.
 """
 
@@ -16,13 +17,14 @@ import json
 import logging
 import time
 from http.server import BaseHTTPRequestHandler, HTTPServer
-from typing import Any, Iterator
+from typing import Any, Iterator, NamedTuple
 
 import torch
 
 from ...checkpoint import build_checkpoint_manager
 from ...core.dtype import str_to_dtype
 from ...models import build_model
+from ...ops.logprobs import TokenLogprobs
 from ...tokenizer import build_tokenizer
 from ..generation import generate_stream, unwrap
 from . import models as M
@@ -117,9 +119,11 @@ class RequestHandler(BaseHTTPRequestHandler):
             self._sse(last.model_dump_json())
             self._sse("[DONE]")
             return
-        text = recipe.generate(prompt, **kw)
+        text = recipe.generate(prompt, logprobs=req.alternatives(), **kw)
+        scored = None if recipe.last_logprobs is None else completion_logprobs(recipe.last_logprobs, len(prompt))
         resp = M.CompletionResponse(id=rid, object="text_completion", created=now, model=req.model,
-                                    choices=[M.Choice(index=0, text=text, finish_reason=recipe.last_finish)],
+                                    choices=[M.Choice(index=0, text=text, logprobs=scored,
+                                                      finish_reason=recipe.last_finish)],
                                     usage=recipe.last_usage)
         self._json(200, resp.model_dump_json())
 
@@ -145,12 +149,35 @@ class RequestHandler(BaseHTTPRequestHandler):
             self._sse(done.model_dump_json())
             self._sse("[DONE]")
             return
-        text = recipe.generate(req.messages, **kw)
+        text = recipe.generate(req.messages, logprobs=req.alternatives(), **kw)
+        scored = None if recipe.last_logprobs is None else chat_logprobs(recipe.last_logprobs)
         resp = M.ChatCompletionResponse(
             id=rid, object="chat.completion", created=now, model=req.model,
-            choices=[M.ChatChoice(index=0, message=M.ChatMessage(role="assistant", content=text),
+            choices=[M.ChatChoice(index=0, message=M.ChatMessage(role="assistant", content=text), logprobs=scored,
                                   finish_reason=recipe.last_finish)], usage=recipe.last_usage)
         self._json(200, resp.model_dump_json())
+
+
+class ScoredToken(NamedTuple):
+    text: str
+    logprob: float
+    top: list[tuple[str, float]]       # alternatives, most likely first
+
+
+def completion_logprobs(tokens: list[ScoredToken], offset: int) -> dict:
+    """The ``logprobs`` object of a text completion; offsets count characters of the prompt and of the token texts."""
+    offsets, at = [], offset
+    for t in tokens:
+        offsets.append(at)
+        at += len(t.text)
+    return {"tokens": [t.text for t in tokens], "token_logprobs": [t.logprob for t in tokens],
+            "top_logprobs": [dict(reversed(t.top)) for t in tokens], "text_offset": offsets}
+
+
+def chat_logprobs(tokens: list[ScoredToken]) -> dict:
+    """The ``logprobs`` object of a chat completion."""
+    one = lambda text, lp: {"token": text, "logprob": lp, "bytes": list(text.encode("utf-8"))}  # noqa: E731
+    return {"content": [{**one(t.text, t.logprob), "top_logprobs": [one(*alt) for alt in t.top]} for t in tokens]}
 
 
 class ServeRecipe:
@@ -160,6 +187,7 @@ class ServeRecipe:
         self.tokenizer = None
         self.device: torch.device | None = None
         self.last_finish = "length"
+        self.last_logprobs: list[ScoredToken] | None = None
         self.last_usage: dict = {"prompt_tokens": 0, "completion_tokens": 0, "total_tokens": 0}
         self._requests = 0
         self.httpd: HTTPServer | None = None
@@ -198,9 +226,11 @@ class ServeRecipe:
 
     @torch.no_grad()
     def generate_stream(self, prompt_or_messages: str | list, max_new_tokens: int = 50, temperature: float = 1.0,
-                        top_k: int | None = None, top_p: float | None = None) -> Iterator[str]:
+                        top_k: int | None = None, top_p: float | None = None,
+                        logprobs: int | None = None) -> Iterator[str]:
         """Yield text pieces. The full token list is re-decoded every step and only the new suffix
-        is emitted, which is safe across multi-byte / multi-token characters."""
+        is emitted, which is safe across multi-byte / multi-token characters. With ``logprobs`` the tokens' log
+        probabilities and that many alternatives are left in ``last_logprobs``."""
         ids = self._encode(prompt_or_messages)
         root = unwrap(self.model)
         limit = int(getattr(root.config, "sequence_length", None) or getattr(root.config, "block_size", 0) or 0)
@@ -216,16 +246,23 @@ class ServeRecipe:
         out: list[int] = []
         emitted = ""
         self.last_finish = "length"
+        vocab = int(getattr(root.config, "vocab_size", 0) or 0)
+        self.last_logprobs = None if logprobs is None else []
         stream = generate_stream(self.model, x, max_new_tokens, temperature=max(float(temperature), 0.0), top_k=top_k,
                                  top_p=top_p, greedy=temperature <= 0, eos_token_id=None,
                                  use_kv_cache=bool(self.cfg.common.get("use_kv_cache", True)),
-                                 seed=int(self.cfg.common.get("seed", 0)) + self._requests)
-        for tok in stream:
+                                 seed=int(self.cfg.common.get("seed", 0)) + self._requests,
+                                 kv_cache_dtype=self.cfg.common.get("kv_cache_dtype"),
+                                 logprobs=None if logprobs is None else min(logprobs, vocab or logprobs))
+        for step in stream:
+            tok, scored = (step, None) if logprobs is None else step
             t = int(tok[0])
             if eos is not None and t == eos:
                 self.last_finish = "stop"
                 break
             out.append(t)
+            if scored is not None:
+                self.last_logprobs.append(self._scored_token(t, scored))
             text = self.tokenizer.decode(out)
             if len(text) > len(emitted) and not text.endswith("�"):
                 yield text[len(emitted):]
@@ -235,9 +272,16 @@ class ServeRecipe:
             yield text[len(emitted):]
         self.last_usage = {"prompt_tokens": len(ids), "completion_tokens": len(out), "total_tokens": len(ids) + len(out)}
 
+    def _scored_token(self, token: int, scored: TokenLogprobs) -> ScoredToken:
+        text = lambda i: self.tokenizer.decode([i])                                             # noqa: E731
+        floor = lambda x: max(x, -9999.0)      # JSON has no -inf                               # noqa: E731
+        top = [] if scored.top_ids is None else [(text(i), floor(x)) for i, x in zip(scored.top_ids[0].tolist(),
+                                                                                    scored.top_logp[0].tolist())]
+        return ScoredToken(text(token), floor(float(scored.logp[0])), top)
+
     def generate(self, prompt_or_messages: str | list, max_new_tokens: int = 50, temperature: float = 1.0,
-                 top_k: int | None = None, top_p: float | None = None) -> str:
-        return "".join(self.generate_stream(prompt_or_messages, max_new_tokens, temperature, top_k, top_p))
+                 top_k: int | None = None, top_p: float | None = None, logprobs: int | None = None) -> str:
+        return "".join(self.generate_stream(prompt_or_messages, max_new_tokens, temperature, top_k, top_p, logprobs))
 
     # ------------------------------------------------------------------ server
     def make_server(self) -> HTTPServer:

@@ -16,6 +16,7 @@ class ServeCommonConfig:
     device: str = "auto"                 # cuda, cpu or auto
     dtype: str | None = None             # cast the served model (default: bf16 on CUDA, unchanged on CPU)
     use_kv_cache: bool = True
+    kv_cache_dtype: str | None = None    # "fp8": hold the key / value cache in 8 bits
     seed: int = 0
 
 

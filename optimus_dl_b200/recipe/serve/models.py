@@ -5,7 +5,7 @@ from __future__ import annotations
 
 from typing import Literal
 
-from pydantic import BaseModel, Field
+from pydantic import BaseModel, Field, model_validator
 
 DEFAULT_MODEL_NAME = "optimus-dl-model"
 
@@ -19,12 +19,32 @@ class _Sampling(BaseModel):
     stream: bool = False
 
 
+    def alternatives(self) -> int | None:
+        """Alternatives per token that the answer lists, None without log probabilities."""
+        raise NotImplementedError
+
+    @model_validator(mode="after")
+    def _no_streamed_logprobs(self):
+        if self.stream and self.alternatives() is not None:
+            raise ValueError("log probabilities are not streamed: use stream=false")
+        return self
+
+
 class ChatCompletionRequest(_Sampling):
     messages: list[dict]
+    logprobs: bool = False
+    top_logprobs: int | None = Field(default=None, ge=0, le=20)
+
+    def alternatives(self) -> int | None:
+        return (self.top_logprobs or 0) if self.logprobs else None
 
 
 class CompletionRequest(_Sampling):
     prompt: str | list[str]
+    logprobs: int | None = Field(default=None, ge=0, le=20)
+
+    def alternatives(self) -> int | None:
+        return self.logprobs
 
 
 class ChatMessage(BaseModel):
@@ -51,6 +71,7 @@ class CompletionResponse(BaseModel):
 class ChatChoice(BaseModel):
     index: int
     message: ChatMessage
+    logprobs: dict | None = None
     finish_reason: str | None = None
 
 
