@@ -269,6 +269,7 @@ def bench_attention(t: Timer, cases, library_rows: bool = True) -> None:
 
 def bench_decode(t: Timer, cases) -> None:
     from . import decode as D
+    from . import decode_fp8 as D8
 
     for B, T, Hq, Hk, hd in cases:
         kc = torch.randn(B, Hk, T, hd, device="cuda").bfloat16().permute(0, 2, 1, 3)   # head-major storage
@@ -283,6 +284,33 @@ def bench_decode(t: Timer, cases) -> None:
         ws: dict = {}
         ms = t(lambda: D.decode_attention(q, kn, vn, kc, vc, lens, n_splits=splits, workspace=ws))
         _emit("decode_attention", dict(B=B, T=T, Hq=Hq, Hk=Hk, hd=hd, splits=splits), ms, bytes_=2.0 * B * T * Hk * hd * 2)
+        # the same step over the cache held in 8 bits, and the write of the whole prompt into it
+        cache = D8.fp8_kv_cache(B, T, Hk, hd, device="cuda")
+        ms_w = t(lambda: D8.append_kv_fp8(kc, vc, cache, lens))
+        _emit("append_kv_fp8", dict(B=B, T=T, Hk=Hk, hd=hd), ms_w, bytes_=2.0 * B * T * Hk * hd * 3)
+        ms8 = t(lambda: D8.decode_attention_fp8(q, kn, vn, cache, lens))
+        _emit("decode_attention_fp8", dict(B=B, T=T, Hq=Hq, Hk=Hk, hd=hd), ms8, bytes_=2.0 * B * T * Hk * (hd + 4 / 64),
+              vs_bf16_cache=round(ms / ms8, 3))
+
+
+def bench_logprobs(t: Timer, cases) -> None:
+    """Log probabilities with entropy from logits; with alternatives; with the gradient (logits read twice, written once)."""
+    from . import logprobs as LP
+
+    for rows, V, dtype in cases:
+        z = (torch.randn(rows, V, device="cuda") * 3).to(dtype)
+        tg = torch.randint(0, V, (rows,), device="cuda")
+        size = float(rows) * V * z.element_size()
+        for k in (0, 20):
+            _emit("token_logprobs", dict(rows=rows, V=V, dtype=str(dtype)[6:], top_k=k),
+                  t(lambda: LP.token_logprobs(z, tg, top_k=k)), bytes_=size)
+        zg, one = z.requires_grad_(True), torch.ones(rows, device="cuda")
+
+        def both():
+            r = LP.token_logprobs(zg, tg)
+            torch.autograd.grad([r.logp, r.entropy], [zg], [one, one])
+
+        _emit("token_logprobs_fwd_bwd", dict(rows=rows, V=V, dtype=str(dtype)[6:]), t(both), bytes_=3 * size)
 
 
 def bench_sampler(t: Timer, cases) -> None:
@@ -564,7 +592,8 @@ def _lib_check(dev) -> None:
 
 def main() -> None:
     ap = argparse.ArgumentParser()
-    ap.add_argument("--op", required=True, choices=["gemm_bf16", "gemm_skinny", "gemm_swiglu_bwd", "linear_ce_stats", "gemm_fp8", "attention", "decode", "sampler", "elementwise",
+    ap.add_argument("--op", required=True, choices=["gemm_bf16", "gemm_skinny", "gemm_swiglu_bwd", "linear_ce_stats", "gemm_fp8", "attention", "decode", "sampler", "logprobs",
+                                                    "elementwise",
                                                     "tp_ag_gemm", "tp_gemm_rs", "tp_ag_gemm_fp8", "tp_gemm_rs_fp8",
                                                     "fsdp_ag_gemm", "fsdp_rs_adamw"])
     ap.add_argument("--iters", type=int, default=20)
@@ -599,6 +628,9 @@ def main() -> None:
         bench_elementwise(t)
     elif args.op == "sampler":
         bench_sampler(t, [(64, 151936)] if args.small else [(64, 151936), (512, 151936)])
+    elif args.op == "logprobs":
+        bench_logprobs(t, [(64, 151936, torch.bfloat16)] if args.small else
+                       [(64, 151936, torch.bfloat16), (1000, 50257, torch.float32), (4096, 128256, torch.bfloat16)])
     elif args.op in ("fsdp_ag_gemm", "fsdp_rs_adamw"):
         # one Llama-3-8B block: 8192 tokens, d_model 4096, 32 / 8 heads of 128, FFN 14336
         bench_fsdp(args.op, [(8192, 4096, 32, 8, 128, 14336)])
