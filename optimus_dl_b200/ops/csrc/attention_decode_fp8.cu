@@ -175,7 +175,8 @@ __global__ void __launch_bounds__(THREADS, CTAS<HD, NT>) decode_kernel(const __g
   auto* slots = reinterpret_cast<Slot<HD, NT>*>(smem_raw);               // [2 * WARPS]: entered in the middle, left unfinished
   int* cum = reinterpret_cast<int*>(slots + 2 * WARPS);                  // [B + 1] units per head, summed up
   int* lens = cum + p.B + 1;                                             // [B]
-  __shared__ int tag[2 * WARPS];
+  __shared__ int tag[2 * WARPS];         // the slots' segments, -1 = empty
+  __shared__ int2 where[2 * WARPS], crossing[2];
   __shared__ int scan[WARPS + 1];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int HC = p.Hk * p.chunks;
@@ -202,6 +203,7 @@ __global__ void __launch_bounds__(THREADS, CTAS<HD, NT>) decode_kernel(const __g
   }
   if (lane == 31) scan[warp + 1] = incl;
   if (tid < 2 * WARPS) tag[tid] = -1;
+  if (tid < 2) crossing[tid] = make_int2(-1, 0);
   if (tid == 0) { scan[0] = 0; cum[0] = 0; }
   __syncthreads();
   int before = incl - mine;
@@ -444,7 +446,15 @@ __global__ void __launch_bounds__(THREADS, CTAS<HD, NT>) decode_kernel(const __g
         }
         if (!complete && g == 0) { part.m[h] = m[nt][c]; part.l[h] = sum; }
       }
-    if (!complete && lane == 0) tag[2 * warp + which] = b * HC + hc;
+    if (!complete && lane == 0) {
+      // where the segment lies: its units are [s0, s1)
+      const long long s0 = ua + done - u0, s1 = s0 + n;
+      const bool starts = s0 >= A, inside = starts && s1 <= E;
+      tag[2 * warp + which] = b * HC + hc;
+      where[2 * warp + which] = make_int2(b * p.Hq + h0, heads | inside << 8 | starts << 9);
+      // joined in this CTA for good, or with the CTAs behind that hold units up to s1
+      if (!inside) crossing[starts] = make_int2(b * HC + hc, starts ? (int)quotient(s1 - 1, per) - (int)blockIdx.x : 0);
+    }
     done += u1 - u0;
     if (done < count) {
       un = 0;
@@ -456,34 +466,29 @@ __global__ void __launch_bounds__(THREADS, CTAS<HD, NT>) decode_kernel(const __g
   }
   __syncthreads();
 
-  // Join the parts of each segment inside the CTA, a warp for each segment and head: lane j holds the reference and sum of slot j,
-  // every lane HD / 32 dimensions.
+  // Join the parts of each segment inside the CTA, a warp for each segment and head: lane j holds the reference and sum
+  // of slot j, every lane HD / 32 dimensions.
   constexpr int PER = HD / 32;
   static_assert(2 * WARPS <= 32, "one lane per slot");
   const int my_tag = lane < 2 * WARPS ? tag[lane] : -1;
-  int2 info[2] = {make_int2(-1, 0), make_int2(-1, 0)};
+  const int2 my_where = lane < 2 * WARPS ? where[lane] : make_int2(0, 0);
   int turn = warp;                       // this warp takes every WARPS-th (segment, head)
-  for (unsigned left = __ballot_sync(0xffffffffu, my_tag >= 0); left;) {
-    const int seg = __shfl_sync(0xffffffffu, my_tag, __ffs(left) - 1);
+  for (unsigned todo = __ballot_sync(0xffffffffu, my_tag >= 0); todo;) {
+    const int leader = __ffs(todo) - 1, seg = __shfl_sync(0xffffffffu, my_tag, leader);
     const unsigned members = __ballot_sync(0xffffffffu, my_tag == seg);
-    left &= ~members;
-    const int b = seg / HC, hc = seg - b * HC, hk = hc / p.chunks, chunk = hc - hk * p.chunks;
-    const int n = cum[b + 1] - cum[b];
-    const long long s0 = (long long)cum[b] * HC + (long long)hc * n, s1 = s0 + n;
-    const bool complete = s0 >= A && s1 <= E;
-    const int heads = min(NH, p.rep - chunk * NH), h0 = hk * p.rep + chunk * NH;
-    const int which = s0 >= A;           // 1: the segment starts in this CTA
-    const long long part = (long long)blockIdx.x * 2 + which;
-    if (!complete && tid == 0) info[which] = make_int2(seg, which ? (int)quotient(s1 - 1, per) - (int)blockIdx.x : 0);
+    todo &= ~members;
+    const int out_row = __shfl_sync(0xffffffffu, my_where.x, leader), bits = __shfl_sync(0xffffffffu, my_where.y, leader);
+    const int live = bits & 0xff;
+    const long long part = (long long)blockIdx.x * 2 + (bits >> 9);
     int h = turn;
-    for (; h < heads; h += WARPS) {
-      const float m = my_tag == seg ? slots[lane].m[h] : -INFINITY, l = my_tag == seg ? slots[lane].l[h] : 0.f;
-      const float top = warp_max(m);
-      const float wgt = l == 0.f ? 0.f : exp2_fast(m - top) * l;
+    for (; h < live; h += WARPS) {
+      const float ref = my_tag == seg ? slots[lane].m[h] : -INFINITY, sum = my_tag == seg ? slots[lane].l[h] : 0.f;
+      const float top = warp_max(ref);
+      const float wgt = sum == 0.f ? 0.f : exp2_fast(ref - top) * sum;
       const float den = warp_sum(wgt), inv = den == 0.f ? 0.f : 1.f / den;
       float o[PER] = {};
-      for (unsigned todo = members; todo; todo &= todo - 1) {
-        const int j = __ffs(todo) - 1;
+      for (unsigned from = members; from; from &= from - 1) {
+        const int j = __ffs(from) - 1;
         const float w = __shfl_sync(0xffffffffu, wgt, j);
         float x[PER];
         read_floats(x, &slots[j].o[h][lane * PER]);
@@ -493,19 +498,16 @@ __global__ void __launch_bounds__(THREADS, CTAS<HD, NT>) decode_kernel(const __g
       }
 #pragma unroll
       for (int e = 0; e < PER; ++e) o[e] *= inv;
-      if (complete) {
-        write_out(static_cast<T*>(p.out) + ((long long)b * p.Hq + h0 + h) * HD + lane * PER, o);
+      if (bits >> 8 & 1) {
+        write_out(static_cast<T*>(p.out) + (long long)(out_row + h) * HD + lane * PER, o);
       } else {
         write_floats(p.part_o + (part * NH + h) * HD + lane * PER, o);
         if (lane == 0) p.part_ml[part * NH + h] = make_float2(top, den);
       }
     }
-    turn = h - heads;
+    turn = h - live;
   }
-  if (tid == 0) {
-    p.part_info[2 * blockIdx.x] = info[0];
-    p.part_info[2 * blockIdx.x + 1] = info[1];
-  }
+  if (tid < 2) p.part_info[2 * blockIdx.x + tid] = crossing[tid];
 }
 
 // Joins the parts of a segment that starts in CTA blockIdx.x and goes on in the CTAs behind it; one head per CTA here.
