@@ -35,16 +35,13 @@ class _CountingLib:
 
     def __init__(self, cdll: ctypes.CDLL):
         object.__setattr__(self, "_cdll", cdll)
-        object.__setattr__(self, "_wrapped", {})
         object.__setattr__(self, "calls", 0)
 
     def __getattr__(self, name: str):
-        w = self._wrapped.get(name)
-        if w is not None:
-            return w
+        # first use of a launcher only: it becomes an attribute of its own
         fn = getattr(self._cdll, name)  # AttributeError if the symbol does not exist
         if name in _NO_LAUNCH:
-            self._wrapped[name] = fn
+            object.__setattr__(self, name, fn)
             return fn
 
         def counted(*args, _fn=fn, _self=self):
@@ -66,7 +63,7 @@ class _CountingLib:
                 return rc
             return _fn(*args)
 
-        self._wrapped[name] = counted
+        object.__setattr__(self, name, counted)
         return counted
 
 
@@ -128,6 +125,13 @@ def stream() -> c_void_p:
     if _raw_stream is not None:
         return c_void_p(_raw_stream(torch.cuda.current_device()))
     return c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def raw_stream() -> int:
+    """:func:`stream` as a plain integer, for calls where the host's time counts."""
+    if _raw_stream is not None:
+        return _raw_stream(torch.cuda.current_device())
+    return torch.cuda.current_stream().cuda_stream
 
 
 class _Here:

@@ -39,8 +39,8 @@ def has_kernel(head_dim: int, dtype: torch.dtype) -> bool:
 
 def _strides(t: torch.Tensor) -> tuple[int, ...]:
     """Strides, 0 for dimensions of size 1 (whose stride means nothing)."""
-    strides = t.stride()
-    return tuple([s if n > 1 else 0 for n, s in zip(t.shape, strides)]) if 1 in t.shape else strides
+    strides, shape = t.stride(), t.shape
+    return tuple([s if n > 1 else 0 for n, s in zip(shape, strides)]) if 1 in shape else strides
 
 
 @dataclass(frozen=True)
@@ -56,32 +56,31 @@ class Fp8KVCache:
     block: int = 64
 
     def __post_init__(self) -> None:
-        k, v, ks, vs = self.k, self.v, self.k_scale, self.v_scale
-        if self.block not in BLOCKS:
-            raise ValueError(f"block must be one of {BLOCKS}, got {self.block}")
+        k, v, ks, vs, block = self.k, self.v, self.k_scale, self.v_scale, self.block
+        if block not in BLOCKS:
+            raise ValueError(f"block must be one of {BLOCKS}, got {block}")
         if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn:
             raise TypeError(f"codes must be float8_e4m3fn, got {k.dtype} and {v.dtype}")
         if ks.dtype != torch.float32 or vs.dtype != torch.float32:
             raise TypeError(f"scales must be float32, got {ks.dtype} and {vs.dtype}")
-        strides = _strides(k)
-        if k.dim() != 4 or k.shape != v.shape or strides != _strides(v) or strides[3] > 1:
+        shape, strides, scale_strides = k.shape, _strides(k), _strides(ks)
+        if len(shape) != 4 or shape != v.shape or strides != _strides(v) or strides[3] > 1:
             raise ValueError("k and v must be [B, capacity, Hk, hd] of the same shape and strides, contiguous in hd")
-        B, capacity, Hk, hd = k.shape
-        want = (B, Hk, -(-capacity // self.block))
-        scale_strides = _strides(ks)
+        B, capacity, Hk, hd = shape
+        want = (B, Hk, -(-capacity // block))
         if ks.shape != want or vs.shape != want or scale_strides != _strides(vs) or scale_strides[2] > 1:
             raise ValueError(f"k_scale and v_scale must be {want} of the same strides, contiguous in the blocks")
         dev = k.device
         if v.device != dev or ks.device != dev or vs.device != dev:
             raise ValueError("codes and scales must be on one device")
-        keep = object.__setattr__
-        keep(self, "_device", dev)
-        keep(self, "_kernels", False)
-        if k.is_cuda:
+        if dev.type == "cuda":
             sb, st, sh, _ = strides
-            keep(self, "_kernels", hd in _HEAD_DIMS and not (sb | st | sh | k.data_ptr() | v.data_ptr()) & 15)
-            keep(self, "_status", _lib.status_word(dev))        # exists before any capture into a graph
-            keep(self, "_geometry", (sb, st, sh, scale_strides[0], scale_strides[1]))
+            kernels = hd in _HEAD_DIMS and not (sb | st | sh | k.data_ptr() | v.data_ptr()) & 15
+            geometry, status = (sb, st, sh, scale_strides[0], scale_strides[1]), _lib.status_word(dev)
+        else:
+            kernels, geometry, status = False, None, None
+        # the status word exists before any capture into a graph
+        self.__dict__.update(_device=dev, _kernels=kernels, _geometry=geometry, _status=status)
 
     def _args(self) -> tuple:
         """What describes the cache to the kernels: codes and their strides, scales and theirs."""
@@ -167,7 +166,7 @@ def append_kv_fp8(k_new: torch.Tensor, v_new: torch.Tensor, cache: Fp8KVCache, s
         rc = _lib.lib().ob_kv_fp8_append(
             k_new.data_ptr(), v_new.data_ptr(), _DTYPES[k_new.dtype], nb, nt, nh, *cache._args(),
             seq_lens.data_ptr(), None if n_new is None else n_new.data_ptr(), B, T, Hk, hd, capacity, cache.block,
-            cache._status.data_ptr(), _lib.stream())
+            cache._status.data_ptr(), _lib.raw_stream())
     _lib.check(rc, "ob_kv_fp8_append")
 
 
@@ -268,7 +267,7 @@ def decode_attention_fp8(q: torch.Tensor, k_new: torch.Tensor | None, v_new: tor
         rc = l.ob_attn_decode_fp8(
             q.data_ptr(), q_batch, _DTYPES[dtype], new_k, new_v, new_batch, new_head, *cache._args(),
             seq_lens.data_ptr(), out.data_ptr(), ws.data_ptr(), B, Hq, Hk, hd, capacity, cache.block,
-            scale, window or 0, cache._status.data_ptr(), _lib.stream())
+            scale, window or 0, cache._status.data_ptr(), _lib.raw_stream())
     _lib.check(rc, "ob_attn_decode_fp8")
     return out
 

@@ -125,7 +125,7 @@ def _forward(z: torch.Tensor, targets: torch.Tensor, top_k: int, temperature: fl
         rc = _lib.lib().ob_logprobs_fwd(
             z.data_ptr(), z.stride(0), _KERNEL_DTYPES[z.dtype], targets.data_ptr(), at, at + 4 * rows,
             at + 8 * rows if keep else None, top_logp.data_ptr() if top_k else None, top_ids.data_ptr() if top_k else None,
-            rows, vocab, top_k, temperature, _lib.stream())
+            rows, vocab, top_k, temperature, _lib.raw_stream())
     _lib.check(rc, "ob_logprobs_fwd")
     return num[0], num[1], top_logp, top_ids, num
 
@@ -148,7 +148,7 @@ def _backward(z: torch.Tensor, targets: torch.Tensor, num: torch.Tensor, d_logp:
         rc = _lib.lib().ob_logprobs_bwd(
             z.data_ptr(), z.stride(0), _KERNEL_DTYPES[z.dtype], targets.data_ptr(), at + 8 * rows, at + 4 * rows,
             None if d_logp is None else d_logp.data_ptr(), None if d_entropy is None else d_entropy.data_ptr(),
-            out.data_ptr(), out.stride(0), rows, vocab, temperature, _lib.stream())
+            out.data_ptr(), out.stride(0), rows, vocab, temperature, _lib.raw_stream())
     _lib.check(rc, "ob_logprobs_bwd")
     return out
 
