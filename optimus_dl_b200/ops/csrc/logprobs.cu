@@ -5,13 +5,19 @@
 //   log p_t = u_t - log S        H = log S - W / S
 //   dz_j = ( g_l (delta_jt - p_j) - g_H p_j (log p_j + H) ) / T
 //
-// The forward reads every logit once: each thread keeps (m, S, W) for its share against its own running maximum m,
-// and two such triples join as S = S_a 2^(m_a - m) + S_b 2^(m_b - m), W likewise after W_a += (m_a - m) S_a.  All
-// exponents are in base 2 (u log2 e = (z - m) c with c = log2 e / T); sums and statistics are fp32.  Differences are
-// taken before the product with c, so a row of the type's lowest value is a uniform row and not an overflow.
-// Exponents are clamped at -200, where 2^x is 0 in fp32 anyway: a banned token (-inf) then adds 0 to W, not 0 * inf.
-// The running maximum propagates NaN, and +inf is found at the end, so such rows give NaN as the formulas do.  A row
-// without any logit above -inf has log probabilities of -inf, entropy 0 and no gradient.
+// The forward reads every logit once: each thread keeps (m, S, W) for its share against its own running maximum m, and
+// two such triples join as S = S_a 2^(r_a - r) + S_b 2^(r_b - r), W likewise after W_a += (r_a - r) S_a.  All
+// exponents are in base 2 against r = m c rounded to fp32, c = log2 e / T: u = fma(z, c, -r) has one rounding, and what
+// r lost against m c cancels in H and is put back into log S at the end.  At 1600 MHz, where the chip settles under
+// power in a long run, the kernel is bound by instruction issue (the loads alone would take 5/6 of the time), so the
+// loop is written for few instructions: packed fp32 pairs, 16-bit pair maxima, one fused operation per exponent.
+//
+// Where nothing may go wrong: a banned token (-inf) has to add 0 to W, not 0 * inf, so bf16 logits are raised to -1e30
+// (a pair at a time) and the exponents of the other types to -200; 2^x is 0 there.  A maximum of 1e29 and more in
+// magnitude (a row of the type's lowest value) would overflow r; distinct fp32 numbers of that size differ by far more
+// than 200 T, so only the equals of the maximum count then.  The running maximum propagates NaN, and +inf is found at
+// the end, so such rows give NaN as the formulas do.  A row without any logit above -inf has log probabilities of -inf,
+// entropy 0 and no gradient.
 //
 // Alternatives: the k largest logits, equal ones by lowest index.  A candidate is one 64-bit number, the logit's
 // order-preserving key above the complement of its index, so "better" is one integer comparison without ties.  The
@@ -33,7 +39,8 @@ constexpr int UNROLL = 4;        // 16-byte loads in flight per thread
 constexpr int MAX_TOPK = 32;
 constexpr int CAP = 1024;        // candidates a CTA can list
 constexpr int MAX_CLUSTER = 8;
-constexpr float FLOOR = -200.0f;
+constexpr float FLOOR = -200.0f;       // of an exponent: 2^x is 0 in fp32
+constexpr float HUGE_LOGIT = 1e29f;    // from here on a maximum is treated apart
 
 using u64 = unsigned long long;
 
@@ -58,6 +65,8 @@ template <typename T> struct Vec;
 template <> struct Vec<float> {
   static constexpr int N = 4;
   static constexpr uint32_t NONE = 0xff800000u;      // 32 bits of -inf
+  static constexpr bool LIFTED = false;              // exponents have to be kept above FLOOR one by one
+  __device__ static uint4 lift(const uint4& u) { return u; }
   __device__ static void unpack(const uint4& u, float (&f)[N]) {
     f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
   }
@@ -75,6 +84,15 @@ template <> struct Vec<float> {
 template <> struct Vec<__nv_bfloat16> {
   static constexpr int N = 8;
   static constexpr uint32_t NONE = 0xff80ff80u;
+  static constexpr bool LIFTED = true;
+  __device__ static uint4 lift(const uint4& u) {         // at least -1e30
+    return make_uint4(lift2(u.x), lift2(u.y), lift2(u.z), lift2(u.w));
+  }
+  __device__ static uint32_t lift2(uint32_t a) {
+    uint32_t r;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(0xf14af14au));
+    return r;
+  }
   __device__ static void unpack(const uint4& u, float (&f)[N]) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -98,6 +116,8 @@ template <> struct Vec<__nv_bfloat16> {
 template <> struct Vec<__half> {
   static constexpr int N = 8;
   static constexpr uint32_t NONE = 0xfc00fc00u;
+  static constexpr bool LIFTED = false;
+  __device__ static uint4 lift(const uint4& u) { return u; }
   __device__ static void unpack(const uint4& u, float (&f)[N]) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -142,10 +162,10 @@ __device__ __forceinline__ float candidate_value(u64 c) {
 }
 __device__ __forceinline__ int candidate_index(u64 c) { return (int)~(uint32_t)c; }
 
-struct Sums { float m, s, w; };
+struct Sums { float m, s, w; };        // s and w against r = m c
 __device__ __forceinline__ void join(Sums& a, const Sums& b, float c) {
-  const float m = max_nan(a.m, b.m);
-  const float da = a.m == m ? 0.f : fmaxf((a.m - m) * c, FLOOR), db = b.m == m ? 0.f : fmaxf((b.m - m) * c, FLOOR);
+  const float m = max_nan(a.m, b.m), r = __fmul_rn(m, c);
+  const float da = a.m == m ? 0.f : fmaxf(__fmul_rn(a.m, c) - r, FLOOR), db = b.m == m ? 0.f : fmaxf(__fmul_rn(b.m, c) - r, FLOOR);
   const float fa = exp2_fast(da), fb = exp2_fast(db);
   a.w = fa * (a.w + da * a.s) + fb * (b.w + db * b.s);
   a.s = fa * a.s + fb * b.s;
@@ -230,13 +250,19 @@ __global__ void __launch_bounds__(THREADS, 4) forward_kernel(const __grid_consta
   const int nv = (p.V - head) / N;
   const int v0 = (int)((long long)nv * rank / p.cluster), v1 = (int)((long long)nv * (rank + 1) / p.cluster);
   const char* zv = reinterpret_cast<const char*>(z + head);
-  auto fetch = [&](int base, uint4 (&raw)[UNROLL]) {             // what lies behind the slice reads as banned
+  const char* at = zv + ((long long)v0 + tid) * 16;
+  auto fetch = [&](int base, uint4 (&raw)[UNROLL]) {             // from `at`; what lies behind the slice reads as banned
+    if (base + STEP <= v1) {
 #pragma unroll
-    for (int j = 0; j < UNROLL; ++j) {
-      const int i = base + j * THREADS + tid;
-      raw[j] = make_uint4(Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE);
-      if (i < v1) raw[j] = load_once(zv + (long long)i * 16);
+      for (int j = 0; j < UNROLL; ++j) raw[j] = load_once(at + j * THREADS * 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < UNROLL; ++j) {
+        raw[j] = make_uint4(Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE);
+        if (base + j * THREADS + tid < v1) raw[j] = load_once(at + j * THREADS * 16);
+      }
     }
+    at += STEP * 16;
   };
   uint4 raw[UNROLL], next[UNROLL];
   fetch(v0, raw);
@@ -253,41 +279,60 @@ __global__ void __launch_bounds__(THREADS, 4) forward_kernel(const __grid_consta
     if (tid < MAX_TOPK) sc.top[tid] = sc.merged[tid] = 0;
   }
 
-  Sums st{-INFINITY, 0.f, 0.f};
+  float m = -INFINITY, r = -INFINITY;
+  float2 s2 = make_float2(0.f, 0.f), w2 = s2;
+  const float2 cc = make_float2(c, c);
   int best_vec = v0 + tid;             // TOPK: a vector that holds this thread's maximum (or one behind it)
-  for (int base = v0; base < v1; base += STEP) {
-    fetch(base + STEP, next);
+  auto add = [&](int base, const uint4 (&raw)[UNROLL]) {
     float top_of[UNROLL], mx = -INFINITY;
 #pragma unroll
     for (int j = 0; j < UNROLL; ++j) {
       top_of[j] = Vec<T>::max_of(raw[j]);
       mx = max_nan(mx, top_of[j]);
     }
-    if (TOPK && !(mx <= st.m)) {
+    if (TOPK && !(mx <= m)) {
       best_vec = base + (UNROLL - 1) * THREADS + tid;
 #pragma unroll
       for (int j = UNROLL - 2; j >= 0; --j) if (top_of[j] == mx) best_vec = base + j * THREADS + tid;
     }
-    float2 s2 = make_float2(0.f, 0.f), w2 = s2;
-    const float2 neg = make_float2(-mx, -mx), cc = make_float2(c, c);
+    mx = max_nan(mx, m);
+    const float now = __fmul_rn(mx, c), d = mx == m ? 0.f : fmaxf(r - now, FLOOR), f = exp2_fast(d);
+    w2 = fmul2(ffma2(make_float2(d, d), s2, w2), make_float2(f, f));
+    s2 = fmul2(s2, make_float2(f, f));
+    m = mx;
+    r = now;
+    if (fabsf(m) < HUGE_LOGIT) {
+      const float2 neg = make_float2(-r, -r);
 #pragma unroll
-    for (int j = 0; j < UNROLL; ++j) {
-      float f[N];
-      Vec<T>::unpack(raw[j], f);
+      for (int j = 0; j < UNROLL; ++j) {
+        float z8[N];
+        Vec<T>::unpack(Vec<T>::lift(raw[j]), z8);
 #pragma unroll
-      for (int e = 0; e < N; e += 2) {
-        float2 u = fmul2(fadd2(make_float2(f[e], f[e + 1]), neg), cc);
-        u.x = fmaxf(u.x, FLOOR);
-        u.y = fmaxf(u.y, FLOOR);
-        const float2 x = make_float2(exp2_fast(u.x), exp2_fast(u.y));
-        s2 = fadd2(s2, x);
-        w2 = ffma2(u, x, w2);
+        for (int e = 0; e < N; e += 2) {
+          float2 u = ffma2(make_float2(z8[e], z8[e + 1]), cc, neg);
+          if (!Vec<T>::LIFTED) u = make_float2(fmaxf(u.x, FLOOR), fmaxf(u.y, FLOOR));
+          const float2 x = make_float2(exp2_fast(u.x), exp2_fast(u.y));
+          s2 = fadd2(s2, x);
+          w2 = ffma2(u, x, w2);
+        }
+      }
+    } else if (fabsf(m) < INFINITY) {
+#pragma unroll
+      for (int j = 0; j < UNROLL; ++j) {
+        float z8[N];
+        Vec<T>::unpack(raw[j], z8);
+        for (int e = 0; e < N; ++e) s2.x += z8[e] == m ? 1.f : 0.f;
       }
     }
-    join(st, Sums{mx, s2.x + s2.y, w2.x + w2.y}, c);
-#pragma unroll
-    for (int j = 0; j < UNROLL; ++j) raw[j] = next[j];
+  };
+  for (int base = v0; base < v1; base += 2 * STEP) {       // two buffers in turn: one is added up, one under way
+    fetch(base + STEP, next);
+    add(base, raw);
+    if (base + STEP >= v1) break;
+    fetch(base + 2 * STEP, raw);
+    add(base + STEP, next);
   }
+  Sums st{m, s2.x + s2.y, w2.x + w2.y};
   const u64 mine = TOPK && v0 + tid < v1 ? candidate(st.m, head + best_vec * N + N - 1) : 0;
   // the ragged ends of the row: fewer than N elements each
   const int tail = p.V - head - nv * N;
@@ -296,7 +341,9 @@ __global__ void __launch_bounds__(THREADS, 4) forward_kernel(const __grid_consta
   float extra = -INFINITY;
   if (tid < extra0 + extra1) {
     extra = Vec<T>::load(z + extra_at);
-    if (extra != -INFINITY) join(st, Sums{extra, 1.f + (extra == extra ? 0.f : extra), 0.f}, c);
+    // 2^u with the u that r = m c rounded leaves; NaN and +inf are found by the maximum
+    const float u = fabsf(extra) < HUGE_LOGIT ? fmaf(extra, c, -__fmul_rn(extra, c)) : 0.f;
+    if (extra != -INFINITY) join(st, Sums{extra, exp2_fast(u), u}, c);
   }
 
   // one triple per CTA
@@ -438,16 +485,18 @@ __global__ void __launch_bounds__(THREADS, 4) forward_kernel(const __grid_consta
   }
   const Sums total = p.cluster > 1 ? warp_sums[0] : cta_sums;
   const bool none = total.m == -INFINITY, broken = !(total.m < INFINITY);     // +inf and NaN
-  const float log2s = broken ? NAN : none ? 0.f : log2f(total.s);
-  const float m = none ? 0.f : total.m;
+  const float sum_log2 = broken ? NAN : none ? 0.f : log2f(total.s);
+  const float top_z = none ? 0.f : total.m;
+  // against the maximum itself from here on
+  const float log2s = fabsf(top_z) < HUGE_LOGIT ? sum_log2 - fmaf(top_z, c, -__fmul_rn(top_z, c)) : sum_log2;
   if (tid == 0) {
-    p.logp[row] = inside ? log_of(z_t, m, c, log2s) : 0.f;
-    p.entropy[row] = none ? 0.f : (log2s - total.w / total.s) * 0.6931471805599453f;
+    p.logp[row] = inside ? log_of(z_t, top_z, c, log2s) : 0.f;
+    p.entropy[row] = none ? 0.f : (sum_log2 - total.w / total.s) * 0.6931471805599453f;
     if (p.stats) p.stats[row] = make_float2(total.m, log2s);
   }
   if (TOPK && tid < p.k) {
     const u64 cand = p.cluster > 1 ? sc.merged[tid] : sc.top[tid];
-    p.top_logp[(long long)row * p.k + tid] = log_of(candidate_value(cand), m, c, log2s);
+    p.top_logp[(long long)row * p.k + tid] = log_of(candidate_value(cand), top_z, c, log2s);
     p.top_ids[(long long)row * p.k + tid] = candidate_index(cand);
   }
 }
@@ -563,7 +612,7 @@ extern "C" int ob_logprobs_fwd(const void* logits, long long ld, int dtype, cons
                                void* stats, void* top_logp, void* top_ids, int rows, int V, int top_k, double temperature,
                                cudaStream_t stream) {
   if (rows <= 0) return 0;
-  if (V <= 0 || top_k < 0 || top_k > MAX_TOPK || top_k > V || !(temperature > 0.0)) return -1;
+  if (V <= 0 || top_k < 0 || top_k > MAX_TOPK || top_k > V || !(temperature >= 1e-6 && temperature <= 1e6)) return -1;
   const int cl = pick_cluster(rows, V, dtype == 2 ? 4 : 8);
   if ((long long)rows * cl > 0x7fffffffLL) return -1;
   const Params p{logits, ld, (const long long*)targets, (float*)logp, (float*)entropy, (float2*)stats, (float*)top_logp,
@@ -578,7 +627,7 @@ extern "C" int ob_logprobs_bwd(const void* logits, long long ld, int dtype, cons
                                const void* entropy, const void* d_logp, const void* d_entropy, void* dz, long long dz_ld,
                                int rows, int V, double temperature, cudaStream_t stream) {
   if (rows <= 0) return 0;
-  if (V <= 0 || !(temperature > 0.0)) return -1;
+  if (V <= 0 || !(temperature >= 1e-6 && temperature <= 1e6)) return -1;
   const int vec = dtype == 2 ? 4 : 8;
   // CTAs per row: four per SM, of half a batch of loads at least, and no more than 8 batches each.  Measured: one row of
   // 128256 bf16 18.5 us with 1, 6.2 with 8, 4.2 with 16; 1000 rows of 50257 42.5 us with 1, 45.2 with 4; 4096 rows of

@@ -56,8 +56,8 @@ def _check(rows_shape: torch.Size, vocab: int, floating: torch.Tensor, targets: 
         raise ValueError("logits need at least one token")
     if not 0 <= top_k <= min(MAX_TOP_K, vocab):
         raise ValueError(f"top_k must be between 0 and {min(MAX_TOP_K, vocab)}, got {top_k}")
-    if not (temperature > 0 and math.isfinite(temperature)):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"temperature must be between 1e-6 and 1e6, got {temperature}")
 
 
 def _ordered(z: torch.Tensor) -> torch.Tensor:

@@ -136,7 +136,7 @@ def test_nan_and_infinity():
 def test_refusals():
     z, t = make(3, 9, torch.float32)
     for kw in (dict(top_k=-1), dict(top_k=10), dict(top_k=33), dict(temperature=0.0), dict(temperature=-1.0),
-               dict(temperature=math.nan), dict(temperature=math.inf)):
+               dict(temperature=math.nan), dict(temperature=math.inf), dict(temperature=1e-7)):
         with pytest.raises(ValueError):
             lp.token_logprobs(z, t, **kw)
     with pytest.raises(ValueError):
@@ -227,6 +227,43 @@ def test_kernel_nan_infinity_zero_signs():
     assert torch.isfinite(g[3:]).all()
     g, = torch.autograd.grad(lp.token_logprobs(zc, t.cuda()).entropy.sum(), [zc])
     assert torch.isnan(g[:3]).all() and torch.isfinite(g[3:]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("temperature", [1.0, 0.5, 3.0])
+def test_extreme_rows(dtype, temperature):
+    """Rows of the lowest value, of it among banned tokens, with huge maxima, and far from zero."""
+    vocab = 9001
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    z, t = make(8, vocab, dtype, seed=5)
+    z[0] = low
+    z[0, ::2] = -math.inf                  # half banned, the rest masked: uniform over the rest
+    z[1] = low
+    z[1, 4000:4010] = 1.0                  # a few live ones
+    z[2, 77] = high
+    z[3, 5:9] = high                       # four equals share it
+    z[4] = (z[4].float() + 300).to(dtype)
+    z[5] = (z[5].float() - 2000).to(dtype)
+    z[6] = low
+    t[:4] = torch.tensor([1, 4003, 77, 8])
+    t[6] = 9000
+    d_logp, d_h = torch.randn(8), torch.randn(8)
+    want = definition(z, t, 4, temperature, d_logp, d_h)
+    zc = z.cuda().requires_grad_(True)
+    for k in (0, 4):
+        r = lp.token_logprobs(zc, t.cuda(), top_k=k, temperature=temperature)
+        err = (r.logp.detach().double().cpu() - want["logp"]).abs()
+        assert bool((err <= 2e-5 + 4e-7 * (want["logp"].abs() + 20)).all())
+        assert (r.entropy.detach().double().cpu() - want["entropy"]).abs().max() <= 1e-3 * (dtype != torch.float32) + 2e-4
+    assert torch.equal(r.top_ids.cpu(), want["top_ids"])
+    fin = torch.isfinite(want["top_logp"].float()) & (want["top_logp"] > -1e30)
+    # an alternative 65504 below the maximum is 2^-24 of that off by its own rounding alone
+    err = (r.top_logp.double().cpu() - want["top_logp"]).abs()
+    assert bool((err <= 2e-5 + 4e-7 * (want["top_logp"].abs() + 20))[fin].all())
+    g, = torch.autograd.grad([r.logp, r.entropy], [zc], [d_logp.cuda(), d_h.cuda()])
+    assert torch.isfinite(g).all()
+    check_grad(g, want, dtype, d_logp, d_h, temperature)
 
 
 @pytest.mark.gpu
