@@ -32,6 +32,7 @@
 //   waits for its results only where it reads them (programmatic dependent launch).
 #include "kv_fp8.cuh"
 #include <atomic>
+#include <string.h>
 
 namespace ob {
 namespace decode_fp8 {
@@ -624,21 +625,42 @@ extern "C" long long ob_attn_decode_fp8_workspace(int B, int Hq, int Hk, int hd,
   return grid * 2 * ((long long)nh * hd * 4 + nh * 8 + 8);
 }
 
-// q_dtype: 0 = bf16, 1 = fp16 (also of k_new, v_new and out).  k_new / v_new may be null when the cache already holds
-// the current token.  Strides of q, new rows and scales in elements, of the cache in bytes.
-extern "C" int ob_attn_decode_fp8(const void* q, long long q_batch, int q_dtype, const void* k_new, const void* v_new,
-                                  long long new_batch, long long new_head, void* k, void* v, long long batch, long long tok,
-                                  long long head, void* k_scale, void* v_scale, long long scale_batch, long long scale_head,
-                                  const void* lens, void* out, void* workspace, int B, int Hq, int Hk, int hd, int capacity,
-                                  int block, float scale, int window, void* status, cudaStream_t stream) {
-  if (B <= 0) return 0;
-  if (Hk <= 0 || Hq <= 0 || Hq % Hk || hd < 32 || hd > 256 || (hd & (hd - 1)) || capacity <= 0 || window < 0) return -1;
+// One block of 8-byte arguments, in this order.  q_dtype: 0 = bf16, 1 = fp16 (also of k_new, v_new and out).  k_new /
+// v_new may be null when the cache already holds the current token.  Strides of q, new rows and scales in elements, of
+// the cache in bytes.
+struct AttentionArgs {
+  const void* q;
+  long long q_batch, q_dtype;
+  const void *k_new, *v_new;
+  long long new_batch, new_head;
+  void *k, *v;
+  long long batch, tok, head;
+  float *k_scale, *v_scale;
+  long long scale_batch, scale_head;
+  const int* lens;
+  void *out, *workspace;
+  long long B, Hq, Hk, hd, capacity, block;
+  double scale;
+  long long window;
+  int* status;
+  cudaStream_t stream;
+};
+static_assert(sizeof(AttentionArgs) == 29 * 8, "packed");
+
+extern "C" int ob_attn_decode_fp8(const void* packed) {
+  AttentionArgs a;
+  memcpy(&a, packed, sizeof(a));
+  if (a.B <= 0) return 0;
+  if (a.B > 0x7fffffffLL || a.Hq > 65536 || a.capacity > 0x3fffffffLL || a.window < 0) return -1;
+  const int B = (int)a.B, Hq = (int)a.Hq, Hk = (int)a.Hk, hd = (int)a.hd, capacity = (int)a.capacity, block = (int)a.block;
+  const int q_dtype = (int)a.q_dtype, window = (int)(a.window < a.capacity ? a.window : 0);     // a wider one hides nothing
+  if (Hk <= 0 || Hq <= 0 || Hq % Hk || hd < 32 || hd > 256 || (hd & (hd - 1)) || capacity <= 0) return -1;
   if (block < 16 || block > 128 || (block & (block - 1)) || q_dtype < 0 || q_dtype > 1) return -1;
-  if ((batch | tok | head) % 16) return -2;
-  if (k_new) {
-    const int rc = launch_append({k_new, v_new, new_batch, 0, new_head, k, v, batch, tok, head, (float*)k_scale,
-                                  (float*)v_scale, scale_batch, scale_head, (const int*)lens, nullptr, (int*)status, B, 1,
-                                  Hk, hd, capacity, block, 0, 0, 0}, q_dtype, stream);
+  if ((a.batch | a.tok | a.head) % 16) return -2;
+  if (a.k_new) {
+    const int rc = launch_append({a.k_new, a.v_new, a.new_batch, 0, a.new_head, a.k, a.v, a.batch, a.tok, a.head, a.k_scale,
+                                  a.v_scale, a.scale_batch, a.scale_head, a.lens, nullptr, a.status, B, 1, Hk, hd, capacity,
+                                  block, 0, 0, 0}, q_dtype, a.stream);
     if (rc) return rc;
   }
   const int rep = Hq / Hk, nt = groups(rep, hd), nh = 8 * nt;
@@ -648,22 +670,22 @@ extern "C" int ob_attn_decode_fp8(const void* q, long long q_batch, int q_dtype,
     const int nb = B - b0 < MAX_BATCH ? B - b0 : MAX_BATCH;
     const int grid = grid_size(nb, Hk, rep, hd, capacity);
     Params p;
-    p.q = (const uint16_t*)q + (long long)b0 * q_batch; p.q_batch = q_batch;
-    p.k = (const uint8_t*)k + (long long)b0 * batch; p.v = (const uint8_t*)v + (long long)b0 * batch;
-    p.batch = batch; p.tok = tok; p.head = head;
-    p.k_scale = (const float*)k_scale + (long long)b0 * scale_batch;
-    p.v_scale = (const float*)v_scale + (long long)b0 * scale_batch;
-    p.scale_batch = scale_batch; p.scale_head = scale_head;
-    p.lens = (const int*)lens + b0;
-    p.out = (uint16_t*)out + (long long)b0 * Hq * hd;
-    p.part_o = (float*)workspace;
+    p.q = (const uint16_t*)a.q + (long long)b0 * a.q_batch; p.q_batch = a.q_batch;
+    p.k = (const uint8_t*)a.k + (long long)b0 * a.batch; p.v = (const uint8_t*)a.v + (long long)b0 * a.batch;
+    p.batch = a.batch; p.tok = a.tok; p.head = a.head;
+    p.k_scale = a.k_scale + (long long)b0 * a.scale_batch;
+    p.v_scale = a.v_scale + (long long)b0 * a.scale_batch;
+    p.scale_batch = a.scale_batch; p.scale_head = a.scale_head;
+    p.lens = a.lens + b0;
+    p.out = (uint16_t*)a.out + (long long)b0 * Hq * hd;
+    p.part_o = (float*)a.workspace;
     p.part_ml = (float2*)(p.part_o + (long long)grid * 2 * nh * hd);
     p.part_info = (int2*)(p.part_ml + (long long)grid * 2 * nh);
     p.B = nb; p.Hq = Hq; p.Hk = Hk; p.rep = rep; p.chunks = (rep + nh - 1) / nh; p.capacity = capacity;
     p.block_shift = shift; p.window = window; p.min_units = MIN_UNITS;
-    p.scale_log2 = scale * 1.4426950408889634f;
-    p.appended = k_new != nullptr && b0 == 0;      // the launch before is the append
-    const int rc = q_dtype == 0 ? dispatch<__nv_bfloat16>(p, hd, nt, grid, stream) : dispatch<__half>(p, hd, nt, grid, stream);
+    p.scale_log2 = (float)(a.scale * 1.4426950408889634);
+    p.appended = a.k_new != nullptr && b0 == 0;      // the launch before is the append
+    const int rc = q_dtype == 0 ? dispatch<__nv_bfloat16>(p, hd, nt, grid, a.stream) : dispatch<__half>(p, hd, nt, grid, a.stream);
     if (rc) return rc;
   }
   return 0;

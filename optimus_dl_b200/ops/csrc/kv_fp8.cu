@@ -11,6 +11,7 @@
 // the larger scale in the same CTA.  The kernel is bound by the stream of new rows (2 or 4 bytes read and 1 written
 // per element); the CTA has one thread per 64 elements of a full block, so each thread has all its loads in flight.
 #include "kv_fp8.cuh"
+#include <string.h>
 
 namespace ob {
 namespace kvfp8 {
@@ -291,17 +292,31 @@ int launch_append(AppendParams p, int dtype, cudaStream_t stream) {
 }  // namespace kvfp8
 }  // namespace ob
 
-// dtype: 0 = bf16, 1 = fp16, 2 = fp32.  Strides of the new rows and scales in elements, of the cache in bytes; rows of
-// both start on 16-byte boundaries.
-extern "C" int ob_kv_fp8_append(const void* k_new, const void* v_new, int dtype, long long new_batch, long long new_tok,
-                                long long new_head, void* k, void* v, long long batch, long long tok, long long head,
-                                void* k_scale, void* v_scale, long long scale_batch, long long scale_head, const void* lens,
-                                const void* n_new, int B, int T, int Hk, int hd, int capacity, int block, void* status,
-                                cudaStream_t stream) {
-  if (Hk <= 0 || hd < 32 || hd > 256 || (hd & (hd - 1)) || block < 16 || block > 128 || (block & (block - 1))) return -1;
-  if ((batch | tok | head) % 16) return -2;
-  return ob::kvfp8::launch_append({k_new, v_new, new_batch, new_tok, new_head, k, v, batch, tok, head, (float*)k_scale,
-                                   (float*)v_scale, scale_batch, scale_head, (const int*)lens, (const int*)n_new,
-                                   (int*)status, B, T, Hk, hd, capacity, block, 0, 0, 0},
-                                  dtype, stream);
+// One block of 8-byte arguments, in this order.  dtype: 0 = bf16, 1 = fp16, 2 = fp32.  Strides of the new rows and
+// scales in elements, of the cache in bytes; rows of both start on 16-byte boundaries.
+struct AppendArgs {
+  const void *k_new, *v_new;
+  long long dtype, new_batch, new_tok, new_head;
+  void *k, *v;
+  long long batch, tok, head;
+  float *k_scale, *v_scale;
+  long long scale_batch, scale_head;
+  const int *lens, *n_new;      // n_new may be null
+  long long B, T, Hk, hd, capacity, block;
+  int* status;
+  cudaStream_t stream;
+};
+static_assert(sizeof(AppendArgs) == 25 * 8, "packed");
+
+extern "C" int ob_kv_fp8_append(const void* packed) {
+  AppendArgs a;
+  memcpy(&a, packed, sizeof(a));
+  const int hd = (int)a.hd, block = (int)a.block;
+  if (a.Hk <= 0 || hd < 32 || hd > 256 || (hd & (hd - 1)) || block < 16 || block > 128 || (block & (block - 1))) return -1;
+  if (a.B > 0x7fffffffLL || a.T > 0x3fffffffLL || a.capacity > 0x3fffffffLL) return -1;
+  if ((a.batch | a.tok | a.head) % 16) return -2;
+  return ob::kvfp8::launch_append({a.k_new, a.v_new, a.new_batch, a.new_tok, a.new_head, a.k, a.v, a.batch, a.tok, a.head,
+                                   a.k_scale, a.v_scale, a.scale_batch, a.scale_head, a.lens, a.n_new, a.status, (int)a.B,
+                                   (int)a.T, (int)a.Hk, hd, (int)a.capacity, block, 0, 0, 0},
+                                  (int)a.dtype, a.stream);
 }

@@ -28,6 +28,7 @@
 // that overflows (thousands of equal logits in one thread's share) is replaced by k plain arg-max passes.
 #include "common.cuh"
 #include <cooperative_groups.h>
+#include <string.h>
 
 namespace ob {
 namespace logprobs {
@@ -607,25 +608,58 @@ static int pick_cluster(int rows, int V, int vec) {
 
 using namespace ob::logprobs;
 
-// dtype: 0 = bf16, 1 = fp16, 2 = fp32 (also of the gradient).
-extern "C" int ob_logprobs_fwd(const void* logits, long long ld, int dtype, const void* targets, void* logp, void* entropy,
-                               void* stats, void* top_logp, void* top_ids, int rows, int V, int top_k, double temperature,
-                               cudaStream_t stream) {
+// Launchers take one block of 8-byte arguments, in this order.  dtype: 0 = bf16, 1 = fp16, 2 = fp32 (also of the
+// gradient).
+struct ForwardArgs {
+  const void* logits;
+  long long ld, dtype;
+  const long long* targets;
+  float *logp, *entropy;
+  float2* stats;                // may be null
+  float* top_logp;
+  long long* top_ids;
+  long long rows, V, top_k;
+  double temperature;
+  cudaStream_t stream;
+};
+struct BackwardArgs {
+  const void* logits;
+  long long ld, dtype;
+  const long long* targets;
+  const float2* stats;
+  const float *entropy, *d_logp, *d_entropy;      // the last two may be null
+  void* dz;
+  long long dz_ld, rows, V;
+  double temperature;
+  cudaStream_t stream;
+};
+static_assert(sizeof(ForwardArgs) == 14 * 8 && sizeof(BackwardArgs) == 14 * 8, "packed");
+
+extern "C" int ob_logprobs_fwd(const void* packed) {
+  ForwardArgs a;
+  memcpy(&a, packed, sizeof(a));
+  const int rows = (int)a.rows, V = (int)a.V, top_k = (int)a.top_k, dtype = (int)a.dtype;
+  if (a.rows > 0x7fffffffLL || a.V > 0x7fffffffLL) return -1;
+  const double temperature = a.temperature;
+  const cudaStream_t stream = a.stream;
   if (rows <= 0) return 0;
   if (V <= 0 || top_k < 0 || top_k > MAX_TOPK || top_k > V || !(temperature >= 1e-6 && temperature <= 1e6)) return -1;
   const int cl = pick_cluster(rows, V, dtype == 2 ? 4 : 8);
   if ((long long)rows * cl > 0x7fffffffLL) return -1;
-  const Params p{logits, ld, (const long long*)targets, (float*)logp, (float*)entropy, (float2*)stats, (float*)top_logp,
-                 (long long*)top_ids, rows, V, top_k, cl, (float)(1.4426950408889634 / temperature)};
+  const Params p{a.logits, a.ld, a.targets, a.logp, a.entropy, a.stats, a.top_logp, a.top_ids, rows, V, top_k, cl,
+                 (float)(1.4426950408889634 / temperature)};
   if (dtype == 0) return run_forward<__nv_bfloat16>(p, stream);
   if (dtype == 1) return run_forward<__half>(p, stream);
   if (dtype == 2) return run_forward<float>(p, stream);
   return -1;
 }
 
-extern "C" int ob_logprobs_bwd(const void* logits, long long ld, int dtype, const void* targets, const void* stats,
-                               const void* entropy, const void* d_logp, const void* d_entropy, void* dz, long long dz_ld,
-                               int rows, int V, double temperature, cudaStream_t stream) {
+extern "C" int ob_logprobs_bwd(const void* packed) {
+  BackwardArgs a;
+  memcpy(&a, packed, sizeof(a));
+  const int rows = (int)a.rows, V = (int)a.V, dtype = (int)a.dtype;
+  if (a.rows > 0x7fffffffLL || a.V > 0x7fffffffLL) return -1;
+  const double temperature = a.temperature;
   if (rows <= 0) return 0;
   if (V <= 0 || !(temperature >= 1e-6 && temperature <= 1e6)) return -1;
   const int vec = dtype == 2 ? 4 : 8;
@@ -640,9 +674,8 @@ extern "C" int ob_logprobs_bwd(const void* logits, long long ld, int dtype, cons
   const float c = (float)(1.4426950408889634 / temperature), inv_t = (float)(1.0 / temperature);
   const unsigned grid = (unsigned)((long long)rows * pieces);
 #define OB_LAUNCH(T)                                                                                                  \
-  backward_kernel<T><<<grid, THREADS, 0, stream>>>((const T*)logits, ld, (const long long*)targets, (const float2*)stats, \
-                                                   (const float*)entropy, (const float*)d_logp, (const float*)d_entropy, \
-                                                   (T*)dz, dz_ld, rows, V, pieces, c, inv_t)
+  backward_kernel<T><<<grid, THREADS, 0, a.stream>>>((const T*)a.logits, a.ld, a.targets, a.stats, a.entropy, a.d_logp, \
+                                                     a.d_entropy, (T*)a.dz, a.dz_ld, rows, V, pieces, c, inv_t)
   if (dtype == 0) OB_LAUNCH(__nv_bfloat16);
   else if (dtype == 1) OB_LAUNCH(__half);
   else if (dtype == 2) OB_LAUNCH(float);

@@ -30,6 +30,9 @@ SCALE_EXP_MIN, SCALE_EXP_MAX = -112, 119
 BLOCKS = (16, 32, 64, 128)
 _HEAD_DIMS = (32, 64, 128, 256)
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_CACHE = "QQqqqQQqq"                     # as Fp8KVCache._args gives it
+_launch_append = _lib.Packed("ob_kv_fp8_append", "QQqqqq" + _CACHE + "QQqqqqqqQQ")
+_launch_attention = _lib.Packed("ob_attn_decode_fp8", "QqqQQqq" + _CACHE + "QQQqqqqqqdqQQ")
 
 
 def has_kernel(head_dim: int, dtype: torch.dtype) -> bool:
@@ -163,11 +166,9 @@ def append_kv_fp8(k_new: torch.Tensor, v_new: torch.Tensor, cache: Fp8KVCache, s
         return
     k_new, v_new, (nb, nt, nh, _) = _new_rows(k_new, v_new)
     with _lib.on_device(cache._device):
-        rc = _lib.lib().ob_kv_fp8_append(
-            k_new.data_ptr(), v_new.data_ptr(), _DTYPES[k_new.dtype], nb, nt, nh, *cache._args(),
-            seq_lens.data_ptr(), None if n_new is None else n_new.data_ptr(), B, T, Hk, hd, capacity, cache.block,
-            cache._status.data_ptr(), _lib.raw_stream())
-    _lib.check(rc, "ob_kv_fp8_append")
+        _launch_append(k_new.data_ptr(), v_new.data_ptr(), _DTYPES[k_new.dtype], nb, nt, nh, *cache._args(),
+                       seq_lens.data_ptr(), 0 if n_new is None else n_new.data_ptr(), B, T, Hk, hd, capacity, cache.block,
+                       cache._status.data_ptr(), _lib.raw_stream())
 
 
 def needed_scale(amax: torch.Tensor) -> torch.Tensor:
@@ -256,19 +257,15 @@ def decode_attention_fp8(q: torch.Tensor, k_new: torch.Tensor | None, v_new: tor
     if q_head not in (0, hd):
         q = q.contiguous()
         q_batch = Hq * hd
-    new_k = new_v = None
-    new_batch = new_head = 0
+    new_k = new_v = new_batch = new_head = 0
     if k_new is not None:
         k_new, v_new, (new_batch, new_head, _) = _new_rows(k_new, v_new)
         new_k, new_v = k_new.data_ptr(), v_new.data_ptr()
-    l = _lib.lib()
     ws = torch.empty(_workspace(B, Hq, Hk, hd, capacity), dtype=torch.uint8, device=cache._device)
     with _lib.on_device(cache._device):
-        rc = l.ob_attn_decode_fp8(
-            q.data_ptr(), q_batch, _DTYPES[dtype], new_k, new_v, new_batch, new_head, *cache._args(),
-            seq_lens.data_ptr(), out.data_ptr(), ws.data_ptr(), B, Hq, Hk, hd, capacity, cache.block,
-            scale, window or 0, cache._status.data_ptr(), _lib.raw_stream())
-    _lib.check(rc, "ob_attn_decode_fp8")
+        _launch_attention(q.data_ptr(), q_batch, _DTYPES[dtype], new_k, new_v, new_batch, new_head, *cache._args(),
+                          seq_lens.data_ptr(), out.data_ptr(), ws.data_ptr(), B, Hq, Hk, hd, capacity, cache.block, scale,
+                          window or 0, cache._status.data_ptr(), _lib.raw_stream())
     return out
 
 

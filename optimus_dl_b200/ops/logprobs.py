@@ -32,6 +32,8 @@ from . import _lib, gemm
 
 MAX_TOP_K = 32
 _KERNEL_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_launch_forward = _lib.Packed("ob_logprobs_fwd", "QqqQQQQQQqqqdQ")
+_launch_backward = _lib.Packed("ob_logprobs_bwd", "QqqQQQQQQqqqdQ")
 
 
 @dataclass
@@ -122,11 +124,9 @@ def _forward(z: torch.Tensor, targets: torch.Tensor, top_k: int, temperature: fl
         top_ids = torch.empty((rows, top_k), dtype=torch.int64, device=dev)
     at = num.data_ptr()
     with _lib.on_device(dev):
-        rc = _lib.lib().ob_logprobs_fwd(
-            z.data_ptr(), z.stride(0), _KERNEL_DTYPES[z.dtype], targets.data_ptr(), at, at + 4 * rows,
-            at + 8 * rows if keep else None, top_logp.data_ptr() if top_k else None, top_ids.data_ptr() if top_k else None,
-            rows, vocab, top_k, temperature, _lib.raw_stream())
-    _lib.check(rc, "ob_logprobs_fwd")
+        _launch_forward(z.data_ptr(), z.stride(0), _KERNEL_DTYPES[z.dtype], targets.data_ptr(), at, at + 4 * rows,
+                        at + 8 * rows if keep else 0, top_logp.data_ptr() if top_k else 0,
+                        top_ids.data_ptr() if top_k else 0, rows, vocab, top_k, temperature, _lib.raw_stream())
     return num[0], num[1], top_logp, top_ids, num
 
 
@@ -145,11 +145,10 @@ def _backward(z: torch.Tensor, targets: torch.Tensor, num: torch.Tensor, d_logp:
     d_entropy = None if d_entropy is None else _rows_fp32(d_entropy)
     at = num.data_ptr()
     with _lib.on_device(z.device):
-        rc = _lib.lib().ob_logprobs_bwd(
-            z.data_ptr(), z.stride(0), _KERNEL_DTYPES[z.dtype], targets.data_ptr(), at + 8 * rows, at + 4 * rows,
-            None if d_logp is None else d_logp.data_ptr(), None if d_entropy is None else d_entropy.data_ptr(),
-            out.data_ptr(), out.stride(0), rows, vocab, temperature, _lib.raw_stream())
-    _lib.check(rc, "ob_logprobs_bwd")
+        _launch_backward(z.data_ptr(), z.stride(0), _KERNEL_DTYPES[z.dtype], targets.data_ptr(), at + 8 * rows,
+                         at + 4 * rows, 0 if d_logp is None else d_logp.data_ptr(),
+                         0 if d_entropy is None else d_entropy.data_ptr(), out.data_ptr(), out.stride(0), rows, vocab,
+                         temperature, _lib.raw_stream())
     return out
 
 
