@@ -660,7 +660,7 @@ extern "C" int ob_attn_decode_fp8(const void* packed) {
   if (a.k_new) {
     const int rc = launch_append({a.k_new, a.v_new, a.new_batch, 0, a.new_head, a.k, a.v, a.batch, a.tok, a.head, a.k_scale,
                                   a.v_scale, a.scale_batch, a.scale_head, a.lens, nullptr, a.status, B, 1, Hk, hd, capacity,
-                                  block, 0, 0, 0}, q_dtype, a.stream);
+                                  block, 0, 0, 0, 0}, q_dtype, a.stream);
     if (rc) return rc;
   }
   const int rep = Hq / Hk, nt = groups(rep, hd), nh = 8 * nt;

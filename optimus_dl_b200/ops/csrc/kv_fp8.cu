@@ -120,11 +120,7 @@ __global__ void __launch_bounds__(512, sizeof(T) == 4 ? 1 : 2) append_kernel(con
   __shared__ uint32_t warp_max_[2][16];
   const int tid = threadIdx.x;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the attention launch may start its own set-up
-  // blockIdx.x = ((b * 2 + kv) * Hk + head) * span + j
-  unsigned i = blockIdx.x;
-  const int j = i % p.span; i /= p.span;
-  const int h = i % p.Hk; i /= p.Hk;
-  const int kv = i & 1, b = i >> 1;
+  const int j = blockIdx.x, kv = blockIdx.y >= p.Hk, h = blockIdx.y - (kv ? p.Hk : 0), b = p.b0 + blockIdx.z;
   const int len = p.lens[b];
   const int n = p.n_new ? p.n_new[b] : (len == 0 ? 0 : p.T);
   const int start = len - n;
@@ -276,17 +272,20 @@ int launch_append(AppendParams p, int dtype, cudaStream_t stream) {
   p.block_shift = p.row_shift = 0;
   while ((1 << p.block_shift) < p.block) ++p.block_shift;
   while ((8 << p.row_shift) < p.hd) ++p.row_shift;
-  const long long grid = (long long)p.B * 2 * p.Hk * p.span;
-  if (grid > 0x7fffffffLL || 2LL * p.B * p.Hk > 0x7fffffffLL) return -1;
+  if (p.Hk > 0x7fff || 2LL * p.B * p.Hk > 0x7fffffffLL) return -1;
   if (p.T == 1)
     return dtype == 0 ? launch_one<__nv_bfloat16>(p, stream) : dtype == 1 ? launch_one<__half>(p, stream)
          : dtype == 2 ? launch_one<float>(p, stream) : -1;
   const int threads = max(32, min(512, p.block * p.hd / (8 * CHUNKS)));
-  if (dtype == 0) append_kernel<__nv_bfloat16><<<(unsigned)grid, threads, 0, stream>>>(p);
-  else if (dtype == 1) append_kernel<__half><<<(unsigned)grid, threads, 0, stream>>>(p);
-  else if (dtype == 2) append_kernel<float><<<(unsigned)grid, threads, 0, stream>>>(p);
-  else return -1;
-  return (int)cudaGetLastError();
+  for (p.b0 = 0; p.b0 < p.B; p.b0 += 0xffff) {
+    const dim3 grid(p.span, 2 * p.Hk, min(p.B - p.b0, 0xffff));
+    if (dtype == 0) append_kernel<__nv_bfloat16><<<grid, threads, 0, stream>>>(p);
+    else if (dtype == 1) append_kernel<__half><<<grid, threads, 0, stream>>>(p);
+    else if (dtype == 2) append_kernel<float><<<grid, threads, 0, stream>>>(p);
+    else return -1;
+    OB_CUDA_CHECK(cudaGetLastError());
+  }
+  return 0;
 }
 
 }  // namespace kvfp8
@@ -317,6 +316,6 @@ extern "C" int ob_kv_fp8_append(const void* packed) {
   if ((a.batch | a.tok | a.head) % 16) return -2;
   return ob::kvfp8::launch_append({a.k_new, a.v_new, a.new_batch, a.new_tok, a.new_head, a.k, a.v, a.batch, a.tok, a.head,
                                    a.k_scale, a.v_scale, a.scale_batch, a.scale_head, a.lens, a.n_new, a.status, (int)a.B,
-                                   (int)a.T, (int)a.Hk, hd, (int)a.capacity, block, 0, 0, 0},
+                                   (int)a.T, (int)a.Hk, hd, (int)a.capacity, block, 0, 0, 0, 0},
                                   (int)a.dtype, a.stream);
 }

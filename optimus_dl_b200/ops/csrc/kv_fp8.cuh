@@ -56,8 +56,9 @@ struct AppendParams {
   const int *lens, *n_new;                     // n_new may be null
   int* status;
   int B, T, Hk, hd, capacity, block;
-  // set by the launcher: blocks that a run of T tokens can touch, log2 of block and of a row's 8-element chunks
-  int span, block_shift, row_shift;
+  // set by the launcher: blocks that a run of T tokens can touch, the launch's first sequence, log2 of block and of a
+  // row's 8-element chunks
+  int span, b0, block_shift, row_shift;
 };
 int launch_append(AppendParams p, int dtype, cudaStream_t stream);
 
