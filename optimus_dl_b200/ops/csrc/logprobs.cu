@@ -21,13 +21,14 @@
 //
 // Alternatives: the k largest logits, equal ones by lowest index.  A candidate is one 64-bit number, the logit's
 // order-preserving key above the complement of its index, so "better" is one integer comparison without ties.  The
-// pass over the logits does nothing for them but note in which vector a thread met its maximum.  Afterwards the k-th
-// best of the threads' maxima is a bound that at least k candidates reach; only threads whose maximum reaches it (k of
-// them, unless logits are equal) can hold one of the k best, and the CTA reads their vectors once more, from the L2
-// cache, and lists what reaches the bound: little more than k candidates, which are then ranked by counting.  A list
-// that overflows (thousands of equal logits in one thread's share) is replaced by k plain arg-max passes.
+// pass over the logits does no more for them than note, per thread, every batch's maximum (in shared memory) and the
+// vector that holds the largest.  Afterwards the k-th best of the threads' maxima is a bound that at least k candidates
+// reach; a thread reads those of its batches again whose maximum reaches it (little more than k in the whole CTA,
+// unless logits are equal) and lists what reaches the bound, and the list is ranked by counting.  A list that overflows
+// (thousands of equal logits in one thread's share) is replaced by k plain arg-max passes.
 #include "common.cuh"
 #include <cooperative_groups.h>
+#include <atomic>
 #include <string.h>
 
 namespace ob {
@@ -38,8 +39,10 @@ namespace cg = cooperative_groups;
 constexpr int THREADS = 256;
 constexpr int UNROLL = 4;        // 16-byte loads in flight per thread
 constexpr int MAX_TOPK = 32;
-constexpr int CAP = 1024;        // candidates a CTA can list
+constexpr int CAP = 512;        // candidates a CTA can list
 constexpr int MAX_CLUSTER = 8;
+constexpr int LOOKS = 512;      // notes that the CTA looks behind together
+constexpr int NOTES = 16;        // maxima a thread notes: one for each batch, or for 2, 4, 8... of longer slices
 constexpr float FLOOR = -200.0f;       // of an exponent: 2^x is 0 in fp32
 constexpr float HUGE_LOGIT = 1e29f;    // from here on a maximum is treated apart
 
@@ -186,10 +189,13 @@ __device__ __forceinline__ float log_of(float z, float m, float c, float log2s) 
   return ((z - m) * c - log2s) * 0.6931471805599453f;
 }
 
-struct Scratch {                 // of a CTA that looks for alternatives
+// Of a CTA that looks for alternatives.  Kept to some 28 KB: four CTAs of 54 KB left the SM so little of its L1 cache for
+// the loads in flight that 1000 rows of 50257 fp32 took 54 us instead of 43.
+struct Scratch {
   u64 list[CAP], few[CAP], top[MAX_TOPK], merged[MAX_TOPK], warp_bound[THREADS / 32], kth;
-  int hot[THREADS];
-  int listed, counted, hots;
+  float note[NOTES][THREADS];
+  int look[LOOKS];
+  int listed, counted, looks;
 };
 
 // A lower bound of the k-th best of the CTA's candidates, one per thread; the first `active` threads have one (0
@@ -235,6 +241,8 @@ __device__ __forceinline__ void select_top(const u64* list, int n, int k, u64* t
   }
 }
 
+static_assert(UNROLL == 4 && THREADS == 256, "how a look is packed and shared out");
+
 template <typename T, bool TOPK>
 __global__ void __launch_bounds__(THREADS, 4) forward_kernel(const __grid_constant__ Params p) {
   constexpr int N = Vec<T>::N, STEP = THREADS * UNROLL;
@@ -276,7 +284,7 @@ __global__ void __launch_bounds__(THREADS, 4) forward_kernel(const __grid_consta
     if (inside) z_t = Vec<T>::load(z + t);
   }
   if (TOPK) {
-    if (tid == 0) { sc.listed = sc.counted = sc.hots = 0; sc.kth = 0; }
+    if (tid == 0) { sc.listed = sc.counted = sc.looks = 0; sc.kth = 0; }
     if (tid < MAX_TOPK) sc.top[tid] = sc.merged[tid] = 0;
   }
 
@@ -284,6 +292,9 @@ __global__ void __launch_bounds__(THREADS, 4) forward_kernel(const __grid_consta
   float2 s2 = make_float2(0.f, 0.f), w2 = s2;
   const float2 cc = make_float2(c, c);
   int best_vec = v0 + tid;             // TOPK: a vector that holds this thread's maximum (or one behind it)
+  int group = 0;                       // log2 of the batches that share a note
+  if (TOPK)
+    while ((v1 - v0 + STEP - 1) / STEP > NOTES << group) ++group;
   auto add = [&](int base, const uint4 (&raw)[UNROLL]) {
     float top_of[UNROLL], mx = -INFINITY;
 #pragma unroll
@@ -295,6 +306,11 @@ __global__ void __launch_bounds__(THREADS, 4) forward_kernel(const __grid_consta
       best_vec = base + (UNROLL - 1) * THREADS + tid;
 #pragma unroll
       for (int j = UNROLL - 2; j >= 0; --j) if (top_of[j] == mx) best_vec = base + j * THREADS + tid;
+    }
+    if (TOPK) {
+      const int batch = (base - v0) / STEP;
+      float& note = sc.note[batch >> group][tid];
+      note = (batch & ((1 << group) - 1)) ? max_nan(note, mx) : mx;
     }
     mx = max_nan(mx, m);
     const float now = __fmul_rn(mx, c), d = mx == m ? 0.f : fmaxf(r - now, FLOOR), f = exp2_fast(d);
@@ -384,11 +400,7 @@ __global__ void __launch_bounds__(THREADS, 4) forward_kernel(const __grid_consta
       if (r == p.k - 1) sc.kth = m;
     }
     __syncthreads();
-    // threads that can hold a candidate at or above it; equal maxima count, their indices are not exact
     const u64 kth = sc.kth;
-    if (mine != 0 && mine >> 32 >= kth >> 32) sc.hot[atomicAdd(&sc.hots, 1)] = tid;
-    if (tid == 0) sc.counted = 0;
-    __syncthreads();
     const float kth_z = kth == 0 ? -INFINITY : candidate_value(kth);
     const int kth_at = kth == 0 ? 0x7fffffff : candidate_index(kth);
     auto push = [&](float f, int idx) {
@@ -398,29 +410,35 @@ __global__ void __launch_bounds__(THREADS, 4) forward_kernel(const __grid_consta
         if (at < CAP) sc.list[at] = cand;
       }
     };
-    const int hots = sc.hots, each = (v1 - v0 + THREADS - 1) / THREADS, looks = hots * each;
-    for (int w = tid; w < looks; w += STEP) {
-      int at[UNROLL];
+    auto examine = [&](const uint4& u, int i) {
+      const float mx = Vec<T>::max_of(u);
+      if (mx < kth_z || (mx == kth_z && head + i * N > kth_at)) return;
+      float f[N];
+      Vec<T>::unpack(u, f);
 #pragma unroll
-      for (int j = 0; j < UNROLL; ++j) {
-        const int q = (w + j * THREADS) / hots, h = (w + j * THREADS) - q * hots;
-        at[j] = w + j * THREADS < looks ? v0 + q * THREADS + sc.hot[h] : v1;
-        raw[j] = make_uint4(Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE);
-        if (at[j] < v1) raw[j] = load_once(zv + (long long)at[j] * 16);
+      for (int e = 0; e < N; ++e)
+        if (!(f[e] < kth_z)) push(f[e], head + i * N + e);
+    };
+    // notes that reach the bound, little more than k; their vectors are shared out over all threads
+    const int notes = ((v1 - v0 + STEP - 1) / STEP + (1 << group) - 1) >> group;
+    for (int n = 0; n < notes; ++n)
+      if (!(sc.note[n][tid] < kth_z) && v0 + tid < v1) {
+        const int at = atomicAdd(&sc.looks, 1);
+        if (at < LOOKS) sc.look[at] = n << 8 | tid;
       }
-#pragma unroll
-      for (int j = 0; j < UNROLL; ++j) {
-        const float mx = Vec<T>::max_of(raw[j]);
-        if (at[j] < v1 && !(mx < kth_z) && !(mx == kth_z && head + at[j] * N > kth_at)) {
-          float f[N];
-          Vec<T>::unpack(raw[j], f);
-#pragma unroll
-          for (int e = 0; e < N; ++e)
-            if (!(f[e] < kth_z)) push(f[e], head + at[j] * N + e);
-        }
+    __syncthreads();
+    const int looks = sc.looks, each = UNROLL << group;
+    if (looks <= LOOKS) {
+      for (int w = tid; w < looks * each; w += THREADS) {
+        const int q = w >> (2 + group), look = sc.look[q];
+        const int i = v0 + (((look >> 8) << group) * UNROLL + (w - q * each)) * THREADS + (look & 255);
+        if (i < v1) examine(load_once(zv + (long long)i * 16), i);
       }
+    } else {                     // most of the slice reaches the bound: everyone looks at all of it
+      for (int i = v0 + tid; i < v1; i += THREADS) examine(load_once(zv + (long long)i * 16), i);
     }
     if (tid < extra0 + extra1) push(extra, extra_at);
+    if (tid == 0) sc.counted = 0;
     __syncthreads();
     const int n = sc.listed;
     if (n <= CAP) {
@@ -585,6 +603,16 @@ static int run_forward(const Params& p, cudaStream_t stream) {
   cfg.blockDim = dim3(THREADS);
   cfg.stream = stream;
   cfg.dynamicSmemBytes = p.k > 0 ? sizeof(Scratch) : 0;
+  if (p.k > 0) {                 // beyond the 48 KB that need no asking; told once for each device
+    static std::atomic<unsigned long long> told{0};
+    int device = 0;
+    OB_CUDA_CHECK(cudaGetDevice(&device));
+    const unsigned long long bit = 1ull << (device & 63);
+    if (!(told.load(std::memory_order_relaxed) & bit)) {
+      OB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Scratch)));
+      told.fetch_or(bit, std::memory_order_relaxed);
+    }
+  }
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = p.cluster;
