@@ -238,9 +238,10 @@ __global__ void __launch_bounds__(THREADS, CTAS<HD, NT>) decode_kernel(const __g
       const int mid = (b + hi) >> 1;
       if ((long long)cum[mid] * HC <= ua) b = mid; else hi = mid;
     }
-    const unsigned rel = (unsigned)(ua - (long long)cum[b] * HC), n = cum[b + 1] - cum[b];
-    hc = rel / n;
-    un = rel - hc * n;
+    const long long rel = ua - (long long)cum[b] * HC;
+    const int n = cum[b + 1] - cum[b];
+    hc = (int)quotient(rel, n);
+    un = (int)(rel - (long long)hc * n);
   }
 
   if (p.appended) wait_for_launch_before();      // codes and scales of the new token

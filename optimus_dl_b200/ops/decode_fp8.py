@@ -46,7 +46,7 @@ def _strides(t: torch.Tensor) -> tuple[int, ...]:
     return tuple([s if n > 1 else 0 for n, s in zip(shape, strides)]) if 1 in shape else strides
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class Fp8KVCache:
     """``k``, ``v``: logical ``[B, capacity, Hk, hd]`` float8_e4m3fn with any strides but a unit one in the last
     dimension (a head-major allocation viewed this way reads fastest); ``k_scale``, ``v_scale``: fp32
@@ -226,8 +226,10 @@ def decode_attention_fp8(q: torch.Tensor, k_new: torch.Tensor | None, v_new: tor
 
     ``q``: ``[B, Hq, hd]`` (a strided view into a fused qkv row is fine); ``k_new`` / ``v_new [B, Hk, hd]``: the current
     token's, appended as token ``seq_lens[b] - 1`` first (``None`` if already stored); ``seq_lens``: int32 ``[B]``,
-    counts *including* the current token, taken as the capacity where larger; ``window``: attend to the last so many
-    tokens only. A sequence of length 0 appends nothing and gives zeros. Returns ``[B, Hq, hd]`` of the type of ``q``.
+    counts *including* the current token, taken as the capacity where larger (the new token of such a sequence is not
+    stored: that raises as in :func:`append_kv_fp8`); ``window``: attend to the last so many tokens only, 0 or None to
+    all. A sequence of length 0 appends nothing and gives zeros. Returns ``[B, Hq, hd]`` of the type of ``q``, without
+    a gradient.
     """
     B, capacity, Hk, hd = cache.k.shape
     shape = q.shape

@@ -317,6 +317,23 @@ def test_many_sequences_and_lengths_beyond_the_capacity():
 
 
 @pytest.mark.gpu
+def test_more_sequences_than_a_grid_dimension_holds():
+    B = 70001
+    cache = d8.fp8_kv_cache(B, 5, 1, 32, block=16, device="cuda")
+    k = torch.randn(B, 2, 1, 32, device="cuda").bfloat16()
+    lens = torch.full((B,), 2, dtype=torch.int32, device="cuda")
+    d8.append_kv_fp8(k, -k, cache, lens)
+    d8.append_kv_fp8(2 * k[:, :1], k[:, 1:], cache, lens + 1)
+    s = d8.needed_scale(k.float().abs().amax(dim=(1, 2, 3)))
+    grown = torch.maximum(s, d8.needed_scale(2 * k[:, 0].float().abs().amax(dim=(1, 2))))
+    assert torch.equal(cache.k_scale[:, 0, 0], grown)
+    first = (k.float() / s[:, None, None, None]).to(torch.float8_e4m3fn).float()
+    want = (first * (s / grown)[:, None, None, None]).to(torch.float8_e4m3fn).float()
+    assert torch.equal(cache.k[:, :2].float(), want)
+    assert torch.equal(cache.k[:, 2].float(), (2 * k[:, 0].float() / grown[:, None, None]).to(torch.float8_e4m3fn).float())
+
+
+@pytest.mark.gpu
 def test_strides_of_single_dimensions_mean_nothing_and_odd_rows_are_copied():
     cache = filled(1, 50, 1, 64, 16)
     k = cache.k.as_strided(cache.k.shape, (7, 64, 3, 1))
