@@ -67,11 +67,12 @@ class Fp8KVCache:
         if ks.dtype != torch.float32 or vs.dtype != torch.float32:
             raise TypeError(f"scales must be float32, got {ks.dtype} and {vs.dtype}")
         shape, strides, scale_strides = k.shape, _strides(k), _strides(ks)
-        if len(shape) != 4 or shape != v.shape or strides != _strides(v) or strides[3] > 1:
+        if len(shape) != 4 or shape != v.shape or strides[3] > 1 or (k.stride() != v.stride() and strides != _strides(v)):
             raise ValueError("k and v must be [B, capacity, Hk, hd] of the same shape and strides, contiguous in hd")
         B, capacity, Hk, hd = shape
         want = (B, Hk, -(-capacity // block))
-        if ks.shape != want or vs.shape != want or scale_strides != _strides(vs) or scale_strides[2] > 1:
+        if (ks.shape != want or vs.shape != want or scale_strides[2] > 1
+                or (ks.stride() != vs.stride() and scale_strides != _strides(vs))):
             raise ValueError(f"k_scale and v_scale must be {want} of the same strides, contiguous in the blocks")
         dev = k.device
         if v.device != dev or ks.device != dev or vs.device != dev:
@@ -133,6 +134,14 @@ def _row_strides(t: torch.Tensor) -> tuple[torch.Tensor, tuple[int, ...]]:
 
 
 def _new_rows(k_new: torch.Tensor, v_new: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, tuple[int, ...]]:
+    """New keys and values as the kernels take them: rows on 16-byte boundaries, the same strides for both."""
+    if k_new.stride() == v_new.stride():
+        strides, size = _strides(k_new), k_new.element_size()
+        bits = k_new.data_ptr() | v_new.data_ptr()
+        for s in strides[:-1]:
+            bits |= s * size
+        if strides[-1] <= 1 and not bits & 15:
+            return k_new, v_new, strides
     k_new, k_strides = _row_strides(k_new)
     v_new, v_strides = _row_strides(v_new)
     if k_strides != v_strides:
@@ -252,7 +261,7 @@ def decode_attention_fp8(q: torch.Tensor, k_new: torch.Tensor | None, v_new: tor
     scale = scale if scale is not None else 1.0 / math.sqrt(hd)
     if not (cache._kernels and has_kernel(hd, dtype)):
         return decode_attention_fp8_ref(q, k_new, v_new, cache, seq_lens, scale=scale, window=window)
-    out = torch.empty(shape, dtype=dtype, device=cache._device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if B == 0 or Hq == 0:
         return out
     q, (q_batch, q_head, _) = _row_strides(q)

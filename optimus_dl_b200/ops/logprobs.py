@@ -117,11 +117,12 @@ def _forward(z: torch.Tensor, targets: torch.Tensor, top_k: int, temperature: fl
     maximum and log2 sum of every row as pairs."""
     rows, vocab = z.shape
     dev = z.device
-    num = torch.empty((4 if keep else 2, rows), dtype=torch.float32, device=dev)
+    # empty_strided: the cheapest way to a new tensor on the host
+    num = torch.empty_strided((4 if keep else 2, rows), (rows, 1), dtype=torch.float32, device=dev)
     top_logp = top_ids = None
     if top_k:
-        top_logp = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
-        top_ids = torch.empty((rows, top_k), dtype=torch.int64, device=dev)
+        top_logp = torch.empty_strided((rows, top_k), (top_k, 1), dtype=torch.float32, device=dev)
+        top_ids = torch.empty_strided((rows, top_k), (top_k, 1), dtype=torch.int64, device=dev)
     at = num.data_ptr()
     with _lib.on_device(dev):
         _launch_forward(z.data_ptr(), z.stride(0), _KERNEL_DTYPES[z.dtype], targets.data_ptr(), at, at + 4 * rows,
@@ -139,7 +140,7 @@ def _backward(z: torch.Tensor, targets: torch.Tensor, num: torch.Tensor, d_logp:
     """``d loss / d z`` from what ``_forward`` kept; ``out`` may be ``z`` itself."""
     rows, vocab = z.shape
     if out is None:
-        out = torch.empty((rows, vocab), dtype=z.dtype, device=z.device)
+        out = torch.empty_like(z, memory_format=torch.contiguous_format)
     # the converted gradients live until the launch has been queued
     d_logp = None if d_logp is None else _rows_fp32(d_logp)
     d_entropy = None if d_entropy is None else _rows_fp32(d_entropy)
