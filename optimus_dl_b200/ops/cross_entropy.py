@@ -219,7 +219,7 @@ class _LinearTokenLoss(torch.autograd.Function):
                 out_view = logits_buf[:rows].as_strided((rows, V), (ld, 1))
                 gemm.gemm(x2[r0:r1], weight, out=out_view)
             if entropy_weight is not None:
-                logp, entropy_all[r0:r1], _, _, num = lp_ops._forward(out_view, tg[r0:r1], 0, 1.0, True)
+                logp, entropy_all[r0:r1], _, _, kept = lp_ops._forward(out_view, tg[r0:r1], 0, 1.0, True)
                 nll = -logp
             elif not fused:
                 rc = l.ob_ce_stats(_lib.ptr(out_view), ld, _lib.ptr(tg[r0:r1]), _lib.ptr(st[0]), _lib.ptr(st[1]),
@@ -237,7 +237,7 @@ class _LinearTokenLoss(torch.autograd.Function):
             if need_dx or need_dw:
                 w_rows = dl_dnll.to(torch.float32).contiguous()
             if (need_dx or need_dw) and entropy_weight is not None:
-                lp_ops._backward(out_view, tg[r0:r1], num, -w_rows, entropy_weight[r0:r1], 1.0, out=out_view)
+                lp_ops._backward(out_view, tg[r0:r1], kept, -w_rows, entropy_weight[r0:r1], 1.0, out=out_view)
             elif need_dx or need_dw:
                 rc = l.ob_ce_grad(_lib.ptr(out_view), ld, _lib.ptr(tg[r0:r1]), _lib.ptr(lse.contiguous()), rows, V, 0, V,
                                   -(1 << 62), 0.0, None, 1.0, 0, 1.0, _lib.ptr(w_rows), _lib.stream())

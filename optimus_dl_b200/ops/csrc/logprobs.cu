@@ -179,7 +179,8 @@ __device__ __forceinline__ void join(Sums& a, const Sums& b, float c) {
 struct Params {
   const void* logits; long long ld;
   const long long* targets;
-  float* logp; float* entropy; float2* stats;     // stats: (max, log2 S), what the gradient needs beside the entropy
+  float* logp; float* entropy;
+  float2* stats; float* kept;                     // for the gradient: (max, log2 S) and the entropy once more
   float* top_logp; long long* top_ids;
   int rows, V, k, cluster;
   float c;
@@ -510,8 +511,12 @@ __global__ void __launch_bounds__(THREADS, 4) forward_kernel(const __grid_consta
   const float log2s = fabsf(top_z) < HUGE_LOGIT ? sum_log2 - fmaf(top_z, c, -__fmul_rn(top_z, c)) : sum_log2;
   if (tid == 0) {
     p.logp[row] = inside ? log_of(z_t, top_z, c, log2s) : 0.f;
-    p.entropy[row] = none ? 0.f : (sum_log2 - total.w / total.s) * 0.6931471805599453f;
-    if (p.stats) p.stats[row] = make_float2(total.m, log2s);
+    const float h = none ? 0.f : (sum_log2 - total.w / total.s) * 0.6931471805599453f;
+    p.entropy[row] = h;
+    if (p.stats) {
+      p.stats[row] = make_float2(total.m, log2s);
+      p.kept[row] = h;
+    }
   }
   if (TOPK && tid < p.k) {
     const u64 cand = p.cluster > 1 ? sc.merged[tid] : sc.top[tid];
@@ -678,7 +683,8 @@ struct ForwardArgs {
   long long ld, dtype;
   const long long* targets;
   float *logp, *entropy;
-  float2* stats;                // may be null
+  float2* stats;                // may be null, and with it:
+  float* kept;
   float* top_logp;
   long long* top_ids;
   long long rows, V, top_k;
@@ -696,7 +702,7 @@ struct BackwardArgs {
   double temperature;
   cudaStream_t stream;
 };
-static_assert(sizeof(ForwardArgs) == 14 * 8 && sizeof(BackwardArgs) == 14 * 8, "packed");
+static_assert(sizeof(ForwardArgs) == 15 * 8 && sizeof(BackwardArgs) == 14 * 8, "packed");
 
 extern "C" int ob_logprobs_fwd(const void* packed) {
   ForwardArgs a;
@@ -709,7 +715,7 @@ extern "C" int ob_logprobs_fwd(const void* packed) {
   if (V <= 0 || top_k < 0 || top_k > MAX_TOPK || top_k > V || !(temperature >= 1e-6 && temperature <= 1e6)) return -1;
   const int cl = pick_cluster(rows, V, dtype == 2 ? 4 : 8);
   if ((long long)rows * cl > 0x7fffffffLL) return -1;
-  const Params p{a.logits, a.ld, a.targets, a.logp, a.entropy, a.stats, a.top_logp, a.top_ids, rows, V, top_k, cl,
+  const Params p{a.logits, a.ld, a.targets, a.logp, a.entropy, a.stats, a.kept, a.top_logp, a.top_ids, rows, V, top_k, cl,
                  (float)(1.4426950408889634 / temperature)};
   if (dtype == 0) return run_forward<__nv_bfloat16>(p, stream);
   if (dtype == 1) return run_forward<__half>(p, stream);

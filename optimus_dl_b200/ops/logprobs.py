@@ -32,7 +32,7 @@ from . import _lib, gemm
 
 MAX_TOP_K = 32
 _KERNEL_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-_launch_forward = _lib.Packed("ob_logprobs_fwd", "QqqQQQQQQqqqdQ")
+_launch_forward = _lib.Packed("ob_logprobs_fwd", "QqqQQQQQQQqqqdQ")
 _launch_backward = _lib.Packed("ob_logprobs_bwd", "QqqQQQQQQqqqdQ")
 
 
@@ -92,7 +92,7 @@ class _TokenLogprobsRef(torch.autograd.Function):
         ctx.save_for_backward(log_p, entropy, inside & ~none.squeeze(-1), at)
         ctx.dtype, ctx.temperature = logits.dtype, temperature
         ctx.mark_non_differentiable(*(t for t in (top_logp, top_ids) if t is not None))
-        return logp, entropy.squeeze(-1), top_logp, top_ids
+        return logp, entropy.squeeze(-1).clone(), top_logp, top_ids      # what is kept is not shared
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -113,29 +113,32 @@ def token_logprobs_ref(logits: torch.Tensor, targets: torch.Tensor, *, top_k: in
 
 def _forward(z: torch.Tensor, targets: torch.Tensor, top_k: int, temperature: float, keep: bool):
     """Kernel call on ``z [rows, V]`` (unit column stride) and contiguous int64 ``targets [rows]``. Returns ``logp,
-    entropy, top_logp, top_ids, num``; with ``keep``, ``num[1:]`` is what the gradient needs: the entropy, and the
-    maximum and log2 sum of every row as pairs."""
+    entropy, top_logp, top_ids, kept``; with ``keep``, ``kept`` is what the gradient needs, none of it shared with the
+    results: the maximum and log2 sum of every row as pairs, then the entropy."""
     rows, vocab = z.shape
     dev = z.device
-    # empty_strided: the cheapest way to a new tensor on the host
-    num = torch.empty_strided((4 if keep else 2, rows), (rows, 1), dtype=torch.float32, device=dev)
-    top_logp = top_ids = None
-    if top_k:
+    logp = torch.empty(rows, dtype=torch.float32, device=dev)
+    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
+    top_logp = top_ids = kept = None
+    pairs = 0
+    if keep:
+        kept = torch.empty(3 * rows, dtype=torch.float32, device=dev)
+        pairs = kept.data_ptr()
+    if top_k:      # empty_strided: the cheapest way to a new tensor on the host
         top_logp = torch.empty_strided((rows, top_k), (top_k, 1), dtype=torch.float32, device=dev)
         top_ids = torch.empty_strided((rows, top_k), (top_k, 1), dtype=torch.int64, device=dev)
-    at = num.data_ptr()
     with _lib.on_device(dev):
-        _launch_forward(z.data_ptr(), z.stride(0), _KERNEL_DTYPES[z.dtype], targets.data_ptr(), at, at + 4 * rows,
-                        at + 8 * rows if keep else 0, top_logp.data_ptr() if top_k else 0,
+        _launch_forward(z.data_ptr(), z.stride(0), _KERNEL_DTYPES[z.dtype], targets.data_ptr(), logp.data_ptr(),
+                        entropy.data_ptr(), pairs, pairs + 8 * rows, top_logp.data_ptr() if top_k else 0,
                         top_ids.data_ptr() if top_k else 0, rows, vocab, top_k, temperature, _lib.raw_stream())
-    return num[0], num[1], top_logp, top_ids, num
+    return logp, entropy, top_logp, top_ids, kept
 
 
 def _rows_fp32(g: torch.Tensor) -> torch.Tensor:
     return g if g.dtype == torch.float32 and g.is_contiguous() else g.to(torch.float32).contiguous()
 
 
-def _backward(z: torch.Tensor, targets: torch.Tensor, num: torch.Tensor, d_logp: torch.Tensor | None,
+def _backward(z: torch.Tensor, targets: torch.Tensor, kept: torch.Tensor, d_logp: torch.Tensor | None,
               d_entropy: torch.Tensor | None, temperature: float, out: torch.Tensor | None = None) -> torch.Tensor:
     """``d loss / d z`` from what ``_forward`` kept; ``out`` may be ``z`` itself."""
     rows, vocab = z.shape
@@ -144,10 +147,10 @@ def _backward(z: torch.Tensor, targets: torch.Tensor, num: torch.Tensor, d_logp:
     # the converted gradients live until the launch has been queued
     d_logp = None if d_logp is None else _rows_fp32(d_logp)
     d_entropy = None if d_entropy is None else _rows_fp32(d_entropy)
-    at = num.data_ptr()
+    at = kept.data_ptr()
     with _lib.on_device(z.device):
-        _launch_backward(z.data_ptr(), z.stride(0), _KERNEL_DTYPES[z.dtype], targets.data_ptr(), at + 8 * rows,
-                         at + 4 * rows, 0 if d_logp is None else d_logp.data_ptr(),
+        _launch_backward(z.data_ptr(), z.stride(0), _KERNEL_DTYPES[z.dtype], targets.data_ptr(), at, at + 8 * rows,
+                         0 if d_logp is None else d_logp.data_ptr(),
                          0 if d_entropy is None else d_entropy.data_ptr(), out.data_ptr(), out.stride(0), rows, vocab,
                          temperature, _lib.raw_stream())
     return out
@@ -156,8 +159,8 @@ def _backward(z: torch.Tensor, targets: torch.Tensor, num: torch.Tensor, d_logp:
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, targets, top_k, temperature):
-        logp, entropy, top_logp, top_ids, num = _forward(z, targets, top_k, temperature, True)
-        ctx.save_for_backward(z, targets, num)
+        logp, entropy, top_logp, top_ids, kept = _forward(z, targets, top_k, temperature, True)
+        ctx.save_for_backward(z, targets, kept)
         ctx.temperature = temperature
         ctx.set_materialize_grads(False)
         if not top_k:
@@ -170,8 +173,8 @@ class _TokenLogprobs(torch.autograd.Function):
     def backward(ctx, d_logp, d_entropy, *_):
         if d_logp is None and d_entropy is None:
             return None, None, None, None
-        z, targets, num = ctx.saved_tensors
-        return _backward(z, targets, num, d_logp, d_entropy, ctx.temperature), None, None, None
+        z, targets, kept = ctx.saved_tensors
+        return _backward(z, targets, kept, d_logp, d_entropy, ctx.temperature), None, None, None
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top_k: int = 0,

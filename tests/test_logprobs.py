@@ -163,6 +163,28 @@ def test_linear_form_and_shapes():
     assert empty.logp.shape == (0, 5) and empty.top_ids.shape == (0, 5, 3)
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_results_may_be_changed_in_place(device):
+    """Masking the results in place, as losses do, neither fails nor changes the gradient of the others."""
+    z, t = make(6, 301, torch.float32, seed=9)
+    z, t = z.to(device), t.to(device)
+    grads = []
+    for in_place in (True, False):
+        x = z.clone().requires_grad_(True)
+        r = lp.token_logprobs(x, t, top_k=2)
+        keep = torch.tensor([1.0, 0, 1, 1, 0, 1], device=device)
+        logp, h = r.logp, r.entropy
+        if in_place:
+            logp.mul_(keep)
+            h[2] = 0.0
+            r.top_logp.zero_()
+        else:
+            logp, h = logp * keep, torch.where(torch.arange(6, device=device) == 2, 0.0, h)
+        (logp.sum() + 2 * h.sum()).backward()
+        grads.append(x.grad)
+    assert torch.equal(*grads)
+
+
 # ------------------------------------------------------------------------------------------------ GPU
 CASES = [(1, 1, 1), (1, 2, 2), (3, 97, 5), (2, 2047, 32), (5, 4097, 20), (2, 8209, 32), (1, 50257, 20), (17, 50257, 1),
          (3, 128256, 20), (2, 200003, 32)]
