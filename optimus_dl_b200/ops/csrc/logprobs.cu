@@ -28,7 +28,6 @@
 // (thousands of equal logits in one thread's share) is replaced by k plain arg-max passes.
 #include "common.cuh"
 #include <cooperative_groups.h>
-#include <atomic>
 #include <string.h>
 
 namespace ob {
@@ -36,7 +35,8 @@ namespace logprobs {
 
 namespace cg = cooperative_groups;
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 256;     // of the gradient's CTAs and, with few rows, of the forward's
+constexpr int NARROW = 128;      // of the forward's with many rows
 constexpr int UNROLL = 4;        // 16-byte loads in flight per thread
 constexpr int MAX_TOPK = 32;
 constexpr int CAP = 512;        // candidates a CTA can list
@@ -192,9 +192,10 @@ __device__ __forceinline__ float log_of(float z, float m, float c, float log2s) 
 
 // Of a CTA that looks for alternatives.  Kept to some 28 KB: four CTAs of 54 KB left the SM so little of its L1 cache for
 // the loads in flight that 1000 rows of 50257 fp32 took 54 us instead of 43.
+template <int TH>
 struct Scratch {
-  u64 list[CAP], few[CAP], top[MAX_TOPK], merged[MAX_TOPK], warp_bound[THREADS / 32], kth;
-  float note[NOTES][THREADS];
+  u64 list[CAP], few[CAP], top[MAX_TOPK], merged[MAX_TOPK], warp_bound[TH / 32], kth;
+  float note[NOTES][TH];
   int look[LOOKS];
   int listed, counted, looks;
 };
@@ -202,8 +203,9 @@ struct Scratch {
 // A lower bound of the k-th best of the CTA's candidates, one per thread; the first `active` threads have one (0
 // elsewhere).  The r-th best of the lanes in each of W warps, r = ceil(k / W), and the least of those: r W >= k
 // candidates reach it.  0 when there are too few to tell.  One barrier, before the result is read.
+template <int TH>
 __device__ __forceinline__ u64 bound(u64 best, int active, int k, u64* warp_bound) {
-  const int warps = max(1, min(active, THREADS) >> 5), warp = threadIdx.x >> 5;
+  const int warps = max(1, min(active, TH) >> 5), warp = threadIdx.x >> 5;
   if (warp < warps) {
     u64 w = 0;
     for (int i = (k + warps - 1) / warps; i > 0; --i) {
@@ -222,18 +224,19 @@ __device__ __forceinline__ u64 bound(u64 best, int active, int k, u64* warp_boun
 
 // The k best of `n` candidates in `list` (0 = none), best first.  Barriers inside, none at the end; sc.counted is 0
 // before.
-__device__ __forceinline__ void select_top(const u64* list, int n, int k, u64* top, Scratch& sc) {
+template <int TH>
+__device__ __forceinline__ void select_top(const u64* list, int n, int k, u64* top, Scratch<TH>& sc) {
   if (n > 64) {
     u64 best = 0;
-    for (int i = threadIdx.x; i < n; i += THREADS) best = max(best, list[i]);
-    const u64 b = bound(best, n, k, sc.warp_bound);
-    for (int i = threadIdx.x; i < n; i += THREADS)
+    for (int i = threadIdx.x; i < n; i += TH) best = max(best, list[i]);
+    const u64 b = bound<TH>(best, n, k, sc.warp_bound);
+    for (int i = threadIdx.x; i < n; i += TH)
       if (list[i] >= b && list[i] != 0) sc.few[atomicAdd(&sc.counted, 1)] = list[i];
     __syncthreads();
     n = sc.counted;
     list = sc.few;
   }
-  for (int i = threadIdx.x; i < n; i += THREADS) {
+  for (int i = threadIdx.x; i < n; i += TH) {
     const u64 mine = list[i];
     int r = 0;
 #pragma unroll 8
@@ -242,15 +245,14 @@ __device__ __forceinline__ void select_top(const u64* list, int n, int k, u64* t
   }
 }
 
-static_assert(UNROLL == 4 && THREADS == 256, "how a look is packed and shared out");
-
-template <typename T, bool TOPK>
-__global__ void __launch_bounds__(THREADS, 4) forward_kernel(const __grid_constant__ Params p) {
-  constexpr int N = Vec<T>::N, STEP = THREADS * UNROLL;
-  __shared__ Sums warp_sums[THREADS / 32];
+template <typename T, bool TOPK, int TH>
+__global__ void __launch_bounds__(TH, 1024 / TH) forward_kernel(const __grid_constant__ Params p) {
+  static_assert(UNROLL == 4 && TH <= 256, "how a look is packed and shared out");
+  constexpr int N = Vec<T>::N, STEP = TH * UNROLL;
+  __shared__ Sums warp_sums[TH / 32];
   __shared__ Sums cta_sums;
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  Scratch& sc = *reinterpret_cast<Scratch*>(smem_raw);          // TOPK only
+  auto& sc = *reinterpret_cast<Scratch<TH>*>(smem_raw);          // TOPK only
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x / p.cluster, rank = blockIdx.x - row * p.cluster;
   const T* z = static_cast<const T*>(p.logits) + (long long)row * p.ld;
@@ -264,12 +266,12 @@ __global__ void __launch_bounds__(THREADS, 4) forward_kernel(const __grid_consta
   auto fetch = [&](int base, uint4 (&raw)[UNROLL]) {             // from `at`; what lies behind the slice reads as banned
     if (base + STEP <= v1) {
 #pragma unroll
-      for (int j = 0; j < UNROLL; ++j) raw[j] = load_once(at + j * THREADS * 16);
+      for (int j = 0; j < UNROLL; ++j) raw[j] = load_once(at + j * TH * 16);
     } else {
 #pragma unroll
       for (int j = 0; j < UNROLL; ++j) {
         raw[j] = make_uint4(Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE);
-        if (base + j * THREADS + tid < v1) raw[j] = load_once(at + j * THREADS * 16);
+        if (base + j * TH + tid < v1) raw[j] = load_once(at + j * TH * 16);
       }
     }
     at += STEP * 16;
@@ -304,9 +306,9 @@ __global__ void __launch_bounds__(THREADS, 4) forward_kernel(const __grid_consta
       mx = max_nan(mx, top_of[j]);
     }
     if (TOPK && !(mx <= m)) {
-      best_vec = base + (UNROLL - 1) * THREADS + tid;
+      best_vec = base + (UNROLL - 1) * TH + tid;
 #pragma unroll
-      for (int j = UNROLL - 2; j >= 0; --j) if (top_of[j] == mx) best_vec = base + j * THREADS + tid;
+      for (int j = UNROLL - 2; j >= 0; --j) if (top_of[j] == mx) best_vec = base + j * TH + tid;
     }
     if (TOPK) {
       const int batch = (base - v0) / STEP;
@@ -376,9 +378,9 @@ __global__ void __launch_bounds__(THREADS, 4) forward_kernel(const __grid_consta
   if (lane == 0) warp_sums[warp] = st;
   __syncthreads();
   if (warp == 0) {
-    Sums t = lane < THREADS / 32 ? warp_sums[lane] : Sums{-INFINITY, 0.f, 0.f};
+    Sums t = lane < TH / 32 ? warp_sums[lane] : Sums{-INFINITY, 0.f, 0.f};
 #pragma unroll
-    for (int o = THREADS / 64; o > 0; o >>= 1) {
+    for (int o = TH / 64; o > 0; o >>= 1) {
       Sums b;
       b.m = __shfl_xor_sync(0xffffffffu, t.m, o);
       b.s = __shfl_xor_sync(0xffffffffu, t.s, o);
@@ -389,11 +391,11 @@ __global__ void __launch_bounds__(THREADS, 4) forward_kernel(const __grid_consta
   }
   if (TOPK) {
     // the k-th best of the threads' maxima
-    const u64 rough = bound(mine, v1 - v0, p.k, sc.warp_bound);
+    const u64 rough = bound<TH>(mine, v1 - v0, p.k, sc.warp_bound);
     if (mine != 0 && mine >= rough) sc.list[atomicAdd(&sc.counted, 1)] = mine;
     __syncthreads();
     const int near = sc.counted;
-    for (int i = tid; i < near; i += THREADS) {
+    for (int i = tid; i < near; i += TH) {
       const u64 m = sc.list[i];
       int r = 0;
 #pragma unroll 8
@@ -430,13 +432,13 @@ __global__ void __launch_bounds__(THREADS, 4) forward_kernel(const __grid_consta
     __syncthreads();
     const int looks = sc.looks, each = UNROLL << group;
     if (looks <= LOOKS) {
-      for (int w = tid; w < looks * each; w += THREADS) {
+      for (int w = tid; w < looks * each; w += TH) {
         const int q = w >> (2 + group), look = sc.look[q];
-        const int i = v0 + (((look >> 8) << group) * UNROLL + (w - q * each)) * THREADS + (look & 255);
+        const int i = v0 + (((look >> 8) << group) * UNROLL + (w - q * each)) * TH + (look & 255);
         if (i < v1) examine(load_once(zv + (long long)i * 16), i);
       }
     } else {                     // most of the slice reaches the bound: everyone looks at all of it
-      for (int i = v0 + tid; i < v1; i += THREADS) examine(load_once(zv + (long long)i * 16), i);
+      for (int i = v0 + tid; i < v1; i += TH) examine(load_once(zv + (long long)i * 16), i);
     }
     if (tid < extra0 + extra1) push(extra, extra_at);
     if (tid == 0) sc.counted = 0;
@@ -449,7 +451,7 @@ __global__ void __launch_bounds__(THREADS, 4) forward_kernel(const __grid_consta
       u64 limit = ~0ull;
       for (int r = 0; r < p.k; ++r) {
         u64 best = 0;
-        for (int i = v0 + tid; i < v1; i += THREADS) {
+        for (int i = v0 + tid; i < v1; i += TH) {
           float f[N];
           Vec<T>::unpack(load_once(zv + (long long)i * 16), f);
 #pragma unroll
@@ -468,7 +470,7 @@ __global__ void __launch_bounds__(THREADS, 4) forward_kernel(const __grid_consta
         if (lane == 0) sc.list[warp] = best;
         __syncthreads();
         best = sc.list[0];
-        for (int i = 1; i < THREADS / 32; ++i) best = max(best, sc.list[i]);
+        for (int i = 1; i < TH / 32; ++i) best = max(best, sc.list[i]);
         if (tid == 0) sc.top[r] = best;
         if (best == 0) break;
         limit = best;
@@ -494,7 +496,7 @@ __global__ void __launch_bounds__(THREADS, 4) forward_kernel(const __grid_consta
       }
       if (TOPK) {
         const int n = p.cluster * p.k;
-        for (int i = tid; i < n; i += THREADS) sc.list[i] = cl.map_shared_rank(sc.top, i / p.k)[i % p.k];
+        for (int i = tid; i < n; i += TH) sc.list[i] = cl.map_shared_rank(sc.top, i / p.k)[i % p.k];
         if (tid == 0) sc.counted = 0;
         __syncthreads();
         select_top(sc.list, n, p.k, sc.merged, sc);
@@ -635,24 +637,15 @@ backward_kernel(const T* logits, long long ld, const long long* __restrict__ tar
   }
 }
 
-template <typename T>
-static int run_forward(const Params& p, cudaStream_t stream) {
-  auto kern = p.k > 0 ? forward_kernel<T, true> : forward_kernel<T, false>;
+template <typename T, bool TOPK, int TH>
+static int launch_forward(const Params& p, cudaStream_t stream) {
+  auto kern = forward_kernel<T, TOPK, TH>;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((long long)p.rows * p.cluster));
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(TH);
   cfg.stream = stream;
-  cfg.dynamicSmemBytes = p.k > 0 ? sizeof(Scratch) : 0;
-  if (p.k > 0) {                 // beyond the 48 KB that need no asking; told once for each device
-    static std::atomic<unsigned long long> told{0};
-    int device = 0;
-    OB_CUDA_CHECK(cudaGetDevice(&device));
-    const unsigned long long bit = 1ull << (device & 63);
-    if (!(told.load(std::memory_order_relaxed) & bit)) {
-      OB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Scratch)));
-      told.fetch_or(bit, std::memory_order_relaxed);
-    }
-  }
+  cfg.dynamicSmemBytes = TOPK ? sizeof(Scratch<TH>) : 0;
+  static_assert(sizeof(Scratch<TH>) <= 48 * 1024, "what needs no asking");
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = p.cluster;
@@ -660,6 +653,16 @@ static int run_forward(const Params& p, cudaStream_t stream) {
   cfg.attrs = attr;
   cfg.numAttrs = p.cluster > 1 ? 1 : 0;
   return (int)cudaLaunchKernelEx(&cfg, kern, p);
+}
+
+// Rows enough to fill the SMs four times over go to CTAs of 128 threads, eight to an SM: their latencies at the start
+// and the end of a row overlap with more of the others. Measured, 128 against 256 threads: 1000 rows of 50257 fp32 37.6
+// and 43.0 us, 4096 of 128256 bf16 with 20 alternatives 183 and 193, without 160 and 162, 8192 in a long run 365 and 375;
+// but 257 rows of 50257 fp32 17.8 and 13.7, 64 of 151936 with 20 alternatives 17.3 and 15.7.
+template <typename T>
+static int run_forward(const Params& p, cudaStream_t stream) {
+  if (p.rows >= 148 * 4) return p.k > 0 ? launch_forward<T, true, NARROW>(p, stream) : launch_forward<T, false, NARROW>(p, stream);
+  return p.k > 0 ? launch_forward<T, true, THREADS>(p, stream) : launch_forward<T, false, THREADS>(p, stream);
 }
 
 // CTAs that share a row: as many as make two per SM with the rows there are, each with at least one full batch of

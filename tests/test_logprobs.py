@@ -187,7 +187,8 @@ def test_results_may_be_changed_in_place(device):
 
 # ------------------------------------------------------------------------------------------------ GPU
 CASES = [(1, 1, 1), (1, 2, 2), (3, 97, 5), (2, 2047, 32), (5, 4097, 20), (2, 8209, 32), (1, 50257, 20), (17, 50257, 1),
-         (3, 128256, 20), (2, 200003, 32)]
+         (3, 128256, 20), (2, 200003, 32),
+         (600, 97, 5), (601, 2053, 20)]         # rows for narrow CTAs
 
 
 @pytest.mark.gpu
