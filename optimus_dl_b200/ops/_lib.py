@@ -128,11 +128,11 @@ def stream() -> c_void_p:
     return c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def raw_stream() -> int:
-    """:func:`stream` as a plain integer, for calls where the host's time counts."""
+def raw_stream(index: int) -> int:
+    """The current stream of device ``index`` as a plain integer, for calls where the host's time counts."""
     if _raw_stream is not None:
-        return _raw_stream(torch.cuda.current_device())
-    return torch.cuda.current_stream().cuda_stream
+        return _raw_stream(index)
+    return torch.cuda.current_stream(index).cuda_stream
 
 
 class _Here:

@@ -84,7 +84,8 @@ class Fp8KVCache:
         else:
             kernels, geometry, status = False, None, None
         # the status word exists before any capture into a graph
-        self.__dict__.update(_device=dev, _kernels=kernels, _geometry=geometry, _status=status)
+        self.__dict__.update(_device=dev, _index=k.get_device(), _shape=tuple(shape), _kernels=kernels, _geometry=geometry,
+                             _status=status)
 
     def _args(self) -> tuple:
         """What describes the cache to the kernels: codes and their strides, scales and theirs."""
@@ -110,12 +111,12 @@ def _check_new(k_new: torch.Tensor, v_new: torch.Tensor, cache: Fp8KVCache, want
         raise ValueError(f"new keys and values must be {want}, got {tuple(k_new.shape)} and {tuple(v_new.shape)}")
     if k_new.dtype != v_new.dtype or k_new.dtype not in _DTYPES:
         raise TypeError(f"new keys and values must share one of bf16, fp16, fp32: got {k_new.dtype}, {v_new.dtype}")
-    if k_new.device != cache._device or v_new.device != cache._device:
+    if k_new.get_device() != cache._index or v_new.get_device() != cache._index:
         raise ValueError("new keys and values must be on the cache's device")
 
 
 def _check_counts(t: torch.Tensor, cache: Fp8KVCache, batch: int, what: str) -> None:
-    if t.dtype != torch.int32 or t.shape != (batch,) or t.device != cache._device or not t.is_contiguous():
+    if t.dtype != torch.int32 or t.shape != (batch,) or t.get_device() != cache._index or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous int32 [{batch}] on the cache's device, got {t.dtype} "
                          f"{tuple(t.shape)} on {t.device}")
 
@@ -160,7 +161,7 @@ def append_kv_fp8(k_new: torch.Tensor, v_new: torch.Tensor, cache: Fp8KVCache, s
     the sequence has, a length beyond the capacity) raise on the CPU; on CUDA the sequence is left as it was and
     ``ops._lib.check_status`` raises.
     """
-    B, capacity, Hk, hd = cache.k.shape
+    B, capacity, Hk, hd = cache._shape
     if k_new.dim() != 4:
         raise ValueError(f"new keys must be [B, T, Hk, hd], got {tuple(k_new.shape)}")
     T = k_new.shape[1]
@@ -177,7 +178,7 @@ def append_kv_fp8(k_new: torch.Tensor, v_new: torch.Tensor, cache: Fp8KVCache, s
     with _lib.on_device(cache._device):
         _launch_append(k_new.data_ptr(), v_new.data_ptr(), _DTYPES[k_new.dtype], nb, nt, nh, *cache._args(),
                        seq_lens.data_ptr(), 0 if n_new is None else n_new.data_ptr(), B, T, Hk, hd, capacity, cache.block,
-                       cache._status.data_ptr(), _lib.raw_stream())
+                       cache._status.data_ptr(), _lib.raw_stream(cache._index))
 
 
 def needed_scale(amax: torch.Tensor) -> torch.Tensor:
@@ -240,14 +241,14 @@ def decode_attention_fp8(q: torch.Tensor, k_new: torch.Tensor | None, v_new: tor
     all. A sequence of length 0 appends nothing and gives zeros. Returns ``[B, Hq, hd]`` of the type of ``q``, without
     a gradient.
     """
-    B, capacity, Hk, hd = cache.k.shape
+    B, capacity, Hk, hd = cache._shape
     shape = q.shape
     if len(shape) != 3 or shape[0] != B or shape[2] != hd or shape[1] % Hk:
         raise ValueError(f"q {tuple(shape)} does not fit a cache of {tuple(cache.k.shape)}")
     dtype, Hq = q.dtype, shape[1]
     if not dtype.is_floating_point:
         raise TypeError(f"q must be floating point, got {dtype}")
-    if q.device != cache._device:
+    if q.get_device() != cache._index:
         raise ValueError("q must be on the cache's device")
     _check_counts(seq_lens, cache, B, "seq_lens")
     if (k_new is None) != (v_new is None):
@@ -264,9 +265,9 @@ def decode_attention_fp8(q: torch.Tensor, k_new: torch.Tensor | None, v_new: tor
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if B == 0 or Hq == 0:
         return out
-    q, (q_batch, q_head, _) = _row_strides(q)
-    if q_head not in (0, hd):
-        q = q.contiguous()
+    q_batch, q_head, q_last = q.stride()
+    if q_last != 1 or q_head != hd or (2 * q_batch | q.data_ptr()) & 15:
+        q = q.clone(memory_format=torch.contiguous_format)
         q_batch = Hq * hd
     new_k = new_v = new_batch = new_head = 0
     if k_new is not None:
@@ -276,7 +277,7 @@ def decode_attention_fp8(q: torch.Tensor, k_new: torch.Tensor | None, v_new: tor
     with _lib.on_device(cache._device):
         _launch_attention(q.data_ptr(), q_batch, _DTYPES[dtype], new_k, new_v, new_batch, new_head, *cache._args(),
                           seq_lens.data_ptr(), out.data_ptr(), ws.data_ptr(), B, Hq, Hk, hd, capacity, cache.block, scale,
-                          window or 0, cache._status.data_ptr(), _lib.raw_stream())
+                          window or 0, cache._status.data_ptr(), _lib.raw_stream(cache._index))
     return out
 
 

@@ -52,7 +52,7 @@ def _check(rows_shape: torch.Size, vocab: int, floating: torch.Tensor, targets: 
         raise TypeError(f"targets must be token ids of an integer type, got {targets.dtype}")
     if targets.shape != rows_shape:
         raise ValueError(f"targets have shape {tuple(targets.shape)}, the rows of logits {tuple(rows_shape)}")
-    if targets.device != floating.device:
+    if targets.get_device() != floating.get_device():
         raise ValueError(f"targets are on {targets.device}, logits on {floating.device}")
     if vocab < 1:
         raise ValueError("logits need at least one token")
@@ -130,7 +130,7 @@ def _forward(z: torch.Tensor, targets: torch.Tensor, top_k: int, temperature: fl
     with _lib.on_device(dev):
         _launch_forward(z.data_ptr(), z.stride(0), _KERNEL_DTYPES[z.dtype], targets.data_ptr(), logp.data_ptr(),
                         entropy.data_ptr(), pairs, pairs + 8 * rows, top_logp.data_ptr() if top_k else 0,
-                        top_ids.data_ptr() if top_k else 0, rows, vocab, top_k, temperature, _lib.raw_stream())
+                        top_ids.data_ptr() if top_k else 0, rows, vocab, top_k, temperature, _lib.raw_stream(dev.index))
     return logp, entropy, top_logp, top_ids, kept
 
 
@@ -152,7 +152,7 @@ def _backward(z: torch.Tensor, targets: torch.Tensor, kept: torch.Tensor, d_logp
         _launch_backward(z.data_ptr(), z.stride(0), _KERNEL_DTYPES[z.dtype], targets.data_ptr(), at, at + 8 * rows,
                          0 if d_logp is None else d_logp.data_ptr(),
                          0 if d_entropy is None else d_entropy.data_ptr(), out.data_ptr(), out.stride(0), rows, vocab,
-                         temperature, _lib.raw_stream())
+                         temperature, _lib.raw_stream(z.device.index))
     return out
 
 
