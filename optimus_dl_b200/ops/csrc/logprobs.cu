@@ -437,8 +437,19 @@ __global__ void __launch_bounds__(TH, 1024 / TH) forward_kernel(const __grid_con
         const int i = v0 + (((look >> 8) << group) * UNROLL + (w - q * each)) * TH + (look & 255);
         if (i < v1) examine(load_once(zv + (long long)i * 16), i);
       }
-    } else {                     // most of the slice reaches the bound: everyone looks at all of it
-      for (int i = v0 + tid; i < v1; i += TH) examine(load_once(zv + (long long)i * 16), i);
+    } else {
+      // Much of the slice reaches the bound: everyone looks at all of it, or, where nothing lies above (equal logits,
+      // all banned), as far as the bound's index.
+      const int end = cta_sums.m == kth_z ? min(v1, max(kth_at - head, 0) / N + 1) : v1;
+#pragma unroll 1
+      for (int w = v0 + tid; w < end; w += TH * UNROLL) {
+#pragma unroll
+        for (int j = 0; j < UNROLL; ++j)
+          if (w + j * TH < end) raw[j] = load_once(zv + (long long)(w + j * TH) * 16);
+#pragma unroll
+        for (int j = 0; j < UNROLL; ++j)
+          if (w + j * TH < end) examine(raw[j], w + j * TH);
+      }
     }
     if (tid < extra0 + extra1) push(extra, extra_at);
     if (tid == 0) sc.counted = 0;
