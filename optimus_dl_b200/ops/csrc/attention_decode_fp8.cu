@@ -235,10 +235,12 @@ __global__ void __launch_bounds__(THREADS, CTAS<HD, NT>) decode_kernel(const __g
   // the segment and position of the first unit: cum[b] * HC <= ua < cum[b + 1] * HC
   int b = 0, hc = 0, un = 0;
   if (count > 0) {
-    int hi = p.B;
-    while (hi - b > 1) {
-      const int mid = (b + hi) >> 1;
-      if ((long long)cum[mid] * HC <= ua) b = mid; else hi = mid;
+    for (int span = p.B; span > 1;) {    // 32 places a round
+      const int step = (span + 31) >> 5, at = lane * step;
+      const bool below = at < span && (long long)cum[b + at] * HC <= ua;
+      const int skip = (__popc(__ballot_sync(0xffffffffu, below)) - 1) * step;
+      b += skip;
+      span = min(step, span - skip);
     }
     const long long rel = ua - (long long)cum[b] * HC;
     const int n = cum[b + 1] - cum[b];
@@ -249,7 +251,7 @@ __global__ void __launch_bounds__(THREADS, CTAS<HD, NT>) decode_kernel(const __g
   if (p.appended) wait_for_launch_before();      // codes and scales of the new token
   for (int done = 0; done < count;) {
     const int n = cum[b + 1] - cum[b], u0 = un, u1 = min(n, un + count - done);
-    const int hk = hc / p.chunks, chunk = hc - hk * p.chunks;
+    const int hk = p.chunks == 1 ? hc : hc / p.chunks, chunk = hc - hk * p.chunks;
     const int len = lens[b], first = first_token(len, p.window), unit0 = first / UNIT;
     const int heads = min(NH, p.rep - chunk * NH), h0 = hk * p.rep + chunk * NH;
 

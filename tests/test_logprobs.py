@@ -290,8 +290,11 @@ def test_extreme_rows(dtype, temperature):
 
 
 @pytest.mark.gpu
-def test_strides_shapes_and_expanded_gradients():
-    base = torch.randn(6, 3, 1031, device="cuda")
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_strides_shapes_and_expanded_gradients(dtype):
+    base = torch.randn(6, 3, 1031, device="cuda").to(dtype)
+    # the statement rounds its gradient to the type as the kernel does, from fp32 values 1e-5 apart at most
+    near = dict(atol=2e-5, rtol=2 * HALF_STEP[dtype])
     t = torch.randint(0, 1000, (6, 3), device="cuda")
     for view in (base[..., 5:1005], base[..., 1:1001], base[::2].repeat_interleave(2, 0)[..., 31:1031],
                  base[:, :1, :1000].expand(6, 3, 1000), base.transpose(0, 1).contiguous().transpose(0, 1)[..., :1000],
@@ -304,7 +307,7 @@ def test_strides_shapes_and_expanded_gradients():
         assert torch.equal(r.top_ids, w.top_ids)
         (r.logp.sum() + 0.5 * r.entropy.mean()).backward()
         (w.logp.sum() + 0.5 * w.entropy.mean()).backward()
-        assert torch.allclose(r.logp, w.logp, atol=2e-5) and torch.allclose(x.grad, v.grad, atol=2e-5)
+        assert torch.allclose(r.logp, w.logp, atol=2e-5) and torch.allclose(x.grad, v.grad, **near)
     only = torch.randn(4, 50, device="cuda", requires_grad=True)
     lp.token_logprobs(only, torch.zeros(4, dtype=torch.int32, device="cuda")).entropy.sum().backward()
     assert torch.isfinite(only.grad).all()
