@@ -42,8 +42,9 @@ namespace decode_fp8 {
 using namespace kvfp8;
 
 constexpr int WARPS = 8;
-// CTAs per SM.  Measured at HD 128, 4 sequences of up to 131072 tokens: 2 x 8 warps 121 us, 1 x 12 129 us, 2 x 6 130 us.
-template <int HD, int NT> constexpr int CTAS = NT == 1 && HD <= 128 ? 2 : 1;
+// CTAs per SM, as many as the registers of a warp's accumulators allow.  Measured at HD 128, 4 sequences of up to 131072
+// tokens: 2 x 8 warps 121 us, 1 x 12 129 us, 2 x 6 130 us; at HD 64, 128 of up to 1024: 3 x 8 36 us, 2 x 8 39 us.
+template <int HD, int NT> constexpr int CTAS = NT > 1 || HD > 128 ? 1 : HD > 64 ? 2 : 3;
 constexpr int THREADS = WARPS * 32;
 constexpr int UNIT = 16;                 // tokens
 constexpr int MAX_BATCH = 2048;          // sequences per launch (their lengths are held in shared memory)
@@ -607,13 +608,13 @@ static int dispatch(const Params& p, int hd, int nt, int grid, cudaStream_t stre
   return launch<256, 1, T>(p, grid, stream);
 }
 
-// CTAs of a launch: two per SM, or one where the accumulators of a warp leave room for no more; fewer when the
-// batch cannot hold that many runs of MIN_UNITS units.
+// CTAs of a launch: as many as fit on the SMs at once (CTAS above), fewer when the batch cannot hold that many runs of
+// MIN_UNITS units.
 constexpr int MIN_UNITS = 8;
 static int grid_size(int B, int Hk, int rep, int hd, int capacity) {
   const int nt = groups(rep, hd), chunks = (rep + 8 * nt - 1) / (8 * nt);
   const long long most = (long long)B * Hk * chunks * ((capacity + UNIT - 1) / UNIT + 1);
-  const long long want = (most + MIN_UNITS - 1) / MIN_UNITS, fit = nt == 1 && hd <= 128 ? 296 : 148;
+  const long long want = (most + MIN_UNITS - 1) / MIN_UNITS, fit = 148 * (nt > 1 || hd > 128 ? 1 : hd > 64 ? 2 : 3);
   return (int)(want < fit ? want : fit);
 }
 
