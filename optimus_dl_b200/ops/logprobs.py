@@ -62,12 +62,6 @@ def _check(rows_shape: torch.Size, vocab: int, floating: torch.Tensor, targets: 
         raise ValueError(f"temperature must be between 1e-6 and 1e6, got {temperature}")
 
 
-def _ordered(z: torch.Tensor) -> torch.Tensor:
-    """Integers in the order of the values: one zero, NaN above everything."""
-    bits = torch.where(torch.isnan(z), 0x7FFFFFFF, (z + 0.0).float().view(torch.int32))
-    return torch.where(bits < 0, bits ^ 0x7FFFFFFF, bits)
-
-
 class _TokenLogprobsRef(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top_k, temperature):
@@ -85,9 +79,8 @@ class _TokenLogprobsRef(torch.autograd.Function):
         logp = torch.where(inside, log_p.gather(-1, at).squeeze(-1), 0.0)
         top_logp = top_ids = None
         if top_k:
-            place = torch.arange(vocab, device=z.device)
-            key = _ordered(z).long() * (1 << 32) + (vocab - 1 - place)
-            top_ids = vocab - 1 - torch.topk(key, top_k, dim=-1).values % (1 << 32)
+            # stable: equal logits stay in the order of their ids; NaN sorts above everything
+            top_ids = torch.sort(z, dim=-1, descending=True, stable=True).indices[..., :top_k].contiguous()
             top_logp = log_p.gather(-1, top_ids)
         ctx.save_for_backward(log_p, entropy, inside & ~none.squeeze(-1), at)
         ctx.dtype, ctx.temperature = logits.dtype, temperature

@@ -133,6 +133,11 @@ def test_nan_and_infinity():
     assert int(r.top_ids[0, 0]) == 4 and int(r.top_ids[1, 0]) == 5
 
 
+def test_statement_orders_doubles_by_all_their_bits():
+    z = torch.ones(1, 5, dtype=torch.float64) + torch.tensor([0.0, 2e-12, 1e-12, 2e-12, -1e-12], dtype=torch.float64)
+    assert lp.token_logprobs(z, torch.tensor([0]), top_k=5).top_ids.tolist() == [[1, 3, 2, 0, 4]]
+
+
 def test_refusals():
     z, t = make(3, 9, torch.float32)
     for kw in (dict(top_k=-1), dict(top_k=10), dict(top_k=33), dict(temperature=0.0), dict(temperature=-1.0),
