@@ -48,9 +48,9 @@ def _strides(t: torch.Tensor) -> tuple[int, ...]:
 
 @dataclass(frozen=True, eq=False)
 class Fp8KVCache:
-    """``k``, ``v``: logical ``[B, capacity, Hk, hd]`` float8_e4m3fn with any strides but a unit one in the last
-    dimension (a head-major allocation viewed this way reads fastest); ``k_scale``, ``v_scale``: fp32
-    ``[B, Hk, ceil(capacity / block)]``, powers of two; ``block``: tokens that share a scale (16, 32, 64 or 128)."""
+    """``k``, ``v``: logical ``[B, capacity, Hk, hd]`` float8_e4m3fn with a unit stride in the last dimension and any
+    others (a head-major allocation viewed this way reads fastest); ``k_scale``, ``v_scale``: fp32
+    ``[B, Hk, ceil(capacity / block)]`` with a unit stride in the blocks, powers of two; ``block``: tokens that share a scale (16, 32, 64 or 128)."""
 
     k: torch.Tensor
     v: torch.Tensor
@@ -67,11 +67,12 @@ class Fp8KVCache:
         if ks.dtype != torch.float32 or vs.dtype != torch.float32:
             raise TypeError(f"scales must be float32, got {ks.dtype} and {vs.dtype}")
         shape, strides, scale_strides = k.shape, _strides(k), _strides(ks)
-        if len(shape) != 4 or shape != v.shape or strides[3] > 1 or (k.stride() != v.stride() and strides != _strides(v)):
+        if (len(shape) != 4 or shape != v.shape or strides[3] != (shape[3] > 1)
+                or (k.stride() != v.stride() and strides != _strides(v))):
             raise ValueError("k and v must be [B, capacity, Hk, hd] of the same shape and strides, contiguous in hd")
         B, capacity, Hk, hd = shape
         want = (B, Hk, -(-capacity // block))
-        if (ks.shape != want or vs.shape != want or scale_strides[2] > 1
+        if (ks.shape != want or vs.shape != want or scale_strides[2] != (want[2] > 1)
                 or (ks.stride() != vs.stride() and scale_strides != _strides(vs))):
             raise ValueError(f"k_scale and v_scale must be {want} of the same strides, contiguous in the blocks")
         dev = k.device
@@ -128,7 +129,7 @@ def _row_strides(t: torch.Tensor) -> tuple[torch.Tensor, tuple[int, ...]]:
     bits, size = t.data_ptr(), t.element_size()
     for s in strides[:-1]:
         bits |= s * size
-    if strides[-1] > 1 or bits & 15:
+    if strides[-1] != 1 or bits & 15:
         t = t.clone(memory_format=torch.contiguous_format)
         strides = _strides(t)
     return t, strides
@@ -141,7 +142,7 @@ def _new_rows(k_new: torch.Tensor, v_new: torch.Tensor) -> tuple[torch.Tensor, t
         bits = k_new.data_ptr() | v_new.data_ptr()
         for s in strides[:-1]:
             bits |= s * size
-        if strides[-1] <= 1 and not bits & 15:
+        if strides[-1] == 1 and not bits & 15:
             return k_new, v_new, strides
     k_new, k_strides = _row_strides(k_new)
     v_new, v_strides = _row_strides(v_new)
