@@ -280,8 +280,12 @@ def linear_token_loss(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tens
     """
     if entropy_weight is not None:
         entropy_weight = entropy_weight.detach().reshape(-1).to(torch.float32).contiguous()
-        if entropy_weight.shape[0] != targets.numel():
-            raise ValueError(f"entropy_weight has {entropy_weight.shape[0]} numbers for {targets.numel()} tokens")
+        if entropy_weight.shape[0] != targets.numel() or x[..., 0].numel() != targets.numel():
+            raise ValueError(f"entropy_weight has {entropy_weight.shape[0]} numbers for {targets.numel()} tokens and "
+                             f"{x[..., 0].numel()} rows")
+        if any(t.device != x.device for t in (weight, targets, entropy_weight)):
+            raise ValueError(f"weight ({weight.device}), targets ({targets.device}) and entropy_weight "
+                             f"({entropy_weight.device}) must be where x is ({x.device})")
     if x.is_cuda and x.dtype == torch.bfloat16 and weight.dtype == torch.bfloat16 and x.shape[-1] % 8 == 0:
         return _LinearTokenLoss.apply(x, weight, targets, loss_fn, chunk_rows, entropy_weight)
     logits = F.linear(x.reshape(-1, x.shape[-1]), weight).float()
