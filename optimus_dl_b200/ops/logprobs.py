@@ -22,6 +22,7 @@ Rules, the same on every path:
 
 from __future__ import annotations
 
+import contextlib
 import math
 from dataclasses import dataclass
 
@@ -215,11 +216,21 @@ def linear_token_logprobs(x: torch.Tensor, weight: torch.Tensor, targets: torch.
     Rows are taken ``chunk_rows`` at a time, so no more than a chunk of logits is held.
     """
     top_k, temperature = int(top_k), float(temperature)
+    if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
+        raise ValueError(f"a weight of {tuple(weight.shape)} does not fit rows of {tuple(x.shape)}")
+    if weight.device != x.device:
+        raise ValueError(f"weight is on {weight.device}, the rows on {x.device}")
     vocab = weight.shape[0]
     _check(x.shape[:-1], vocab, x, targets, top_k, temperature)
     if chunk_rows < 1:
         raise ValueError(f"chunk_rows must be positive, got {chunk_rows}")
-    shape, d = targets.shape, x.shape[-1]
+    with _lib.on_device(x.device) if x.is_cuda else contextlib.nullcontext():
+        return _linear_token_logprobs(x, weight, targets, top_k, temperature, chunk_rows)
+
+
+def _linear_token_logprobs(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, top_k: int, temperature: float,
+                           chunk_rows: int) -> TokenLogprobs:
+    shape, d, vocab = targets.shape, x.shape[-1], weight.shape[0]
     x2, tg = x.reshape(-1, d), targets.reshape(-1)
     kernel = x.is_cuda and x.dtype == torch.bfloat16 and weight.dtype == torch.bfloat16 and d % 8 == 0
     if kernel:
