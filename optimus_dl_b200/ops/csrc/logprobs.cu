@@ -362,8 +362,8 @@ __global__ void __launch_bounds__(TH, 1024 / TH) forward_kernel(const __grid_con
   if (tid < extra0 + extra1) {
     extra = Vec<T>::load(z + extra_at);
     // 2^u with the u that r = m c rounded leaves; NaN and +inf are found by the maximum
-    const float u = fabsf(extra) < HUGE_LOGIT ? fmaf(extra, c, -__fmul_rn(extra, c)) : 0.f;
-    if (extra != -INFINITY) join(st, Sums{extra, exp2_fast(u), u}, c);
+    const float u = fabsf(extra) < HUGE_LOGIT ? fmaf(extra, c, -__fmul_rn(extra, c)) : 0.f, x = exp2_fast(u);
+    if (extra != -INFINITY) join(st, Sums{extra, x, u * x}, c);
   }
 
   // one triple per CTA

@@ -59,3 +59,20 @@ def test_the_head_projection_runs_on_the_rows_own_device(monkeypatch):
         x, w = (torch.empty(n, 16, dtype=torch.bfloat16, device=there) for n in (6, 9))
         r = lp.linear_token_logprobs(x, w, torch.zeros(6, dtype=torch.int64, device=there), chunk_rows=4)
     assert r.logp.shape == (6,) and inside == [[there], [there]]
+
+
+# ------------------------------------------------------------------------------------------------ ends of rows, GPU
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("size,temperature", [(30.0, 1e-6), (7e5, 1.0), (60000.0, 0.1), (50.0, 7e-5)])
+def test_a_maximum_at_either_end_of_a_row(dtype, size, temperature):
+    """Alone with the distribution: its entropy is 0 wherever it stands, to what the logarithm and the reference's own
+    rounding leave, 2^-20 of the exponent's residue (at most 2) and of 1."""
+    if size > torch.finfo(dtype).max:
+        pytest.skip("not a number of this type")
+    for vocab in (1025, 1027, 4099, 20003):
+        z = torch.zeros(24, vocab)
+        for i in range(24):
+            z[i, [0, 1, 2, 3, 6, 7, vocab // 2, vocab - 8, vocab - 7, vocab - 3, vocab - 2, vocab - 1][i % 12]] = size + i
+        r = lp.token_logprobs(z.to(dtype).cuda(), z.argmax(-1).cuda(), temperature=temperature)
+        assert float(r.entropy.abs().max()) <= 5e-5 and float(r.logp.abs().max()) <= 5e-5
