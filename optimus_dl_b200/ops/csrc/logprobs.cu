@@ -13,11 +13,12 @@
 // loop is written for few instructions: packed fp32 pairs, 16-bit pair maxima, one fused operation per exponent.
 //
 // Where nothing may go wrong: a banned token (-inf) has to add 0 to W, not 0 * inf, so bf16 logits are raised to -1e30
-// (a pair at a time) and the exponents of the other types to -200; 2^x is 0 there.  A maximum of 1e29 and more in
-// magnitude (a row of the type's lowest value) would overflow r; distinct fp32 numbers of that size differ by far more
-// than 200 T, so only the equals of the maximum count then.  The running maximum propagates NaN, and +inf is found at
-// the end, so such rows give NaN as the formulas do.  A row without any logit above -inf has log probabilities of -inf,
-// entropy 0 and no gradient.
+// (a pair at a time) and the exponents of the other types to -200; 2^x is 0 there.  What r lost, up to half a unit in
+// its last place, is the exponent of the maximum itself: at most 2^-4 while |r| is below 2^20, but 128, which 2^x does
+// not hold, at 2^32 (a row masked with -1e10).  So from 2^20 on, where no ordinary row comes, the exponents are (z - m) c
+// and the sums are against m itself: one instruction more per logit.  The running maximum propagates NaN, and +inf is
+// found at the end, so such rows give NaN as the formulas do.  A row without any logit above -inf has log probabilities
+// of -inf, entropy 0 and no gradient.
 //
 // Alternatives: the k largest logits, equal ones by lowest index.  A candidate is one 64-bit number, the logit's
 // order-preserving key above the complement of its index, so "better" is one integer comparison without ties.  The
@@ -44,7 +45,7 @@ constexpr int MAX_CLUSTER = 8;
 constexpr int LOOKS = 512;      // notes that the CTA looks behind together
 constexpr int NOTES = 16;        // maxima a thread notes: one for each batch, or for 2, 4, 8... of longer slices
 constexpr float FLOOR = -200.0f;       // of an exponent: 2^x is 0 in fp32
-constexpr float HUGE_LOGIT = 1e29f;    // from here on a maximum is treated apart
+constexpr float FAR = 1048576.f;       // 2^20: a maximum with an r of this magnitude or more is treated apart
 
 using u64 = unsigned long long;
 
@@ -166,10 +167,21 @@ __device__ __forceinline__ float candidate_value(u64 c) {
 }
 __device__ __forceinline__ int candidate_index(u64 c) { return (int)~(uint32_t)c; }
 
-struct Sums { float m, s, w; };        // s and w against r = m c
+struct Sums { float m, s, w; };        // s and w against r = m c, from FAR on against m itself
+// The exponent of the maximum itself: what r = m c rounded leaves of it.
+__device__ __forceinline__ float residue(float m, float c) {
+  const float r = __fmul_rn(m, c);
+  return fabsf(r) < FAR ? fmaf(m, c, -r) : 0.f;
+}
+// log2 of the factor that takes sums of a maximum `a` to a larger one, `m`; ra and r are their references.
+__device__ __forceinline__ float shift(float a, float ra, float m, float r, float c) {
+  if (a == m) return 0.f;
+  const float d = fmaxf(fabsf(r), fabsf(ra)) < FAR ? ra - r : (a - m) * c - residue(a, c) + residue(m, c);
+  return fmaxf(d, FLOOR);
+}
 __device__ __forceinline__ void join(Sums& a, const Sums& b, float c) {
   const float m = max_nan(a.m, b.m), r = __fmul_rn(m, c);
-  const float da = a.m == m ? 0.f : fmaxf(__fmul_rn(a.m, c) - r, FLOOR), db = b.m == m ? 0.f : fmaxf(__fmul_rn(b.m, c) - r, FLOOR);
+  const float da = shift(a.m, __fmul_rn(a.m, c), m, r, c), db = shift(b.m, __fmul_rn(b.m, c), m, r, c);
   const float fa = exp2_fast(da), fb = exp2_fast(db);
   a.w = fa * (a.w + da * a.s) + fb * (b.w + db * b.s);
   a.s = fa * a.s + fb * b.s;
@@ -316,12 +328,12 @@ __global__ void __launch_bounds__(TH, 1024 / TH) forward_kernel(const __grid_con
       note = (batch & ((1 << group) - 1)) ? max_nan(note, mx) : mx;
     }
     mx = max_nan(mx, m);
-    const float now = __fmul_rn(mx, c), d = mx == m ? 0.f : fmaxf(r - now, FLOOR), f = exp2_fast(d);
+    const float now = __fmul_rn(mx, c), d = shift(m, r, mx, now, c), f = exp2_fast(d);
     w2 = fmul2(ffma2(make_float2(d, d), s2, w2), make_float2(f, f));
     s2 = fmul2(s2, make_float2(f, f));
     m = mx;
     r = now;
-    if (fabsf(m) < HUGE_LOGIT) {
+    if (fabsf(r) < FAR) {
       const float2 neg = make_float2(-r, -r);
 #pragma unroll
       for (int j = 0; j < UNROLL; ++j) {
@@ -341,7 +353,11 @@ __global__ void __launch_bounds__(TH, 1024 / TH) forward_kernel(const __grid_con
       for (int j = 0; j < UNROLL; ++j) {
         float z8[N];
         Vec<T>::unpack(raw[j], z8);
-        for (int e = 0; e < N; ++e) s2.x += z8[e] == m ? 1.f : 0.f;
+        for (int e = 0; e < N; ++e) {
+          const float u = fmaxf((z8[e] - m) * c, FLOOR), x = exp2_fast(u);
+          s2.x += x;
+          w2.x = fmaf(u, x, w2.x);
+        }
       }
     }
   };
@@ -361,8 +377,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) forward_kernel(const __grid_con
   float extra = -INFINITY;
   if (tid < extra0 + extra1) {
     extra = Vec<T>::load(z + extra_at);
-    // 2^u with the u that r = m c rounded leaves; NaN and +inf are found by the maximum
-    const float u = fabsf(extra) < HUGE_LOGIT ? fmaf(extra, c, -__fmul_rn(extra, c)) : 0.f, x = exp2_fast(u);
+    const float u = residue(extra, c), x = exp2_fast(u);       // NaN and +inf are found by the maximum
     if (extra != -INFINITY) join(st, Sums{extra, x, u * x}, c);
   }
 
@@ -521,7 +536,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) forward_kernel(const __grid_con
   const float sum_log2 = broken ? NAN : none ? 0.f : log2f(total.s);
   const float top_z = none ? 0.f : total.m;
   // against the maximum itself from here on
-  const float log2s = fabsf(top_z) < HUGE_LOGIT ? sum_log2 - fmaf(top_z, c, -__fmul_rn(top_z, c)) : sum_log2;
+  const float log2s = sum_log2 - residue(top_z, c);
   if (tid == 0) {
     p.logp[row] = inside ? log_of(z_t, top_z, c, log2s) : 0.f;
     const float h = none ? 0.f : (sum_log2 - total.w / total.s) * 0.6931471805599453f;
@@ -590,8 +605,8 @@ backward_kernel(const T* logits, long long ld, const long long* __restrict__ tar
   // p (log p + H) = p (v ln 2 + H) with v = log2 p: dz = -(p / T) (a + b v), a = g_l + g_H H, b = g_H ln 2
   const float a = none ? 0.f : -inv_t * (gl + gh * entropy[row]), b = none ? 0.f : -inv_t * gh * 0.6931471805599453f;
   const float at_token = gl * inv_t;
-  const bool apart = !(fabsf(m) < HUGE_LOGIT);       // also NaN and infinities, whose log2 S is NaN
-  const float r = __fmul_rn(m, c), log2s = st.y + fmaf(m, c, -r);      // log2 S against r
+  const float r = __fmul_rn(m, c), log2s = st.y + residue(m, c);       // log2 S against r
+  const bool apart = !(fabsf(r) < FAR);              // also NaN and infinities, whose log2 S is NaN
   auto grad = [&](float f) {                         // of one element, whatever the maximum
     const float v = max_nan((f - m) * c - st.y, FLOOR);
     return exp2_fast(v) * fmaf(b, v, a);

@@ -1,11 +1,78 @@
 """Token log probabilities at their edges: where tensors lie, magnitudes of logits, the ends of rows, ties, and the forms
-over a head projection."""
+over a head projection.
+
+Tolerances, with u = (z - max z) / T in 64 bits and S = sum e^u. An exponent carries one rounding of c = log2 e / T, one of
+the difference and one of the product in fp32, and the logarithm of one element the same again: 6 * 2^-24 |u| < 4e-7 |u|.
+A reference's residue (at most 2^-4) cancels but for its own rounding. 2^x and log2 x are off by 2^-22 relative and
+2^-21 absolute; a thread's sum of n terms of one sign by (n / 2) 2^-24 at most (it is two sums), n <= 2^9 for the rows
+here, and joining 2^8 of them by 2^4 steps: together below 5e-5 of S and of sum u e^u. So
+    |error of log p_j| <= 4e-7 |u_j| + 5e-5        |error of H| <= 5e-5 (1 + H) + 4e-7 (H + 1)
+as sum p |u| <= H. An element of the gradient, -p_j (g_l + g_H (log p_j + H)) / T with g_l / T more at the token, is off by
+p_j times the errors of log p_j and H times what p_j is multiplied with, and by half a step of its type. Exponentials below
+2^-126 are flushed to 0, so p_j itself may be off by that much.
+"""
+
+import math
 
 import pytest
 import torch
 
 from optimus_dl_b200.ops import logprobs as lp
 from optimus_dl_b200.ops.cross_entropy import linear_token_loss
+
+LARGEST = 2.3e38          # of a log probability: times log2 e it is still an fp32 number
+HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+
+
+def definition(z, t, temperature, d_logp, d_h):
+    z, d_logp, d_h = z.detach().double().cpu(), d_logp.double().cpu()[:, None], d_h.double().cpu()[:, None]
+    t = t.cpu()[:, None]
+    top = z.amax(-1, keepdim=True)
+    none = top == -math.inf
+    u = (z - torch.where(none, 0.0, top)) / temperature
+    log_s = torch.log(torch.where(none, 1.0, torch.exp(u).sum(-1, keepdim=True)))
+    log_p = u - log_s
+    p = torch.exp(log_p)
+    h = -torch.where(p == 0, 0.0, p * log_p).sum(-1, keepdim=True)
+    inside = (t >= 0) & (t < z.shape[-1])
+    at = t.clamp(0, z.shape[-1] - 1)
+    logp = torch.where(inside, log_p.gather(-1, at), 0.0)
+    a = torch.where(inside & ~none, d_logp, 0.0)
+    times = a.abs() + d_h.abs() * (torch.where(p == 0, 0.0, log_p).abs() + h + 1)
+    g = -p * a - d_h * torch.where(p == 0, 0.0, p * (log_p + h))
+    g = g.scatter_add(-1, at, a)
+    off = 4e-7 * torch.where(u == -math.inf, 0.0, u).abs() + 5e-5
+    # 2^x is 0 below 2^-126: such a p_j is off by all of itself
+    slack = (p * (off + 6e-5 * (1 + h)) + torch.finfo(torch.float32).tiny) * times / temperature
+    return dict(logp=logp[:, 0], h=h[:, 0], grad=g / temperature, slack=slack, u=torch.where(inside, u.gather(-1, at), 0.0)[:, 0],
+                log_p=log_p)
+
+
+def check(z, t, temperature, d_logp=None, d_h=None, top_k=0):
+    """The kernels' results on the GPU against the definition; returns them."""
+    rows = z.shape[0]
+    g = torch.Generator().manual_seed(rows)
+    d_logp = torch.randn(rows, generator=g) if d_logp is None else d_logp
+    d_h = torch.randn(rows, generator=g) if d_h is None else d_h
+    want = definition(z, t, temperature, d_logp, d_h)
+    x = z.cuda().requires_grad_(True)
+    r = lp.token_logprobs(x, t.cuda(), top_k=top_k, temperature=temperature)
+    logp, h = r.logp.detach().double().cpu(), r.entropy.detach().double().cpu()
+    fin, none = want["logp"].abs() <= LARGEST, want["logp"] == -math.inf
+    assert torch.equal(logp[none], want["logp"][none])
+    err = ((logp - want["logp"]).abs() / (4e-7 * want["u"].abs() + 5e-5))[fin]
+    assert not err.numel() or float(err.max()) <= 1, (err.argmax(), err.max())
+    err = (h - want["h"]).abs() / (5.1e-5 * (1 + want["h"]))
+    assert float(err.max()) <= 1, (err.argmax(), err.max())
+    grad, = torch.autograd.grad([r.logp, r.entropy], [x], [d_logp.cuda(), d_h.cuda()])
+    tol = want["slack"] + (1.01 * HALF_STEP[z.dtype] + 3 * 2.0 ** -24) * want["grad"].abs() + torch.finfo(z.dtype).tiny
+    fits = want["grad"].abs() <= torch.finfo(z.dtype).max
+    err = ((grad.double().cpu() - want["grad"]).abs() / tol)[fits]
+    assert bool((err <= 1).all()), (err.argmax(), err.max())
+    if top_k:
+        order = torch.sort(z.double(), dim=-1, descending=True, stable=True).indices[:, :top_k]
+        assert torch.equal(r.top_ids.cpu(), order)
+    return r, grad
 
 
 # ------------------------------------------------------------------------------------------------ where tensors lie
@@ -76,3 +143,54 @@ def test_a_maximum_at_either_end_of_a_row(dtype, size, temperature):
             z[i, [0, 1, 2, 3, 6, 7, vocab // 2, vocab - 8, vocab - 7, vocab - 3, vocab - 2, vocab - 1][i % 12]] = size + i
         r = lp.token_logprobs(z.to(dtype).cuda(), z.argmax(-1).cuda(), temperature=temperature)
         assert float(r.entropy.abs().max()) <= 5e-5 and float(r.logp.abs().max()) <= 5e-5
+
+
+# ------------------------------------------------------------------------------------------------ magnitudes, GPU
+def masked_rows(dtype, vocab, temperature, fills):
+    """Ordinary logits with a fill in the whole row, in a stretch of it, in the first or the last token, in every other
+    token, beside its neighbour; and rows whose m c lies about the places where exponents are taken differently."""
+    g = torch.Generator().manual_seed(vocab)
+    rows = []
+    for fill in fills:
+        fill = torch.tensor(fill, dtype=torch.float64).to(dtype)
+        if not torch.isfinite(fill):
+            continue
+        base = (torch.randn(6, vocab, generator=g) * 3).to(dtype)
+        base[0] = fill
+        base[1, vocab // 5:vocab // 5 + 16384] = fill
+        base[2, 0] = fill
+        base[3, -1] = fill
+        base[4, ::2] = fill
+        base[5] = fill
+        base[5, 1::3] = torch.nextafter(fill.float(), torch.tensor(math.inf)).to(dtype) if dtype != torch.bfloat16 else \
+            (fill.view(torch.int16) + 1).view(dtype)
+        rows.append(base)
+    for far in (2.0 ** 20, 2.0 ** 24, 2.0 ** 30, 2.0 ** 32):
+        for sign in (1, -1):
+            at = sign * far * temperature * math.log(2)
+            if abs(at) < torch.finfo(dtype).max:
+                rows.append((torch.randn(2, vocab, generator=g) * 3 * max(1.0, abs(at) * 2.0 ** -22) + at).to(dtype))
+    return torch.cat(rows)
+
+
+FILLS = [s * f for f in (1e5, 1e9, 3e9, 1e10, 1e12, 1e20, 1e25, 3e38) for s in (-1, 1)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("temperature", [1.0, 0.5, 0.1, 1e-3, 1e-6, 1e6])
+@pytest.mark.parametrize("vocab", [1025, 33001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_logits_of_any_finite_magnitude(dtype, vocab, temperature):
+    fills = [s * f for f in (1000.0, 30000.0, 65504.0) for s in (-1, 1)] if dtype == torch.float16 else FILLS
+    z = masked_rows(dtype, vocab, temperature, fills)
+    t = torch.randint(0, vocab, (z.shape[0],), generator=torch.Generator().manual_seed(1))
+    t[::7] = vocab - 1
+    r, _ = check(z, t, temperature, top_k=3)
+    few = lp.token_logprobs(z[:2].cuda(), t[:2].cuda(), temperature=temperature)             # a cluster a row
+    many = lp.token_logprobs(z.repeat(12, 1).cuda(), t.repeat(12).cuda(), temperature=temperature)     # narrow CTAs
+    for part in (few, lp.TokenLogprobs(many.logp[-z.shape[0]:], many.entropy[-z.shape[0]:], None, None)):
+        n = part.logp.shape[0]
+        want = definition(z[:n], t[:n], temperature, torch.zeros(n), torch.zeros(n))
+        fin = want["logp"].abs() <= LARGEST
+        assert bool(((part.logp.double().cpu() - want["logp"]).abs() <= 4e-7 * want["u"].abs() + 5e-5)[fin].all())
+        assert bool(((part.entropy.double().cpu() - want["h"]).abs() <= 5.1e-5 * (1 + want["h"])).all())
