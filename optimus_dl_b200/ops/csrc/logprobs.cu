@@ -195,11 +195,12 @@ struct Params {
   float2* stats; float* kept;                     // for the gradient: (max, log2 S) and the entropy once more
   float* top_logp; long long* top_ids;
   int rows, V, k, cluster;
-  float c;
+  float c, inv_t;
 };
 
-__device__ __forceinline__ float log_of(float z, float m, float c, float log2s) {
-  return ((z - m) * c - log2s) * 0.6931471805599453f;
+// Not in base 2: log2 e times the type's lowest value is no fp32 number.
+__device__ __forceinline__ float log_of(float z, float m, float inv_t, float log2s) {
+  return (z - m) * inv_t - log2s * 0.6931471805599453f;
 }
 
 // Of a CTA that looks for alternatives.  Kept to some 28 KB: four CTAs of 54 KB left the SM so little of its L1 cache for
@@ -538,7 +539,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) forward_kernel(const __grid_con
   // against the maximum itself from here on
   const float log2s = sum_log2 - residue(top_z, c);
   if (tid == 0) {
-    p.logp[row] = inside ? log_of(z_t, top_z, c, log2s) : 0.f;
+    p.logp[row] = inside ? log_of(z_t, top_z, p.inv_t, log2s) : 0.f;
     const float h = none ? 0.f : (sum_log2 - total.w / total.s) * 0.6931471805599453f;
     p.entropy[row] = h;
     if (p.stats) {
@@ -548,7 +549,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) forward_kernel(const __grid_con
   }
   if (TOPK && tid < p.k) {
     const u64 cand = p.cluster > 1 ? sc.merged[tid] : sc.top[tid];
-    p.top_logp[(long long)row * p.k + tid] = log_of(candidate_value(cand), top_z, c, log2s);
+    p.top_logp[(long long)row * p.k + tid] = log_of(candidate_value(cand), top_z, p.inv_t, log2s);
     p.top_ids[(long long)row * p.k + tid] = candidate_index(cand);
   }
 }
@@ -745,7 +746,7 @@ extern "C" int ob_logprobs_fwd(const void* packed) {
   const int cl = pick_cluster(rows, V, dtype == 2 ? 4 : 8);
   if ((long long)rows * cl > 0x7fffffffLL) return -1;
   const Params p{a.logits, a.ld, a.targets, a.logp, a.entropy, a.stats, a.kept, a.top_logp, a.top_ids, rows, V, top_k, cl,
-                 (float)(1.4426950408889634 / temperature)};
+                 (float)(1.4426950408889634 / temperature), (float)(1.0 / temperature)};
   if (dtype == 0) return run_forward<__nv_bfloat16>(p, stream);
   if (dtype == 1) return run_forward<__half>(p, stream);
   if (dtype == 2) return run_forward<float>(p, stream);

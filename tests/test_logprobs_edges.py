@@ -20,7 +20,7 @@ import torch
 from optimus_dl_b200.ops import logprobs as lp
 from optimus_dl_b200.ops.cross_entropy import linear_token_loss
 
-LARGEST = 2.3e38          # of a log probability: times log2 e it is still an fp32 number
+LARGEST = torch.finfo(torch.float32).max        # of a log probability; beyond, it is -inf
 HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
 
 
@@ -58,8 +58,8 @@ def check(z, t, temperature, d_logp=None, d_h=None, top_k=0):
     x = z.cuda().requires_grad_(True)
     r = lp.token_logprobs(x, t.cuda(), top_k=top_k, temperature=temperature)
     logp, h = r.logp.detach().double().cpu(), r.entropy.detach().double().cpu()
-    fin, none = want["logp"].abs() <= LARGEST, want["logp"] == -math.inf
-    assert torch.equal(logp[none], want["logp"][none])
+    fin = want["logp"].abs() <= LARGEST
+    assert bool((logp[~fin] == -math.inf).all())
     err = ((logp - want["logp"]).abs() / (4e-7 * want["u"].abs() + 5e-5))[fin]
     assert not err.numel() or float(err.max()) <= 1, (err.argmax(), err.max())
     err = (h - want["h"]).abs() / (5.1e-5 * (1 + want["h"]))
@@ -194,3 +194,17 @@ def test_logits_of_any_finite_magnitude(dtype, vocab, temperature):
         fin = want["logp"].abs() <= LARGEST
         assert bool(((part.logp.double().cpu() - want["logp"]).abs() <= 4e-7 * want["u"].abs() + 5e-5)[fin].all())
         assert bool(((part.entropy.double().cpu() - want["h"]).abs() <= 5.1e-5 * (1 + want["h"])).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_tokens_of_the_lowest_value_keep_their_log_probability(dtype):
+    """It is that value itself here, less 0.7 to 6.2: within a rounding of each of two terms."""
+    low = torch.finfo(dtype).min
+    z = torch.full((3, 501), low, dtype=dtype)
+    z[:, :2], z[1, 2:] = 0.0, 0.0
+    z[1, 500] = low
+    r = lp.token_logprobs(z.cuda(), torch.tensor([500, 500, 2]).cuda(), top_k=4)
+    assert bool(((r.logp.double().cpu() - low).abs() <= 2.0 ** -23 * abs(low)).all())
+    for got, want in ((r.top_logp[0, 2:], low), (r.top_logp[2, 3:], low), (r.top_logp[1], -math.log(500))):
+        assert bool(((got.double().cpu() - want).abs() <= 2.0 ** -23 * abs(want) + 5e-5).all())
