@@ -71,7 +71,8 @@ template <> struct Vec<float> {
   static constexpr int N = 4;
   static constexpr uint32_t NONE = 0xff800000u;      // 32 bits of -inf
   static constexpr bool LIFTED = false;              // exponents have to be kept above FLOOR one by one
-  __device__ static uint4 lift(const uint4& u) { return u; }
+  __device__ static uint4 lift(const uint4& u, uint32_t = 0) { return u; }
+  __device__ static uint32_t below(float) { return 0; }
   __device__ static void unpack(const uint4& u, float (&f)[N]) {
     f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
   }
@@ -90,13 +91,17 @@ template <> struct Vec<__nv_bfloat16> {
   static constexpr int N = 8;
   static constexpr uint32_t NONE = 0xff80ff80u;
   static constexpr bool LIFTED = true;
-  __device__ static uint4 lift(const uint4& u) {         // at least -1e30
-    return make_uint4(lift2(u.x), lift2(u.y), lift2(u.z), lift2(u.w));
+  __device__ static uint4 lift(const uint4& u, uint32_t low = 0xf14af14au) {         // at least -1e30, or `low` (a pair)
+    return make_uint4(lift2(u.x, low), lift2(u.y, low), lift2(u.z, low), lift2(u.w, low));
   }
-  __device__ static uint32_t lift2(uint32_t a) {
+  __device__ static uint32_t lift2(uint32_t a, uint32_t low) {
     uint32_t r;
-    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(0xf14af14au));
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(low));
     return r;
+  }
+  __device__ static uint32_t below(float f) {            // a pair of f rounded down
+    const uint32_t b = __bfloat16_as_ushort(__float2bfloat16_rd(f));
+    return b << 16 | b;
   }
   __device__ static void unpack(const uint4& u, float (&f)[N]) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -122,7 +127,8 @@ template <> struct Vec<__half> {
   static constexpr int N = 8;
   static constexpr uint32_t NONE = 0xfc00fc00u;
   static constexpr bool LIFTED = false;
-  __device__ static uint4 lift(const uint4& u) { return u; }
+  __device__ static uint4 lift(const uint4& u, uint32_t = 0) { return u; }
+  __device__ static uint32_t below(float) { return 0; }
   __device__ static void unpack(const uint4& u, float (&f)[N]) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -605,15 +611,25 @@ backward_kernel(const T* logits, long long ld, const long long* __restrict__ tar
   const float gl = inside && d_logp ? d_logp[row] : 0.f, gh = d_entropy ? d_entropy[row] : 0.f;
   // p (log p + H) = p (v ln 2 + H) with v = log2 p: dz = -(p / T) (a + b v), a = g_l + g_H H, b = g_H ln 2
   const float a = none ? 0.f : -inv_t * (gl + gh * entropy[row]), b = none ? 0.f : -inv_t * gh * 0.6931471805599453f;
-  const float at_token = gl * inv_t;
   const float r = __fmul_rn(m, c), log2s = st.y + residue(m, c);       // log2 S against r
   const bool apart = !(fabsf(r) < FAR);              // also NaN and infinities, whose log2 S is NaN
+  // what the loop below seldom needs is read again: kept, it costs registers that the loop lacks
+  auto at_token = [&] {
+    float g = 0.f;
+    if (d_logp) asm volatile("ld.global.f32 %0, [%1];" : "=f"(g) : "l"(d_logp + row));
+    return g * inv_t;
+  };
   auto grad = [&](float f) {                         // of one element, whatever the maximum
-    const float v = max_nan((f - m) * c - st.y, FLOOR);
+    float2 s;
+    asm volatile("ld.global.v2.f32 {%0, %1}, [%2];" : "=f"(s.x), "=f"(s.y) : "l"(stats + row));
+    const float v = max_nan((f - (s.x == -INFINITY ? 0.f : s.x)) * c - s.y, FLOOR);
     return exp2_fast(v) * fmaf(b, v, a);
   };
   const float2 cc = make_float2(c, c), neg_r = make_float2(-r, -r), neg_s = make_float2(-log2s, -log2s);
   const float2 aa = make_float2(a, a), bb = make_float2(b, b);
+  // bf16: p is 0 300 below the maximum in the exponent, and b v stays a number there whatever g_H and T are (raised to
+  // -1e30 as in the forward pass, a banned token had 0 * inf from |g_H| / T^2 of 3e8 on)
+  const uint32_t low = Vec<T>::below(m - 300.f / c);
   auto put = [&](int base, const uint4 (&raw)[UNROLL]) {
     const bool full = base + STEP <= v1;
 #pragma unroll
@@ -622,7 +638,7 @@ backward_kernel(const T* logits, long long ld, const long long* __restrict__ tar
       if (full || i < v1) {
         float f[N];
         if (!apart) {
-          Vec<T>::unpack(Vec<T>::lift(raw[j]), f);
+          Vec<T>::unpack(Vec<T>::lift(raw[j], low), f);
 #pragma unroll
           for (int e = 0; e < N; e += 2) {
             float2 v = fadd2(ffma2(make_float2(f[e], f[e + 1]), cc, neg_r), neg_s);
@@ -644,7 +660,7 @@ backward_kernel(const T* logits, long long ld, const long long* __restrict__ tar
         const unsigned off = (unsigned)(t - (head + i * N));       // t = -1 is never below N
         if (off < N)
 #pragma unroll
-          for (int e = 0; e < N; ++e) if (e == off) f[e] += at_token;
+          for (int e = 0; e < N; ++e) if (e == off) f[e] += at_token();
         *reinterpret_cast<uint4*>(to + j * THREADS * N) = Vec<T>::pack(f);
       }
     }
@@ -660,7 +676,7 @@ backward_kernel(const T* logits, long long ld, const long long* __restrict__ tar
   const int tail = V - head - nv * N;
   if (piece == 0 && tid < head + tail) {
     const int idx = tid < head ? tid : nv * N + tid;
-    g[idx] = Vec<T>::cast(grad(Vec<T>::load(z + idx)) + (idx == t ? at_token : 0.f));
+    g[idx] = Vec<T>::cast(grad(Vec<T>::load(z + idx)) + (idx == t ? at_token() : 0.f));
   }
 }
 

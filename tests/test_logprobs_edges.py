@@ -67,6 +67,7 @@ def check(z, t, temperature, d_logp=None, d_h=None, top_k=0):
     grad, = torch.autograd.grad([r.logp, r.entropy], [x], [d_logp.cuda(), d_h.cuda()])
     tol = want["slack"] + (1.01 * HALF_STEP[z.dtype] + 3 * 2.0 ** -24) * want["grad"].abs() + torch.finfo(z.dtype).tiny
     fits = want["grad"].abs() <= torch.finfo(z.dtype).max
+    assert not torch.isnan(grad).any()
     err = ((grad.double().cpu() - want["grad"]).abs() / tol)[fits]
     assert bool((err <= 1).all()), (err.argmax(), err.max())
     if top_k:
@@ -208,3 +209,21 @@ def test_tokens_of_the_lowest_value_keep_their_log_probability(dtype):
     assert bool(((r.logp.double().cpu() - low).abs() <= 2.0 ** -23 * abs(low)).all())
     for got, want in ((r.top_logp[0, 2:], low), (r.top_logp[2, 3:], low), (r.top_logp[1], -math.log(500))):
         assert bool(((got.double().cpu() - want).abs() <= 2.0 ** -23 * abs(want) + 5e-5).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("temperature,g_h", [(1.0, 1e9), (1e-2, 1e5), (1e-4, 1e5), (1e-6, 1.0), (1e-6, 1e5), (1e6, 1e9)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_gradients_of_banned_tokens_under_large_weights(dtype, temperature, g_h):
+    """0 at a banned token, whatever the entropy's weight (a loss scale) and the temperature."""
+    g = torch.Generator().manual_seed(3)
+    z = (torch.randn(8, 4099, generator=g) * 3).to(dtype)
+    z[:, torch.rand(4099, generator=g) < 0.3] = -math.inf
+    z[1] = -math.inf
+    z[2, :4000] = torch.finfo(dtype).min
+    z[3, :2000] = -30000.0
+    t = torch.randint(0, 4099, (8,), generator=g)
+    d_logp, d_h = torch.randn(8, generator=g), torch.randn(8, generator=g) * g_h
+    _, grad = check(z, t, temperature, d_logp, d_h)
+    banned = (z == -math.inf) & (torch.arange(4099) != t[:, None])
+    assert not grad.cpu()[banned].any()
