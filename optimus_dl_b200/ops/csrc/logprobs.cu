@@ -14,11 +14,13 @@
 //
 // Where nothing may go wrong: a banned token (-inf) has to add 0 to W, not 0 * inf, so bf16 logits are raised to -1e30
 // (a pair at a time) and the exponents of the other types to -200; 2^x is 0 there.  What r lost, up to half a unit in
-// its last place, is the exponent of the maximum itself: at most 2^-4 while |r| is below 2^20, but 128, which 2^x does
+// its last place, is the exponent of the maximum itself: at most 2^-5 while |r| is below 2^20, but 128, which 2^x does
 // not hold, at 2^32 (a row masked with -1e10).  So from 2^20 on, where no ordinary row comes, the exponents are (z - m) c
-// and the sums are against m itself: one instruction more per logit.  The running maximum propagates NaN, and +inf is
-// found at the end, so such rows give NaN as the formulas do.  A row without any logit above -inf has log probabilities
-// of -inf, entropy 0 and no gradient.
+// with that residue added, and from 2^24 on without it: the sums are against m itself then.  References of both sides of
+// 2^20 are therefore of one kind, and a sum from beyond 2^24 is nothing beside one from below 2^20, so where the larger
+// maximum's r is below 2^20 the shift between two sums is r_a - r.  The running maximum propagates NaN, and +inf is found
+// at the end, so such rows give NaN as the formulas do.  A row without any logit above -inf has log probabilities of
+// -inf, entropy 0 and no gradient.
 //
 // Alternatives: the k largest logits, equal ones by lowest index.  A candidate is one 64-bit number, the logit's
 // order-preserving key above the complement of its index, so "better" is one integer comparison without ties.  The
@@ -46,6 +48,7 @@ constexpr int LOOKS = 512;      // notes that the CTA looks behind together
 constexpr int NOTES = 16;        // maxima a thread notes: one for each batch, or for 2, 4, 8... of longer slices
 constexpr float FLOOR = -200.0f;       // of an exponent: 2^x is 0 in fp32
 constexpr float FAR = 1048576.f;       // 2^20: a maximum with an r of this magnitude or more is treated apart
+constexpr float FARTHER = 16777216.f;  // 2^24: from here on sums are against the maximum itself
 
 using u64 = unsigned long long;
 
@@ -173,25 +176,42 @@ __device__ __forceinline__ float candidate_value(u64 c) {
 }
 __device__ __forceinline__ int candidate_index(u64 c) { return (int)~(uint32_t)c; }
 
-struct Sums { float m, s, w; };        // s and w against r = m c, from FAR on against m itself
+struct Sums { float m, s, w; };        // s and w against r = m c, from FARTHER on against m itself
 // The exponent of the maximum itself: what r = m c rounded leaves of it.
 __device__ __forceinline__ float residue(float m, float c) {
   const float r = __fmul_rn(m, c);
-  return fabsf(r) < FAR ? fmaf(m, c, -r) : 0.f;
+  return fabsf(r) < FARTHER ? fmaf(m, c, -r) : 0.f;
 }
-// log2 of the factor that takes sums of a maximum `a` to a larger one, `m`; ra and r are their references.
-__device__ __forceinline__ float shift(float a, float ra, float m, float r, float c) {
-  if (a == m) return 0.f;
-  const float d = fmaxf(fabsf(r), fabsf(ra)) < FAR ? ra - r : (a - m) * c - residue(a, c) + residue(m, c);
-  return fmaxf(d, FLOOR);
+// log2 of the factor that takes sums of a maximum `a` to a larger one, `m`: the second form holds for any maxima, the
+// first where |r| is below FAR.
+__device__ __forceinline__ float shift(float a, float ra, float m, float r) {
+  return a == m ? 0.f : fmaxf(ra - r, FLOOR);
 }
-__device__ __forceinline__ void join(Sums& a, const Sums& b, float c) {
-  const float m = max_nan(a.m, b.m), r = __fmul_rn(m, c);
-  const float da = shift(a.m, __fmul_rn(a.m, c), m, r, c), db = shift(b.m, __fmul_rn(b.m, c), m, r, c);
-  const float fa = exp2_fast(da), fb = exp2_fast(db);
-  a.w = fa * (a.w + da * a.s) + fb * (b.w + db * b.s);
-  a.s = fa * a.s + fb * b.s;
+__device__ __forceinline__ float shift_far(float a, float m, float c) {
+  return a == m ? 0.f : fmaxf((a - m) * c - residue(a, c) + residue(m, c), FLOOR);
+}
+// Sums against another maximum, at least their own.
+__device__ __forceinline__ void carry(Sums& a, float m, float c) {
+  const float r = __fmul_rn(m, c);
+  // lanes without a share (m = -inf) take the short way: they do not keep the others waiting
+  const float d = fabsf(r) < FAR || m == -INFINITY ? shift(a.m, __fmul_rn(a.m, c), m, r) : shift_far(a.m, m, c);
+  const float f = exp2_fast(d);
+  a.w = f * (a.w + d * a.s);
+  a.s *= f;
   a.m = m;
+}
+// The sums of LANES neighbouring lanes together, in each of them: the maximum first, then one shift for each lane.
+template <int LANES>
+__device__ __forceinline__ void join_lanes(Sums& a, float c) {
+  float m = a.m;
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  carry(a, m, c);
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) {
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+    a.w += __shfl_xor_sync(0xffffffffu, a.w, o);
+  }
 }
 
 struct Params {
@@ -335,12 +355,16 @@ __global__ void __launch_bounds__(TH, 1024 / TH) forward_kernel(const __grid_con
       note = (batch & ((1 << group) - 1)) ? max_nan(note, mx) : mx;
     }
     mx = max_nan(mx, m);
-    const float now = __fmul_rn(mx, c), d = shift(m, r, mx, now, c), f = exp2_fast(d);
-    w2 = fmul2(ffma2(make_float2(d, d), s2, w2), make_float2(f, f));
-    s2 = fmul2(s2, make_float2(f, f));
-    m = mx;
-    r = now;
-    if (fabsf(r) < FAR) {
+    const float now = __fmul_rn(mx, c);
+    auto raise = [&](float d) {                                  // the sums so far to the new maximum
+      const float f = exp2_fast(d);
+      w2 = fmul2(ffma2(make_float2(d, d), s2, w2), make_float2(f, f));
+      s2 = fmul2(s2, make_float2(f, f));
+      m = mx;
+      r = now;
+    };
+    if (fabsf(now) < FAR) {
+      raise(shift(m, r, mx, now));
       const float2 neg = make_float2(-r, -r);
 #pragma unroll
       for (int j = 0; j < UNROLL; ++j) {
@@ -355,15 +379,22 @@ __global__ void __launch_bounds__(TH, 1024 / TH) forward_kernel(const __grid_con
           w2 = ffma2(u, x, w2);
         }
       }
-    } else if (fabsf(m) < INFINITY) {
+    } else {
+      raise(shift_far(m, mx, c));
+      if (fabsf(m) < INFINITY) {
+        const float rest = residue(m, c);
 #pragma unroll
-      for (int j = 0; j < UNROLL; ++j) {
-        float z8[N];
-        Vec<T>::unpack(raw[j], z8);
-        for (int e = 0; e < N; ++e) {
-          const float u = fmaxf((z8[e] - m) * c, FLOOR), x = exp2_fast(u);
-          s2.x += x;
-          w2.x = fmaf(u, x, w2.x);
+        for (int j = 0; j < UNROLL; ++j) {
+          float z8[N];
+          Vec<T>::unpack(raw[j], z8);
+#pragma unroll 1
+          for (int k = 0; k < N; ++k) {            // one element a turn: code that is hardly ever run stays small
+            const float u = fmaxf(fmaf(z8[0] - m, c, rest), FLOOR), x = exp2_fast(u);
+            s2.x += x;
+            w2.x = fmaf(u, x, w2.x);
+#pragma unroll
+            for (int e = 0; e + 1 < N; ++e) z8[e] = z8[e + 1];
+          }
         }
       }
     }
@@ -385,30 +416,23 @@ __global__ void __launch_bounds__(TH, 1024 / TH) forward_kernel(const __grid_con
   if (tid < extra0 + extra1) {
     extra = Vec<T>::load(z + extra_at);
     const float u = residue(extra, c), x = exp2_fast(u);       // NaN and +inf are found by the maximum
-    if (extra != -INFINITY) join(st, Sums{extra, x, u * x}, c);
+    if (extra != -INFINITY) {
+      Sums end{extra, x, u * x};
+      const float m = max_nan(st.m, extra);
+      carry(st, m, c);
+      carry(end, m, c);
+      st.s += end.s;
+      st.w += end.w;
+    }
   }
 
   // one triple per CTA
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Sums b;
-    b.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-    b.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-    b.w = __shfl_xor_sync(0xffffffffu, st.w, o);
-    join(st, b, c);
-  }
+  join_lanes<32>(st, c);
   if (lane == 0) warp_sums[warp] = st;
   __syncthreads();
   if (warp == 0) {
     Sums t = lane < TH / 32 ? warp_sums[lane] : Sums{-INFINITY, 0.f, 0.f};
-#pragma unroll
-    for (int o = TH / 64; o > 0; o >>= 1) {
-      Sums b;
-      b.m = __shfl_xor_sync(0xffffffffu, t.m, o);
-      b.s = __shfl_xor_sync(0xffffffffu, t.s, o);
-      b.w = __shfl_xor_sync(0xffffffffu, t.w, o);
-      join(t, b, c);
-    }
+    join_lanes<TH / 32>(t, c);
     if (lane == 0) cta_sums = t;
   }
   if (TOPK) {
@@ -517,14 +541,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) forward_kernel(const __grid_con
     if (rank == 0) {
       if (warp == 0) {
         Sums t = lane < p.cluster ? *cl.map_shared_rank(&cta_sums, lane) : Sums{-INFINITY, 0.f, 0.f};
-#pragma unroll
-        for (int o = MAX_CLUSTER / 2; o > 0; o >>= 1) {
-          Sums b;
-          b.m = __shfl_xor_sync(0xffffffffu, t.m, o);
-          b.s = __shfl_xor_sync(0xffffffffu, t.s, o);
-          b.w = __shfl_xor_sync(0xffffffffu, t.w, o);
-          join(t, b, c);
-        }
+        join_lanes<MAX_CLUSTER>(t, c);
         if (lane == 0) warp_sums[0] = t;
       }
       if (TOPK) {
