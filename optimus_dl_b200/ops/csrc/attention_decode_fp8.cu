@@ -23,8 +23,10 @@
 // * q is scaled by a power of two per head so that its largest element lies in [2^14, 2^15): f16 then holds a bf16 or
 //   fp16 q exactly down to 2^-28 of that.  The softmax runs against a reference that follows the maximum only when a
 //   score exceeds it by more than 2^8, so most units need no reduction across lanes and no rescaling.  Probabilities
-//   are held as p 2^7 s_v / r in f16, r being the largest value scale met so far: at most 2^15, normal down to 2^-21 of
-//   the reference.  Scores, references, sums and both accumulators are fp32.
+//   are held as p s_v 2^7 in f16 against a reference of their own, which follows the largest p s_v of the head in the same
+//   way: at most 2^15, normal down to 2^-21 of the reference and nothing below 2^-32.  (Against the largest s_v alone, a
+//   block with 2^31 times the scale of the others hid them even where its own p was nothing.)  Scores, references, sums
+//   and both accumulators are fp32.
 // * Work is cut evenly, not by sequence: units of 16 tokens of one (sequence, kv head, group of query heads) are
 //   numbered through the batch, every CTA takes an equal run of them and every warp an equal part of that.  A warp
 //   that sees all units of a segment writes its output; parts are joined first inside the CTA through shared memory
@@ -49,7 +51,7 @@ constexpr int THREADS = WARPS * 32;
 constexpr int UNIT = 16;                 // tokens
 constexpr int MAX_BATCH = 2048;          // sequences per launch (their lengths are held in shared memory)
 constexpr float LAZY = 8.f;              // log2 of how far a score may exceed the reference
-constexpr float P_SCALE = 128.f;         // 2^7: probabilities up to 2^8 stay below 2^15 in f16
+constexpr float P_SCALE = 7.f;           // log2 of what p s_v is held times: up to 2^8 it stays below 2^15 in f16
 constexpr int COMBINE_GROUPS = 8;
 
 struct Params {
@@ -332,10 +334,10 @@ __global__ void __launch_bounds__(THREADS, CTAS<HD, NT>) decode_kernel(const __g
     }
 
     float acc[NT][KS][4];
-    float m[NT][2], l[NT][2], r = 0.f, inv_r = 0.f;
+    float m[NT][2], l[NT][2], r[NT][2];        // reference of p (log2), sums of p, reference of p s_v 2^-7
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m[nt][0] = m[nt][1] = -INFINITY;
+      m[nt][0] = m[nt][1] = r[nt][0] = r[nt][1] = -INFINITY;
       l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
       for (int j = 0; j < KS; ++j) acc[nt][j][0] = acc[nt][j][1] = acc[nt][j][2] = acc[nt][j][3] = 0.f;
@@ -356,8 +358,9 @@ __global__ void __launch_bounds__(THREADS, CTAS<HD, NT>) decode_kernel(const __g
       }
       const float ks_now = ks, vs_now = vs;
       if (un + 1 < u1) fetch_k(un + 1);
-      // scores in log2 units; the reference moves only if one exceeds it by more than LAZY
-      bool high = vs_now > r;
+      // scores in log2 units; the references move only if one exceeds them by more than LAZY
+      const float lift = (float)((int)(__float_as_uint(vs_now) >> 23) - 127);        // log2 of the value scale
+      bool high = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const float f0 = f_scale[nt][0] * ks_now, f1 = f_scale[nt][1] * ks_now;
@@ -366,15 +369,10 @@ __global__ void __launch_bounds__(THREADS, CTAS<HD, NT>) decode_kernel(const __g
           if (tk + g < first || tk + g >= len) s[nt][0] = s[nt][1] = -INFINITY;
           if (tk + g + 8 < first || tk + g + 8 >= len) s[nt][2] = s[nt][3] = -INFINITY;
         }
-        high |= fmaxf(s[nt][0], s[nt][2]) > m[nt][0] + LAZY || fmaxf(s[nt][1], s[nt][3]) > m[nt][1] + LAZY;
+        high |= fmaxf(s[nt][0], s[nt][2]) - m[nt][0] > fminf(LAZY, r[nt][0] - (lift - P_SCALE - LAZY)) ||
+                fmaxf(s[nt][1], s[nt][3]) - m[nt][1] > fminf(LAZY, r[nt][1] - (lift - P_SCALE - LAZY));
       }
       if (__any_sync(0xffffffffu, high)) {
-        float drop = 1.f;                // of the value reference, if this block's scale is larger
-        if (vs_now > r) {
-          drop = r * inverse_pow2(vs_now);
-          r = vs_now;
-          inv_r = inverse_pow2(vs_now);
-        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float m0 = fmaxf(s[nt][0], s[nt][2]), m1 = fmaxf(s[nt][1], s[nt][3]);
@@ -383,22 +381,24 @@ __global__ void __launch_bounds__(THREADS, CTAS<HD, NT>) decode_kernel(const __g
             m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
             m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
           }
-          m0 = fmaxf(m0, m[nt][0]);
-          m1 = fmaxf(m1, m[nt][1]);
-          // -inf only while every score was -inf: nothing to scale then
-          const float a0 = m0 == m[nt][0] ? 1.f : exp2_fast(m[nt][0] - m0), a1 = m1 == m[nt][1] ? 1.f : exp2_fast(m[nt][1] - m1);
-          m[nt][0] = m0;
-          m[nt][1] = m1;
-          l[nt][0] *= a0;
-          l[nt][1] *= a1;
-          const float d0 = a0 * drop, d1 = a1 * drop;
+          const float n0 = fmaxf(m0, m[nt][0]), n1 = fmaxf(m1, m[nt][1]);
+          // both references are -inf only while every score was -inf: nothing to scale then
+          const float e0 = n0 == m[nt][0] ? 0.f : m[nt][0] - n0, e1 = n1 == m[nt][1] ? 0.f : m[nt][1] - n1;
+          const float was0 = r[nt][0] + e0, was1 = r[nt][1] + e1;
+          const float r0 = fmaxf(was0, m0 - n0 + (lift - P_SCALE)), r1 = fmaxf(was1, m1 - n1 + (lift - P_SCALE));
+          const float d0 = r0 == was0 ? 1.f : exp2_fast(was0 - r0), d1 = r1 == was1 ? 1.f : exp2_fast(was1 - r1);
+          l[nt][0] *= exp2_fast(e0);
+          l[nt][1] *= exp2_fast(e1);
+          m[nt][0] = n0;
+          m[nt][1] = n1;
+          r[nt][0] = r0;
+          r[nt][1] = r1;
 #pragma unroll
           for (int j = 0; j < KS; ++j) {
             acc[nt][j][0] *= d0; acc[nt][j][1] *= d1; acc[nt][j][2] *= d0; acc[nt][j][3] *= d1;
           }
         }
       }
-      const float w = vs_now * inv_r * P_SCALE;
       uint32_t pf[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -407,8 +407,11 @@ __global__ void __launch_bounds__(THREADS, CTAS<HD, NT>) decode_kernel(const __g
         const float p2 = exp2_fast(s[nt][2] - b0), p3 = exp2_fast(s[nt][3] - b1);
         l[nt][0] += p0 + p2;
         l[nt][1] += p1 + p3;
-        pf[nt][0] = transpose8(pack_half2(p0 * w, p1 * w));
-        pf[nt][1] = transpose8(pack_half2(p2 * w, p3 * w));
+        // s_v 2^7 against the second reference; as a number even where p is 0
+        const float w0 = exp2_fast(fminf(lift - r[nt][0], 120.f));
+        const float w1 = exp2_fast(fminf(lift - r[nt][1], 120.f));
+        pf[nt][0] = transpose8(pack_half2(p0 * w0, p1 * w1));
+        pf[nt][1] = transpose8(pack_half2(p2 * w0, p3 * w1));
       }
 #pragma unroll
       for (int i = 0; i < VW; ++i) {
@@ -437,13 +440,13 @@ __global__ void __launch_bounds__(THREADS, CTAS<HD, NT>) decode_kernel(const __g
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         const int h = nt * 8 + 2 * t + c;
-        const float inv = sum == 0.f ? 0.f : 1.f / sum * (1.f / P_SCALE);
+        const float inv = sum == 0.f ? 0.f : 1.f / sum, back = exp2_fast(r[nt][c]);
 #pragma unroll
         for (int i = 0; i < VW; ++i) {
           // words 4 and up of a 256-wide head lie 128 dimensions on
           const int d = (i >> 2) * 128 + g * VCB + (i & 3) * 4;
-          const float x0 = acc[nt][2 * i][c] * inv * r, x1 = acc[nt][2 * i][c + 2] * inv * r;
-          const float x2 = acc[nt][2 * i + 1][c] * inv * r, x3 = acc[nt][2 * i + 1][c + 2] * inv * r;
+          const float x0 = acc[nt][2 * i][c] * inv * back, x1 = acc[nt][2 * i][c + 2] * inv * back;
+          const float x2 = acc[nt][2 * i + 1][c] * inv * back, x3 = acc[nt][2 * i + 1][c + 2] * inv * back;
           if (!complete) {
             *reinterpret_cast<float4*>(&part.o[h][d]) = make_float4(x0, x1, x2, x3);
           } else if (h < heads) {

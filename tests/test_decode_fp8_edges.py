@@ -1,9 +1,9 @@
 """The 8-bit cache at its edges: layouts, ranges of scales, windows, what is refused and what must stay as it was.
 
-Codes and scales have to be equal to the PyTorch statement's. Attention is compared with the definition in 64 bits.
-Probabilities times value scales are rounded to f16 relative to the largest such product met (half a step, 2^-12, for
-what lies above 2^-21 of it, else 2^-32 of it), exponentials and sums are fp32 (2^-20 and less): |error| <= 2^-11
-sum p |v| / sum p + 2^-32 * 448 max(p s_v) / sum p + half a step of |out|.
+Codes and scales have to be equal to the PyTorch statement's. Attention is compared with the definition in 64 bits. The
+kernel rounds p s_v (probability times value scale) to f16: by 2^-11 of itself at most while it is above 2^-21 of the
+largest of its head, and by 2^-32 of that largest one below; codes are at most 448. Exponentials, scores and sums of fp32
+add less than 2^-18. So |error| <= ((2^-11 + 2^-18) sum p |v| + n 2^-32 448 max(p s_v)) / sum p + half a step of |out|.
 """
 
 import math
@@ -14,6 +14,42 @@ import torch
 from optimus_dl_b200.ops import decode_fp8 as d8
 
 HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+def random_cache(B, capacity, Hk, hd, block, seed=0, device="cuda"):
+    g = torch.Generator().manual_seed(seed)
+    codes = [(torch.randn(B, Hk, capacity, hd, generator=g) * 60).clamp(-448, 448).to(torch.float8_e4m3fn).to(device)
+             for _ in range(2)]
+    nb = -(-capacity // block)
+    scales = [torch.exp2(torch.randint(-9, -4, (B, Hk, nb), generator=g).float()).to(device) for _ in range(2)]
+    return d8.Fp8KVCache(codes[0].permute(0, 2, 1, 3), codes[1].permute(0, 2, 1, 3), *scales, block)
+
+
+def check_attention(q, cache, lens, window=None, scale=None, out=None):
+    B, Hq, hd = q.shape
+    Hk = cache.k.shape[2]
+    c = 1 / math.sqrt(hd) if scale is None else scale
+    if out is None:
+        out = d8.decode_attention_fp8(q, None, None, cache, lens, window=window, scale=scale)
+    for b in range(B):
+        n = min(int(lens[b]), cache.k.shape[1])
+        first = max(0, n - window) if window else 0
+        if n <= 0:
+            assert not out[b].any()
+            continue
+        j = torch.arange(first, n, device=q.device) // cache.block
+        k = cache.k[b, first:n].double() * cache.k_scale[b][:, j].t()[..., None]
+        sv = cache.v_scale[b][:, j].double()                                             # [Hk, n]
+        v = cache.v[b, first:n].double() * sv.t()[..., None]
+        s = torch.einsum("hrd,thd->hrt", q[b].double().view(Hk, Hq // Hk, hd), k) * c
+        p = torch.softmax(s, -1)
+        want = torch.einsum("hrt,thd->hrd", p, v).reshape(Hq, hd)
+        size = torch.einsum("hrt,thd->hrd", p, v.abs()).reshape(Hq, hd)
+        most = (p * sv[:, None]).amax(-1).reshape(Hq, 1)
+        tol = (2.0 ** -11 + 2.0 ** -18) * size + (n - first) * 2.0 ** -32 * 448 * most + HALF_STEP[q.dtype] * want.abs()
+        err = (out[b].double() - want).abs() / (tol + torch.finfo(q.dtype).tiny)
+        assert bool((err <= 1).all()), (b, float(err.max()))
+    return out
 
 
 def same_cache(a, b):
@@ -65,3 +101,62 @@ def test_broadcast_rows_equal_their_contiguous_form(dtype):
             out = d8.decode_attention_fp8(q, k[:, 0], v[:, 0], a, lens + 1)
             assert torch.equal(out, d8.decode_attention_fp8(q, k[:, 0].contiguous(), v[:, 0].contiguous(), b, lens + 1))
             assert same_cache(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hd,Hq,Hk", [(32, 3, 1), (64, 2, 2), (128, 8, 2), (128, 12, 1), (256, 4, 2)])
+def test_a_block_of_large_values_and_no_probability_hides_nothing(hd, Hq, Hk, dtype):
+    """Blocks whose values are up to 2^60 times the others', with scores 60 below them (p = 2^-86), wherever they lie: the
+    result is that of the other blocks. And the other way round: p = 2^-14, but values that outweigh all others."""
+    torch.manual_seed(4)
+    B, capacity, block = 8, 12000, 16                  # several blocks a warp
+    lens = torch.tensor([12000, 33, 17, 9000, 64, 11650, 0, 5001], dtype=torch.int32, device="cuda")
+    q = torch.ones(B, Hq, hd, device="cuda").to(dtype) + 0.25 * torch.randn(B, Hq, hd, device="cuda").to(dtype)
+    step = math.sqrt(hd) / hd
+    for drop, ratio in ((60.0, 10), (60.0, 30), (60.0, 60), (10.0, 20), (10.0, 12)):
+        if dtype == torch.float16 and drop < 60:
+            ratio = min(ratio, 12)                     # results that this type holds
+        for first, every in ((0, 4), (1, 2), (2, 7), (0, 10 ** 6)):
+            cache = random_cache(B, capacity, Hk, hd, block)
+            cache.k.view(torch.uint8).copy_((torch.randn(B, capacity, Hk, hd, device="cuda") * 4).to(
+                torch.float8_e4m3fn).view(torch.uint8))
+            cache.k_scale.fill_(2.0 ** -6)
+            cache.v_scale.fill_(2.0 ** -8)
+            s = 2.0 ** (math.ceil(math.log2(drop * step)) - 8)
+            code = torch.full((), -drop * step / s, device="cuda").to(torch.float8_e4m3fn).view(torch.uint8)
+            large = torch.arange(capacity, device="cuda") // block % every == first
+            cache.k.view(torch.uint8).copy_(torch.where(large[:, None, None], code, cache.k.view(torch.uint8)))
+            cache.k_scale[:, :, first::every] = s
+            cache.v_scale[:, :, first::every] = 2.0 ** (ratio - 8)
+            check_attention(q, cache, lens)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,Hq,Hk,window", [(128, 8, 2, 1), (128, 20, 1, 37), (64, 3, 3, 64), (32, 6, 2, 100), (256, 2, 2, 16)])
+def test_tokens_before_the_window_are_not_looked_at(hd, Hq, Hk, window):
+    """NaN codes on both sides of what a sequence may see."""
+    torch.manual_seed(5)
+    lens = torch.tensor([0, 1, 16, 63, 64, 65, 300, 333], dtype=torch.int32, device="cuda")
+    cache = random_cache(8, 333, Hk, hd, 64)
+    at = torch.arange(333, device="cuda")
+    dead = (at >= lens[:, None]) | (at < lens[:, None] - window)
+    for c in (cache.k, cache.v):
+        c.view(torch.uint8).masked_fill_(dead[:, :, None, None], 0x7F)
+    q = torch.randn(8, Hq, hd, device="cuda").bfloat16()
+    check_attention(q, cache, lens, window=window)
+
+
+@pytest.mark.gpu
+def test_scores_beyond_fp32_leave_the_other_tokens():
+    """A unit of tokens whose every score is -inf in fp32 (so its probabilities are 0), then ordinary ones."""
+    cache = random_cache(2, 64, 1, 64, 16)
+    cache.k.view(torch.uint8)[:, :16] = 0xFE                     # -448
+    cache.k_scale[:, :, 0] = 2.0 ** 115
+    q = torch.full((2, 2, 64), 1000.0, device="cuda").bfloat16()
+    lens = torch.tensor([64, 16], dtype=torch.int32, device="cuda")
+    cache.k.view(torch.uint8)[:, 16:] = 0
+    out = d8.decode_attention_fp8(q, None, None, cache, lens)
+    want = (cache.v[0, 16:, 0].double() * cache.v_scale[0, 0, 1:].double().repeat_interleave(16)[:, None]).mean(0)
+    size = (cache.v[0, 16:, 0].double() * cache.v_scale[0, 0, 1:].double().repeat_interleave(16)[:, None]).abs().mean(0)
+    assert bool(((out[0].double() - want).abs() <= 2.0 ** -10 * size + 2.0 ** -8 * want.abs()).all())
