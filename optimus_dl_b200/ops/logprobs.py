@@ -63,30 +63,73 @@ def _check(rows_shape: torch.Size, vocab: int, floating: torch.Tensor, targets: 
         raise ValueError(f"temperature must be between 1e-6 and 1e6, got {temperature}")
 
 
+def _largest(z: torch.Tensor, k: int) -> torch.Tensor:
+    """Ids ``[rows, k]`` of the largest of ``z [rows, V]``: the largest first, equal ones by lowest id, NaN above all."""
+    if k == 1:
+        return z.argmax(-1, keepdim=True)          # the first of equal maxima
+    # sorting whole rows for this takes 20 times the rest of the statement; topk orders equal values as it likes
+    kth = torch.topk(z, k).values[:, -1:]
+    if bool(torch.isnan(kth).any()):
+        return torch.sort(z, dim=-1, descending=True, stable=True).indices[:, :k]
+    keep = ~(z < kth)                              # k of them, and what is equal to the last
+    more = (keep.sum(-1) > k).nonzero()[:, 0]
+    if len(more):
+        some, last = z[more], kth[more]
+        equal = some == last
+        above = keep[more] & ~equal
+        keep[more] = above | (equal & (equal.cumsum(-1) <= k - above.sum(-1, keepdim=True)))
+    ids = keep.nonzero()[:, 1].view(-1, k)
+    return ids.gather(-1, torch.sort(z.gather(-1, ids), dim=-1, descending=True, stable=True).indices)
+
+
 class _TokenLogprobsRef(torch.autograd.Function):
+    CHUNK = 1 << 20                                # logits taken at a time: what stays in a processor's cache
+
     @staticmethod
     def forward(ctx, logits, targets, top_k, temperature):
-        vocab = logits.shape[-1]
-        z = logits if logits.dtype == torch.float64 else logits.float()
-        top = z.amax(-1, keepdim=True)
-        none = top == -math.inf
-        u = (z - torch.where(none, 0.0, top)) / temperature
-        e = torch.exp(u)
-        total = torch.where(none, 1.0, e.sum(-1, keepdim=True))
-        log_p = u - torch.log(total)
-        entropy = torch.log(total) - torch.where(u == -math.inf, 0.0, u * e).sum(-1, keepdim=True) / total
-        inside = (targets >= 0) & (targets < vocab)
-        at = targets.long().clamp(0, vocab - 1).unsqueeze(-1)
-        logp = torch.where(inside, log_p.gather(-1, at).squeeze(-1), 0.0)
-        top_logp = top_ids = None
+        shape, vocab = targets.shape, logits.shape[-1]
+        wide = logits.dtype if logits.dtype == torch.float64 else torch.float32
+        z2, at = logits.reshape(-1, vocab), targets.reshape(-1).long()
+        rows = z2.shape[0]
+        inside = (at >= 0) & (at < vocab)
+        at = at.clamp(0, vocab - 1).unsqueeze(-1)
+        new = lambda *size, dtype=wide: torch.empty(size, dtype=dtype, device=logits.device)    # noqa: E731
+        results = [new(*shape), new(*shape)]           # no views of one another: they may be changed in place
         if top_k:
-            # stable: equal logits stay in the order of their ids; NaN sorts above everything
-            top_ids = torch.sort(z, dim=-1, descending=True, stable=True).indices[..., :top_k].contiguous()
-            top_logp = log_p.gather(-1, top_ids)
-        ctx.save_for_backward(log_p, entropy, inside & ~none.squeeze(-1), at)
+            results += [new(*shape, top_k), new(*shape, top_k, dtype=torch.int64)]
+        logp, entropy, *listed = [r.view(rows, *r.shape[len(shape):]) for r in results]
+        counts = new(rows, dtype=torch.bool)
+        kept = new(rows, vocab) if ctx.needs_input_grad[0] else None
+        step = max(1, _TokenLogprobsRef.CHUNK // vocab)
+        for r in range(0, rows, step):
+            part = slice(r, r + step)
+            z = z2[part].to(wide)
+            top = z.amax(-1, keepdim=True)
+            none = top == -math.inf
+            top = torch.where(none, 0.0, top)
+            u = z - top
+            if temperature != 1.0:
+                u.div_(temperature)
+            e = torch.exp(u)
+            total = torch.where(none, 1.0, e.sum(-1, keepdim=True))
+            log_total = torch.log(total)
+            if kept is not None:
+                torch.sub(u, log_total, out=kept[part])
+            # a banned token adds 0 and not -inf * 0
+            moment = e.mul_(u.clamp_(min=-1e6)).sum(-1, keepdim=True)
+            entropy[part] = (log_total - moment / total)[:, 0]
+            log_p = lambda ids: (z.gather(-1, ids) - top) / temperature - log_total             # noqa: E731
+            logp[part] = torch.where(inside[part], log_p(at[part])[:, 0], 0.0)
+            counts[part] = inside[part] & ~none[:, 0]
+            if top_k:
+                listed[1][part] = _largest(z, top_k)
+                listed[0][part] = log_p(listed[1][part])
+        if kept is not None:
+            ctx.save_for_backward(kept.view(logits.shape), entropy.clone().view(*shape, 1), counts.view(shape),
+                                  at.view(*shape, 1))                        # what is kept is not shared
         ctx.dtype, ctx.temperature = logits.dtype, temperature
-        ctx.mark_non_differentiable(*(t for t in (top_logp, top_ids) if t is not None))
-        return logp, entropy.squeeze(-1).clone(), top_logp, top_ids      # what is kept is not shared
+        ctx.mark_non_differentiable(*results[2:])
+        return (*results, None, None)[:4]
 
     @staticmethod
     @torch.autograd.function.once_differentiable

@@ -129,6 +129,72 @@ def test_the_head_projection_runs_on_the_rows_own_device(monkeypatch):
     assert r.logp.shape == (6,) and inside == [[there], [there]]
 
 
+# ------------------------------------------------------------------------------------------------ the statement
+def by_sorting(z, k):
+    return torch.sort(z, dim=-1, descending=True, stable=True).indices[:, :k]
+
+
+@pytest.mark.parametrize("k", [1, 2, 5, 32])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.bfloat16])
+def test_the_statements_alternatives_are_those_of_a_stable_sort(dtype, k):
+    g = torch.Generator().manual_seed(k)
+    z = torch.randn(14, 3001, generator=g).to(dtype)
+    z[1] = 0.0
+    z[2] = (torch.arange(3001) % 5 == 0).to(dtype)
+    z[3, 2000:] = 9.0
+    z[4] = -math.inf
+    z[5, ::3] = -math.inf
+    z[6, 5:] = -math.inf
+    z[7, 2999], z[8, ::100] = math.nan, math.nan
+    z[9, 10], z[9, 20], z[9, 30] = math.inf, math.nan, math.inf
+    z[10] = math.nan
+    z[11, ::2] = -0.0
+    z[11, 1::2] = 0.0
+    z[12] = torch.finfo(dtype).min
+    r = lp.token_logprobs_ref(z, torch.zeros(14, dtype=torch.int64), top_k=k)
+    assert torch.equal(r.top_ids, by_sorting(z if dtype == torch.float64 else z.float(), k))
+    rows = [0, 1, 2, 3, 11]
+    want = torch.log_softmax(z[rows].double(), -1).gather(-1, r.top_ids[rows])
+    assert torch.allclose(r.top_logp[rows].double(), want, atol=1e-5)
+
+
+def test_the_statement_does_not_sort_rows_and_holds_no_copies_of_them(monkeypatch):
+    """What scoring on the CPU costs: parts of a batch at a time, and sorts of what is listed only."""
+    sizes, real = [], torch.sort
+    monkeypatch.setattr(torch, "sort", lambda t, *a, **kw: (sizes.append(t.shape[-1]), real(t, *a, **kw))[1])
+    monkeypatch.setattr(lp._TokenLogprobsRef, "CHUNK", 4000)
+    z = torch.randn(3, 7, 1501)
+    t = torch.randint(0, 1501, (3, 7))
+    for k in (1, 4):
+        r = lp.token_logprobs(z, t, top_k=k, temperature=0.7)
+        want = torch.log_softmax(z.double() / 0.7, -1)
+        assert torch.allclose(r.logp.double(), want.gather(-1, t[..., None])[..., 0], atol=1e-5)
+        assert torch.allclose(r.entropy.double(), -(want.exp() * want).sum(-1), atol=1e-5)
+        assert torch.equal(r.top_ids, z.topk(k, -1).indices)
+    assert not sizes or max(sizes) <= 4
+
+
+def test_the_statements_gradient_over_several_parts(monkeypatch):
+    monkeypatch.setattr(lp._TokenLogprobsRef, "CHUNK", 30)
+    z = torch.randn(2, 5, 11, dtype=torch.float64, requires_grad=True)
+    t = torch.randint(0, 11, (2, 5))
+    t[0, 1] = -100
+
+    def f(x):
+        r = lp.token_logprobs(x, t, temperature=0.8)
+        return (r.logp * torch.arange(10.0).view(2, 5)).sum() + (r.entropy ** 2).sum()
+
+    assert torch.autograd.gradcheck(f, (z,))
+    r = lp.token_logprobs(z, t)
+    with torch.no_grad():
+        z.mul_(2)                  # the gradient is of what was scored
+    g, = torch.autograd.grad(r.logp.sum(), z)
+    p = torch.softmax(z.detach() / 2, -1)
+    inside = (t >= 0)[..., None]
+    want = inside * (torch.nn.functional.one_hot(t.clamp(min=0), 11) - p)
+    assert torch.allclose(g, want)
+
+
 # ------------------------------------------------------------------------------------------------ ends of rows, GPU
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
