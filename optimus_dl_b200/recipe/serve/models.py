@@ -18,25 +18,20 @@ class _Sampling(BaseModel):
     top_p: float | None = Field(default=None, gt=0.0, le=1.0)
     stream: bool = False
 
-
     def alternatives(self) -> int | None:
         """Alternatives per token that the answer lists, None without log probabilities."""
         raise NotImplementedError
 
-    @model_validator(mode="after")
-    def _no_streamed_logprobs(self):
-        if self.stream and self.alternatives() is not None:
-            raise ValueError("log probabilities are not streamed: use stream=false")
-        return self
-
 
 class ChatCompletionRequest(_Sampling):
+    """Clients send ``logprobs`` as null and with streams as well: a stream is answered, without log probabilities."""
+
     messages: list[dict]
-    logprobs: bool = False
+    logprobs: bool | None = None
     top_logprobs: int | None = Field(default=None, ge=0, le=20)
 
     def alternatives(self) -> int | None:
-        return (self.top_logprobs or 0) if self.logprobs else None
+        return (self.top_logprobs or 0) if self.logprobs and not self.stream else None
 
 
 class CompletionRequest(_Sampling):
@@ -45,6 +40,12 @@ class CompletionRequest(_Sampling):
 
     def alternatives(self) -> int | None:
         return self.logprobs
+
+    @model_validator(mode="after")
+    def _no_streamed_logprobs(self):
+        if self.stream and self.logprobs is not None:
+            raise ValueError("log probabilities are not streamed: use stream=false")
+        return self
 
 
 class ChatMessage(BaseModel):

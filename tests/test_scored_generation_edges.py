@@ -1,0 +1,48 @@
+"""Scoring and the 8-bit cache as the framework's own paths use them: requests that were answered before they existed,
+tokens outside the vocabulary, heads that are scored without their logits."""
+
+import http.client
+import json
+import threading
+
+import pytest
+import torch
+
+from optimus_dl_b200.core import conf
+
+
+def _server():
+    from optimus_dl_b200.recipe.serve import ServeConfig, ServeRecipe
+
+    recipe = ServeRecipe(conf.merge(conf.create(ServeConfig()), conf.create({
+        "serve": {"host": "127.0.0.1", "port": 0},
+        "common": {"device": "cpu", "tokenizer": {"_name": "char_tokenize", "add_eos": False},
+                   "model": {"_name": "llama2", "n_layer": 1, "n_head": 2, "n_embd": 32, "vocab_size": 258,
+                             "sequence_length": 64, "intermediate_size": 64}}})))
+    recipe.setup()
+    httpd = recipe.make_server()
+    threading.Thread(target=httpd.serve_forever, daemon=True).start()
+    return httpd
+
+
+def test_chats_with_fields_that_were_ignored_before_are_still_answered():
+    httpd = _server()
+    msgs = [{"role": "user", "content": "hi"}]
+
+    def post(**fields):
+        c = http.client.HTTPConnection("127.0.0.1", httpd.server_address[1], timeout=60)
+        c.request("POST", "/v1/chat/completions", body=json.dumps({"messages": msgs, "max_tokens": 3, **fields}),
+                  headers={"Content-Type": "application/json"})
+        r = c.getresponse()
+        return r.status, r.read().decode()
+
+    try:
+        for fields in (dict(logprobs=None), dict(logprobs=None, top_logprobs=None), dict(logprobs=False, top_logprobs=3)):
+            status, body = post(**fields)
+            assert status == 200 and json.loads(body)["choices"][0]["logprobs"] is None
+        for fields in (dict(logprobs=None), dict(logprobs=False), dict(logprobs=True), dict(logprobs=True, top_logprobs=2)):
+            status, body = post(stream=True, **fields)
+            assert status == 200 and body.rstrip().endswith("[DONE]")
+    finally:
+        httpd.shutdown()
+        httpd.server_close()
