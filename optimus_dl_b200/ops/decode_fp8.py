@@ -217,6 +217,7 @@ def _append_one_ref(new: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor,
             at = stop
 
 
+@torch.no_grad()
 def append_kv_fp8_ref(k_new: torch.Tensor, v_new: torch.Tensor, cache: Fp8KVCache, seq_lens: torch.Tensor,
                       n_new: torch.Tensor | None = None) -> None:
     """PyTorch statement of :func:`append_kv_fp8`, block by block."""
@@ -287,6 +288,7 @@ def _workspace(B: int, Hq: int, Hk: int, hd: int, capacity: int) -> int:
     return _lib.lib().ob_attn_decode_fp8_workspace(B, Hq, Hk, hd, capacity)
 
 
+@torch.no_grad()
 def decode_attention_fp8_ref(q, k_new, v_new, cache: Fp8KVCache, seq_lens, *, scale=None, window=None) -> torch.Tensor:
     """PyTorch statement of :func:`decode_attention_fp8` in fp32 (fp64 for fp64 queries); also appends."""
     B, Hq, hd = q.shape

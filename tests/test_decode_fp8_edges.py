@@ -79,6 +79,15 @@ def test_broadcast_codes_and_scales_are_refused():
     d8.Fp8KVCache(one.k, one.v, torch.ones(2, 2, 1).expand(2, 2, 1), one.v_scale, 16)
 
 
+def test_neither_the_cache_nor_the_result_takes_part_in_a_gradient():
+    cache = d8.fp8_kv_cache(2, 40, 2, 32, block=16)
+    k, q = torch.randn(2, 3, 2, 32, requires_grad=True), torch.randn(2, 4, 32, requires_grad=True)
+    lens = torch.tensor([3, 3], dtype=torch.int32)
+    d8.append_kv_fp8(k, k, cache, lens)
+    out = d8.decode_attention_fp8(q, k[:, 0], k[:, 0], cache, lens + 1)
+    assert not any(t.requires_grad for t in (out, cache.k, cache.v, cache.k_scale, cache.v_scale))
+
+
 # ------------------------------------------------------------------------------------------------ GPU
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
