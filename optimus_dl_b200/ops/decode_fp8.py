@@ -50,7 +50,8 @@ def _strides(t: torch.Tensor) -> tuple[int, ...]:
 class Fp8KVCache:
     """``k``, ``v``: logical ``[B, capacity, Hk, hd]`` float8_e4m3fn with a unit stride in the last dimension and any
     others (a head-major allocation viewed this way reads fastest); ``k_scale``, ``v_scale``: fp32
-    ``[B, Hk, ceil(capacity / block)]`` with a unit stride in the blocks, powers of two; ``block``: tokens that share a scale (16, 32, 64 or 128)."""
+    ``[B, Hk, ceil(capacity / block)]`` with a unit stride in the blocks, powers of two (a cache that repeats a sequence
+    or a head by a stride of 0, or has keys and values in one place, can be attended over, not written); ``block``: tokens that share a scale (16, 32, 64 or 128)."""
 
     k: torch.Tensor
     v: torch.Tensor
@@ -84,9 +85,12 @@ class Fp8KVCache:
             geometry, status = (sb, st, sh, scale_strides[0], scale_strides[1]), _lib.status_word(dev)
         else:
             kernels, geometry, status = False, None, None
+        shared = (k.data_ptr() == v.data_ptr() or ks.data_ptr() == vs.data_ptr()) and k.numel() > 0
+        if 0 in strides or 0 in scale_strides:       # of a dimension of size 1, or of several elements in one place
+            shared = shared or any(n > 1 and s == 0 for n, s in (*zip(shape, strides), *zip(want, scale_strides)))
         # the status word exists before any capture into a graph
         self.__dict__.update(_device=dev, _index=k.get_device(), _shape=tuple(shape), _kernels=kernels, _geometry=geometry,
-                             _status=status)
+                             _status=status, _shared=shared)
 
     def _args(self) -> tuple:
         """What describes the cache to the kernels: codes and their strides, scales and theirs."""
@@ -114,6 +118,8 @@ def _check_new(k_new: torch.Tensor, v_new: torch.Tensor, cache: Fp8KVCache, want
         raise TypeError(f"new keys and values must share one of bf16, fp16, fp32: got {k_new.dtype}, {v_new.dtype}")
     if k_new.get_device() != cache._index or v_new.get_device() != cache._index:
         raise ValueError("new keys and values must be on the cache's device")
+    if cache._shared:
+        raise ValueError("sequences, tokens, heads or keys and values of this cache share memory: it can be read only")
 
 
 def _check_counts(t: torch.Tensor, cache: Fp8KVCache, batch: int, what: str) -> None:

@@ -88,6 +88,30 @@ def test_neither_the_cache_nor_the_result_takes_part_in_a_gradient():
     assert not any(t.requires_grad for t in (out, cache.k, cache.v, cache.k_scale, cache.v_scale))
 
 
+def test_caches_that_share_memory_are_read_only():
+    """Two sequences in one place would be written by two CTAs at once."""
+    a = d8.fp8_kv_cache(1, 40, 1, 32, block=16)
+    d8.append_kv_fp8(torch.randn(1, 40, 1, 32), torch.randn(1, 40, 1, 32), a, torch.tensor([40], dtype=torch.int32))
+    own = d8.fp8_kv_cache(3, 40, 2, 32, block=16)
+    shared = [d8.Fp8KVCache(a.k.expand(3, 40, 2, 32), a.v.expand(3, 40, 2, 32), a.k_scale.expand(3, 2, 3),
+                            a.v_scale.expand(3, 2, 3), 16),
+              d8.Fp8KVCache(own.k, own.v, a.k_scale.expand(3, 2, 3), a.v_scale.expand(3, 2, 3), 16),
+              d8.Fp8KVCache(own.k, own.k, own.k_scale, own.v_scale, 16),
+              d8.Fp8KVCache(own.k, own.v, own.k_scale, own.k_scale, 16)]
+    new, q = torch.randn(3, 2, 2, 32), torch.randn(3, 4, 32)
+    lens = torch.tensor([40, 17, 2], dtype=torch.int32)
+    for cache in shared:
+        with pytest.raises(ValueError, match="share memory"):
+            d8.append_kv_fp8(new, new, cache, lens)
+        with pytest.raises(ValueError, match="share memory"):
+            d8.decode_attention_fp8(q, new[:, 0], new[:, 0], cache, lens)
+        assert torch.isfinite(d8.decode_attention_fp8(q, None, None, cache, lens)).all()
+    one = d8.decode_attention_fp8(q[:1], None, None, d8.Fp8KVCache(a.k.expand(1, 40, 2, 32), a.v.expand(1, 40, 2, 32),
+                                                                   a.k_scale.expand(1, 2, 3), a.v_scale.expand(1, 2, 3), 16),
+                                  lens[:1])
+    assert torch.equal(d8.decode_attention_fp8(q, None, None, shared[0], lens)[:1], one)
+
+
 # ------------------------------------------------------------------------------------------------ GPU
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
