@@ -72,6 +72,8 @@ class Fp8KVCache:
                 or (k.stride() != v.stride() and strides != _strides(v))):
             raise ValueError("k and v must be [B, capacity, Hk, hd] of the same shape and strides, contiguous in hd")
         B, capacity, Hk, hd = shape
+        if capacity < 1 or Hk < 1 or hd < 1:
+            raise ValueError(f"a cache needs at least one token, head and dimension, got {tuple(shape)}")
         want = (B, Hk, -(-capacity // block))
         if (ks.shape != want or vs.shape != want or scale_strides[2] != (want[2] > 1)
                 or (ks.stride() != vs.stride() and scale_strides != _strides(vs))):
@@ -271,7 +273,11 @@ def decode_attention_fp8(q: torch.Tensor, k_new: torch.Tensor | None, v_new: tor
     if not (cache._kernels and has_kernel(hd, dtype)):
         return decode_attention_fp8_ref(q, k_new, v_new, cache, seq_lens, scale=scale, window=window)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    if B == 0 or Hq == 0:
+    if B == 0:
+        return out
+    if Hq == 0:
+        if k_new is not None:
+            append_kv_fp8(k_new[:, None], v_new[:, None], cache, seq_lens)
         return out
     q_batch, q_head, q_last = q.stride()
     if q_last != 1 or q_head != hd or (2 * q_batch | q.data_ptr()) & 15:

@@ -112,7 +112,37 @@ def test_caches_that_share_memory_are_read_only():
     assert torch.equal(d8.decode_attention_fp8(q, None, None, shared[0], lens)[:1], one)
 
 
+def test_caches_without_anything_in_them_are_refused_but_for_an_empty_batch():
+    for shape in ((2, 0, 2, 32), (2, 40, 0, 32), (2, 40, 2, 0)):
+        codes = torch.zeros(shape, dtype=torch.uint8).view(torch.float8_e4m3fn)
+        scales = torch.ones(shape[0], shape[2], -(-shape[1] // 16))
+        with pytest.raises(ValueError, match="at least one"):
+            d8.Fp8KVCache(codes, codes.clone(), scales, scales.clone(), 16)
+    codes, scales = torch.zeros(0, 40, 2, 32, dtype=torch.uint8).view(torch.float8_e4m3fn), torch.ones(0, 2, 3)
+    empty, none = d8.Fp8KVCache(codes, codes.clone(), scales, scales.clone(), 16), torch.zeros(0, dtype=torch.int32)
+    rows = torch.zeros(0, 2, 32)
+    assert d8.decode_attention_fp8(torch.zeros(0, 4, 32), rows, rows, empty, none).shape == (0, 4, 32)
+
+
+def _step_without_query_heads(device):
+    cache = d8.fp8_kv_cache(2, 40, 2, 32, block=16, device=device)
+    new = torch.ones(2, 2, 32, device=device).bfloat16()
+    lens = torch.tensor([1, 0], dtype=torch.int32, device=device)
+    out = d8.decode_attention_fp8(new[:, :0], new, new, cache, lens)
+    assert out.shape == (2, 0, 32)
+    assert bool((cache.k[0, 0].float() == 256).all()) and not cache.k[1].float().any()
+
+
+def test_a_step_without_query_heads_stores_its_token():
+    _step_without_query_heads("cpu")
+
+
 # ------------------------------------------------------------------------------------------------ GPU
+@pytest.mark.gpu
+def test_a_step_without_query_heads_stores_its_token_on_the_gpu():
+    _step_without_query_heads("cuda")
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 def test_broadcast_rows_equal_their_contiguous_form(dtype):
