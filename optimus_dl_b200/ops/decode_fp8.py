@@ -68,12 +68,12 @@ class Fp8KVCache:
         if ks.dtype != torch.float32 or vs.dtype != torch.float32:
             raise TypeError(f"scales must be float32, got {ks.dtype} and {vs.dtype}")
         shape, strides, scale_strides = k.shape, _strides(k), _strides(ks)
+        if len(shape) == 4 and min(shape[1:]) < 1:
+            raise ValueError(f"a cache needs at least one token, head and dimension, got {tuple(shape)}")
         if (len(shape) != 4 or shape != v.shape or strides[3] != (shape[3] > 1)
                 or (k.stride() != v.stride() and strides != _strides(v))):
             raise ValueError("k and v must be [B, capacity, Hk, hd] of the same shape and strides, contiguous in hd")
         B, capacity, Hk, hd = shape
-        if capacity < 1 or Hk < 1 or hd < 1:
-            raise ValueError(f"a cache needs at least one token, head and dimension, got {tuple(shape)}")
         want = (B, Hk, -(-capacity // block))
         if (ks.shape != want or vs.shape != want or scale_strides[2] != (want[2] > 1)
                 or (ks.stride() != vs.stride() and scale_strides != _strides(vs))):
