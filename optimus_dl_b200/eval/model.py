@@ -110,8 +110,9 @@ class LLMBaselinesModel(_LMBase):
                     wanted[j, a:b] = torch.tensor(targets, dtype=torch.long)
             seq_lens = torch.tensor([len(r) for r in rows], dtype=torch.long)
             logits = self.model(x.to(self._device), seq_lens=seq_lens.to(self._device))["logits"]
-            if wanted.numel() and int(wanted.max()) >= logits.shape[-1]:
-                raise IndexError(f"token {int(wanted.max())} is outside the model's vocabulary of {logits.shape[-1]}")
+            for t in (t for _, _, targets in spans for t in targets):
+                if not 0 <= t < logits.shape[-1]:
+                    raise IndexError(f"token {t} is outside the model's vocabulary of {logits.shape[-1]}")
             scored = token_logprobs(logits, wanted.to(logits.device), top_k=1)
             logp, best = scored.logp.cpu(), scored.top_ids[..., 0].cpu()
             for j, i in enumerate(idx):

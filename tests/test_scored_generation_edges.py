@@ -46,3 +46,19 @@ def test_chats_with_fields_that_were_ignored_before_are_still_answered():
     finally:
         httpd.shutdown()
         httpd.server_close()
+
+
+def _model(**kw):
+    from optimus_dl_b200.models.llama2 import Llama, LlamaConfig
+
+    torch.manual_seed(0)
+    base = dict(n_layer=2, n_head=4, n_kv_head=2, n_embd=64, vocab_size=97, sequence_length=48, intermediate_size=128)
+    return Llama(LlamaConfig(**{**base, **kw}))
+
+
+@pytest.mark.parametrize("token", [-1, -100, 97, 1 << 40])
+def test_scored_tokens_outside_the_vocabulary_are_refused(token):
+    from optimus_dl_b200.eval.model import LLMBaselinesModel
+
+    with pytest.raises(IndexError):
+        LLMBaselinesModel(_model(), None)._score([([1, 2], [3]), ([1, 2], [5, token])])
