@@ -2,20 +2,23 @@
 (optimus_dl/modules/eval/model.py:14-242).
 
 Implements the harness's three request kinds. ``loglikelihood`` and ``loglikelihood_rolling`` score
-with one forward per *batch* of requests (right-padded, the padded positions are masked out of the
-sums); ``generate_until`` decodes greedily with the KV cache and stops at the first stop string.
+with one forward per *batch* of requests (right-padded; logits are formed for the continuations' positions
+only, a part at a time); ``generate_until`` decodes greedily with the KV cache and stops at the first stop string.
 The class derives from ``lm_eval.api.model.LM`` when the harness is installed and is a plain object
 otherwise, so it can be unit-tested without it.
 """
 
 from __future__ import annotations
 
+import inspect
 import logging
 from typing import Any
 
 import torch
 
-from ..ops.logprobs import token_logprobs
+from ..models.gpt2 import GPT
+from ..ops.linear import fp8_route
+from ..ops.logprobs import linear_token_logprobs, token_logprobs
 from ..recipe.generation import generate_stream, unwrap
 
 logger = logging.getLogger(__name__)
@@ -30,6 +33,18 @@ except Exception:  # noqa: BLE001
 
 def _args(request: Any) -> tuple:
     return tuple(request.args) if hasattr(request, "args") else tuple(request)
+
+
+def _plain_head(model: torch.nn.Module) -> torch.Tensor | None:
+    """The weight of a head that is one product of whole hidden states, so that only the rows to be scored need logits;
+    None for other models (sharded, tensor-parallel, in 8 bits, with a head or forward pass of their own)."""
+    root = unwrap(model)
+    weight = getattr(getattr(root, "lm_head", None), "weight", None)
+    if (getattr(type(root), "head", None) is not GPT.head or "skip_lm_head" not in inspect.signature(root.forward).parameters
+            or getattr(root, "_tp", None) is not None or getattr(root, "_sharding_engine", None) is not None
+            or fp8_route([weight])):
+        return None
+    return weight
 
 
 class LLMBaselinesModel(_LMBase):
@@ -109,12 +124,24 @@ class LLMBaselinesModel(_LMBase):
                 if b > a:
                     wanted[j, a:b] = torch.tensor(targets, dtype=torch.long)
             seq_lens = torch.tensor([len(r) for r in rows], dtype=torch.long)
-            logits = self.model(x.to(self._device), seq_lens=seq_lens.to(self._device))["logits"]
+            x, seq_lens = x.to(self._device), seq_lens.to(self._device)
+            head = _plain_head(self.model)
+            if head is not None:
+                out_of, vocab = self.model(x, seq_lens=seq_lens, skip_lm_head=True)["hidden"], head.shape[0]
+            else:
+                out_of = self.model(x, seq_lens=seq_lens)["logits"]
+                vocab = out_of.shape[-1]
             for t in (t for _, _, targets in spans for t in targets):
-                if not 0 <= t < logits.shape[-1]:
-                    raise IndexError(f"token {t} is outside the model's vocabulary of {logits.shape[-1]}")
-            scored = token_logprobs(logits, wanted.to(logits.device), top_k=1)
-            logp, best = scored.logp.cpu(), scored.top_ids[..., 0].cpu()
+                if not 0 <= t < vocab:
+                    raise IndexError(f"token {t} is outside the model's vocabulary of {vocab}")
+            some = wanted >= 0
+            rows, targets = out_of[some.to(out_of.device)], wanted[some].to(out_of.device)
+            if head is not None:
+                scored = linear_token_logprobs(rows, head, targets, top_k=1)
+            else:
+                scored = token_logprobs(rows, targets, top_k=1)
+            logp, best = torch.zeros(wanted.shape, dtype=scored.logp.dtype), torch.full(wanted.shape, -1)
+            logp[some], best[some] = scored.logp.cpu(), scored.top_ids[:, 0].cpu()
             for j, i in enumerate(idx):
                 a, b, _ = spans[j]
                 if b <= a:

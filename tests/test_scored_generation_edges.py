@@ -62,3 +62,45 @@ def test_scored_tokens_outside_the_vocabulary_are_refused(token):
 
     with pytest.raises(IndexError):
         LLMBaselinesModel(_model(), None)._score([([1, 2], [3]), ([1, 2], [5, token])])
+
+
+def _scores(model, device="cpu"):
+    from optimus_dl_b200.eval.model import LLMBaselinesModel
+
+    g = torch.Generator().manual_seed(2)
+    ids = lambda n: torch.randint(0, 97, (n,), generator=g).tolist()                             # noqa: E731
+    pairs = [(ids(5), ids(3)), (ids(1), ids(40)), (ids(60), ids(2)), (ids(3), []), (ids(2), ids(1)), (ids(30), ids(60))]
+    return LLMBaselinesModel(model, None, device=device, batch_size=4)._score(pairs)
+
+
+def _check_scores(device, dtype, tol, **kw):
+    """Scores without all logits, against those of a model whose forward pass forms them."""
+    from optimus_dl_b200.models.llama2 import Llama
+
+    class Whole(Llama):
+        def head(self, x):
+            return super().head(x)
+
+    class Scored(Llama):
+        def forward(self, *a, skip_lm_head=False, **kw):
+            assert skip_lm_head, "logits of all positions"
+            return super().forward(*a, skip_lm_head=True, **kw)
+
+    model = _model(**kw).to(device, dtype)
+    got = []
+    for cls in (Scored, Whole):
+        model.__class__ = cls
+        got.append(_scores(model, device))
+    for (a, ga), (b, gb) in zip(*got):
+        assert abs(a - b) <= tol * (1 + abs(b)) and (ga == gb or dtype != torch.float32)
+    assert got[0][3] == (0.0, True)
+
+
+def test_scoring_forms_the_logits_of_scored_positions_only():
+    _check_scores("cpu", torch.float32, 1e-5)
+
+
+@pytest.mark.gpu
+def test_scoring_forms_the_logits_of_scored_positions_only_on_the_gpu():
+    """A logit may be rounded to the neighbouring bf16 number, 2^-8 of it; logits here are below 4."""
+    _check_scores("cuda", torch.bfloat16, 2.0 ** -6, n_embd=256, n_kv_head=4)
