@@ -18,7 +18,7 @@
 // * So every thread consumes exactly the bytes it asked for, and codes go straight from global memory to registers with
 //   16-byte loads. The keys of the next unit of 16 tokens are loaded behind the first product of the current one, the
 //   values behind its second; 16 warps on an SM with 2 to 4 KB each under way cover the latency (4 sequences of up to
-//   131072 tokens, 40 / 8 heads of 128: 114 us for 671 MB, 0.90 of the measured copy bandwidth). The same bytes through
+//   131072 tokens, 40 / 8 heads of 128: 116 us for 671 MB, 0.89 of the measured copy bandwidth). The same bytes through
 //   a two-stage cp.async ring in shared memory took 168 us: its reads add a second latency to every unit's chain.
 // * q is scaled by a power of two per head so that its largest element lies in [2^14, 2^15): f16 then holds a bf16 or
 //   fp16 q exactly down to 2^-28 of that.  The softmax runs against a reference that follows the maximum only when a
@@ -44,8 +44,9 @@ namespace decode_fp8 {
 using namespace kvfp8;
 
 constexpr int WARPS = 8;
-// CTAs per SM, as many as the registers of a warp's accumulators allow.  Measured at HD 128, 4 sequences of up to 131072
-// tokens: 2 x 8 warps 121 us, 1 x 12 129 us, 2 x 6 130 us; at HD 64, 128 of up to 1024: 3 x 8 36 us, 2 x 8 39 us.
+// CTAs per SM, as many as the registers of a warp's accumulators allow; at HD 64 one more, whose 80 registers spill 44
+// bytes (52 loaded again) and which is faster all the same.  Measured at HD 128, 4 sequences of up to 131072 tokens:
+// 2 x 8 warps 121 us, 1 x 12 129 us, 2 x 6 130 us; at HD 64, 128 of up to 1024: 3 x 8 36 us, 2 x 8 39 us.
 template <int HD, int NT> constexpr int CTAS = NT > 1 || HD > 128 ? 1 : HD > 64 ? 2 : 3;
 constexpr int THREADS = WARPS * 32;
 constexpr int UNIT = 16;                 // tokens
@@ -521,6 +522,7 @@ __global__ void __launch_bounds__(THREADS, CTAS<HD, NT>) decode_kernel(const __g
 }
 
 // Joins the parts of a segment that starts in CTA blockIdx.x and goes on in the CTAs behind it; one head per CTA here.
+// At HD 32 the compiler spills 4 bytes at 32 registers.
 template <int HD, int NH, typename T>
 __global__ void __launch_bounds__(COMBINE_GROUPS * 32) combine_kernel(const __grid_constant__ Params p) {
   constexpr int PER = HD / 32;

@@ -97,8 +97,8 @@ class GRPORecipe(TrainingIterationMixin):
     @torch.no_grad()
     def rollout_scored(self, model: torch.nn.Module, prompts: torch.Tensor, step: int,
                        with_logprobs: bool = True) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
-        """:meth:`rollout`, with the log probabilities ``[P * G, n]`` the completions were sampled under (at
-        temperature 1, from the decode steps' logits) as a third part."""
+        """:meth:`rollout`, with the completions' log probabilities ``[P * G, n]`` from the decode steps' logits as a third
+        part: at temperature 1 and before top-k and top-p, whatever the sampler's are."""
         g = self.cfg.grpo
         eng = getattr(unwrap(model), "_sharding_engine", None)
         if eng is not None:

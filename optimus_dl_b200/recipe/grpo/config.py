@@ -47,8 +47,9 @@ class GRPOSection:
     use_kv_cache: bool = True
     use_cuda_graph: bool = True
     kv_cache_dtype: str | None = None   # "fp8": rollouts read an 8-bit cache (half its memory and traffic)
-    rollout_logprobs: bool = False      # sampling-time log probabilities from the decode steps' own logits (with an
-                                        # 8-bit cache: of the distribution that was sampled) instead of a forward pass
+    rollout_logprobs: bool = False      # log probabilities from the decode steps' own logits (of the 8-bit cache, where
+                                        # that is used) instead of a forward pass; at temperature 1 without top_k and
+                                        # top_p, as the update's: of what was sampled only where the sampler is that too
     reward: Any = field(default_factory=lambda: {"_name": "even_fraction"})
     prompts: Any = field(default_factory=lambda: {"_name": "uniform_random"})
 
