@@ -44,8 +44,8 @@ namespace decode_fp8 {
 using namespace kvfp8;
 
 constexpr int WARPS = 8;
-// CTAs per SM, as many as the registers of a warp's accumulators allow; at HD 64 one more, whose 80 registers spill 44
-// bytes (52 loaded again) and which is faster all the same.  Measured at HD 128, 4 sequences of up to 131072 tokens:
+// CTAs per SM, as many as the registers of a warp's accumulators allow; at HD 64 one more, whose 80 registers spill 48
+// bytes (60 loaded again) and which is faster all the same.  Measured at HD 128, 4 sequences of up to 131072 tokens:
 // 2 x 8 warps 121 us, 1 x 12 129 us, 2 x 6 130 us; at HD 64, 128 of up to 1024: 3 x 8 36 us, 2 x 8 39 us.
 template <int HD, int NT> constexpr int CTAS = NT > 1 || HD > 128 ? 1 : HD > 64 ? 2 : 3;
 constexpr int THREADS = WARPS * 32;
@@ -77,6 +77,21 @@ struct Slot {                            // one part of one segment: normalised 
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float log2_fast(float x) {
+  float r;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
@@ -360,7 +375,7 @@ __global__ void __launch_bounds__(THREADS, CTAS<HD, NT>) decode_kernel(const __g
       const float ks_now = ks, vs_now = vs;
       if (un + 1 < u1) fetch_k(un + 1);
       // scores in log2 units; the references move only if one exceeds them by more than LAZY
-      const float lift = (float)((int)(__float_as_uint(vs_now) >> 23) - 127);        // log2 of the value scale
+      const float lift = max_nan(log2_fast(vs_now), -127.f);       // of the value scale; NaN where that is none
       bool high = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -409,8 +424,8 @@ __global__ void __launch_bounds__(THREADS, CTAS<HD, NT>) decode_kernel(const __g
         l[nt][0] += p0 + p2;
         l[nt][1] += p1 + p3;
         // s_v 2^7 against the second reference; as a number even where p is 0
-        const float w0 = exp2_fast(fminf(lift - r[nt][0], 120.f));
-        const float w1 = exp2_fast(fminf(lift - r[nt][1], 120.f));
+        const float w0 = exp2_fast(min_nan(lift - r[nt][0], 120.f));
+        const float w1 = exp2_fast(min_nan(lift - r[nt][1], 120.f));
         pf[nt][0] = transpose8(pack_half2(p0 * w0, p1 * w1));
         pf[nt][1] = transpose8(pack_half2(p2 * w0, p3 * w1));
       }

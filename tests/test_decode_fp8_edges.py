@@ -223,3 +223,23 @@ def test_scores_beyond_fp32_leave_the_other_tokens():
     want = (cache.v[0, 16:, 0].double() * cache.v_scale[0, 0, 1:].double().repeat_interleave(16)[:, None]).mean(0)
     size = (cache.v[0, 16:, 0].double() * cache.v_scale[0, 0, 1:].double().repeat_interleave(16)[:, None]).abs().mean(0)
     assert bool(((out[0].double() - want).abs() <= 2.0 ** -10 * size + 2.0 ** -8 * want.abs()).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+def test_value_scales_that_are_no_number_show_and_zeros_count_nothing(hd):
+    torch.manual_seed(6)
+    cache = random_cache(4, 200, 2, hd, 16)
+    lens = torch.tensor([200, 100, 200, 200], dtype=torch.int32, device="cuda")
+    cache.v_scale[0, 1, 3] = math.nan
+    cache.v_scale[1, 0, 7:] = math.nan              # tokens 112 and on: not seen
+    cache.v_scale[2, :, 1::2] = 0.0
+    cache.v_scale[3] = 0.0
+    q = torch.randn(4, 6, hd, device="cuda").bfloat16()
+    out = d8.decode_attention_fp8(q, None, None, cache, lens)
+    assert torch.isnan(out[0, 3:]).all() and torch.isfinite(out[0, :3]).all() and torch.isfinite(out[1:]).all()
+    assert float(out[3].abs().max()) < 1e-30
+    cache.v_scale[0, 1, 3] = 1.0
+    cache.v_scale[1, 0, 7:] = 1.0
+    cache.v_scale[3] = 1.0
+    check_attention(q, cache, lens)
