@@ -243,3 +243,57 @@ def test_value_scales_that_are_no_number_show_and_zeros_count_nothing(hd):
     cache.v_scale[1, 0, 7:] = 1.0
     cache.v_scale[3] = 1.0
     check_attention(q, cache, lens)
+
+
+@pytest.mark.gpu
+def test_captured_appends_replay_with_other_counts():
+    B, T, Hk, hd = 5, 9, 2, 64
+    k, v = (torch.empty(B, T, Hk, hd, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    lens, n = (torch.zeros(B, dtype=torch.int32, device="cuda") for _ in range(2))
+    a, b = (d8.fp8_kv_cache(B, 100, Hk, hd, block=16, device="cuda") for _ in range(2))
+    d8.append_kv_fp8(k, v, a, lens, n)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        d8.append_kv_fp8(k, v, a, lens, n)
+    g = torch.Generator().manual_seed(0)
+    for step in range(8):
+        more = torch.randint(0, T + 1, (B,), generator=g).int()
+        n.copy_(more)
+        lens.add_(n)
+        k.normal_().mul_(1 + step)
+        v.normal_()
+        graph.replay()
+        d8.append_kv_fp8_ref(k, v, b, lens, n)
+        assert same_cache(a, b)
+
+
+@pytest.mark.gpu
+def test_two_threads_step_over_caches_of_their_own():
+    import threading
+
+    def work(seed):
+        g = torch.Generator().manual_seed(seed)
+        cache = random_cache(3, 400, 2, 128, 64, seed)
+        lens = torch.tensor([100, 0, 300], dtype=torch.int32, device="cuda")
+        out = []
+        for _ in range(20):
+            q, kn, vn = (torch.randn(3, h, 128, generator=g).bfloat16().cuda() for h in (8, 2, 2))
+            lens = lens + (lens > 0).int()
+            out.append(d8.decode_attention_fp8(q, kn, vn, cache, lens))
+        return torch.stack(out)
+
+    want = [work(s) for s in (1, 2)]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got[i] = work(i + 1)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -293,3 +293,78 @@ def test_gradients_of_banned_tokens_under_large_weights(dtype, temperature, g_h)
     _, grad = check(z, t, temperature, d_logp, d_h)
     banned = (z == -math.inf) & (torch.arange(4099) != t[:, None])
     assert not grad.cpu()[banned].any()
+
+
+# ------------------------------------------------------------------------------------------------ calls at once, replays
+@pytest.mark.gpu
+def test_two_threads_on_streams_of_their_own():
+    import threading
+
+    def work(seed, dtype):
+        g = torch.Generator().manual_seed(seed)
+        z = (torch.randn(70, 20011, generator=g) * 3).to(dtype).cuda().requires_grad_(True)
+        t = torch.randint(0, 20011, (70,), generator=g).cuda()
+        r = lp.token_logprobs(z, t, top_k=7)
+        grad, = torch.autograd.grad(r.logp.sum() + 0.1 * r.entropy.sum(), z)
+        return r.logp.detach(), r.entropy.detach(), r.top_ids, grad
+
+    jobs = [(1, torch.bfloat16), (2, torch.float32)]
+    want = [work(*j) for j in jobs]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                got[i] = work(*jobs[i])
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+
+
+@pytest.mark.gpu
+def test_forward_and_gradient_captured_and_replayed_with_other_logits():
+    rows, vocab = 33, 5003
+    z = torch.empty(rows, vocab, device="cuda", dtype=torch.bfloat16)
+    t = torch.randint(0, vocab, (rows,), device="cuda")
+    ones = torch.ones(rows, device="cuda")
+
+    def step(logits):
+        x = logits.detach().requires_grad_(True)
+        r = lp.token_logprobs(x, t)
+        return r.logp.detach(), r.entropy.detach(), torch.autograd.grad([r.logp, r.entropy], [x], [ones, -ones])[0]
+
+    z.normal_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(z)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(z)
+    for scale in (1.0, 30.0, 1e10):
+        z.normal_().mul_(scale)
+        t.random_(0, vocab)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(out, step(z)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab,chunk", [(1, 50257, 4096), (5, 1003, 2), (65, 33001, 64), (129, 4096, 4096)])
+def test_few_and_many_rows_over_a_head(rows, vocab, chunk):
+    """Logits are bf16 products; a product of 128 terms in fp32 may round to the neighbouring one."""
+    torch.manual_seed(rows)
+    x, w = torch.randn(rows, 128, device="cuda").bfloat16(), (torch.randn(vocab, 128, device="cuda") * 0.1).bfloat16()
+    t = torch.randint(0, vocab, (rows,), device="cuda")
+    r = lp.linear_token_logprobs(x, w, t, top_k=3, chunk_rows=chunk)
+    z = x.double() @ w.double().t()
+    want = torch.log_softmax(z, -1)
+    tol = 2 * 2.0 ** -8 * float(z.abs().max()) + 1e-4
+    assert float((r.logp.double() - want.gather(-1, t[:, None])[:, 0]).abs().max()) <= tol
+    assert float((r.top_logp.double() - want.topk(3).values).abs().max()) <= tol
