@@ -68,7 +68,7 @@ class Fp8KVCache:
         if ks.dtype != torch.float32 or vs.dtype != torch.float32:
             raise TypeError(f"scales must be float32, got {ks.dtype} and {vs.dtype}")
         shape, strides, scale_strides = k.shape, _strides(k), _strides(ks)
-        if len(shape) == 4 and min(shape[1:]) < 1:
+        if 0 in shape[1:]:
             raise ValueError(f"a cache needs at least one token, head and dimension, got {tuple(shape)}")
         if (len(shape) != 4 or shape != v.shape or strides[3] != (shape[3] > 1)
                 or (k.stride() != v.stride() and strides != _strides(v))):
@@ -81,13 +81,14 @@ class Fp8KVCache:
         dev = k.device
         if v.device != dev or ks.device != dev or vs.device != dev:
             raise ValueError("codes and scales must be on one device")
+        codes_k, codes_v = k.data_ptr(), v.data_ptr()
         if dev.type == "cuda":
             sb, st, sh, _ = strides
-            kernels = hd in _HEAD_DIMS and not (sb | st | sh | k.data_ptr() | v.data_ptr()) & 15
+            kernels = hd in _HEAD_DIMS and not (sb | st | sh | codes_k | codes_v) & 15
             geometry, status = (sb, st, sh, scale_strides[0], scale_strides[1]), _lib.status_word(dev)
         else:
             kernels, geometry, status = False, None, None
-        shared = (k.data_ptr() == v.data_ptr() or ks.data_ptr() == vs.data_ptr()) and k.numel() > 0
+        shared = (codes_k == codes_v or ks.data_ptr() == vs.data_ptr()) and k.numel() > 0
         if 0 in strides or 0 in scale_strides:       # of a dimension of size 1, or of several elements in one place
             shared = shared or any(n > 1 and s == 0 for n, s in (*zip(shape, strides), *zip(want, scale_strides)))
         # the status word exists before any capture into a graph
